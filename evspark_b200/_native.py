@@ -57,8 +57,19 @@ class DrafterConfig(C.Structure):
                                           "vocab_size", "mask_id", "ctx_window", "mlp_mult")]
 
 
+class Q4CacheDesc(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("err", C.c_void_p), ("num_pages", C.c_int64), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class Q4RowsDesc(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("lengths", C.c_void_p), ("counts", C.c_void_p), ("table_stride", C.c_int64),
+                ("max_pages", C.c_int32), ("batch", C.c_int32), ("tokens", C.c_int32)]
+
+
 _P = C.c_void_p
 _I = C.c_int
+_L = C.c_int64
 _PROTOS = {
     "evs_version": (_I, []),
     "evs_last_error": (C.c_char_p, []),
@@ -90,6 +101,13 @@ _PROTOS = {
     "evs_sample": (_I, [_P, _I, _I, _P, _P, _P]),
     "evs_gemm_bf16": (_I, [_P, _P, _P, _I, _I, _I, _I, _P]),
     "evs_gemm_bf16_noalloc": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "evs_q4_quantize": (_I, [_P, _I, _L, _I, _I, _I, _P, _P, _P]),
+    "evs_q4_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _I, _L, _P]),
+    "evs_q4_linear": (_I, [_P, _I, _L, _I, _P, _P, _I, _I, _I, _P, _I, _L, _P]),
+    "evs_q4_kv_append": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, C.c_double, _P]),
+    "evs_q4_kv_read": (_I, [_P, _P, _P, _P, _P, _P, _I, _P]),
+    "evs_q4_attention_workspace": (_L, [_P, _P, _I, _I]),
+    "evs_q4_attention": (_I, [_P, _P, _P, _P, _I, C.c_float, _I, _P, _P, _I, _P, _L, _P]),
     "evs_drafter_create": (_I, [C.POINTER(DrafterConfig), _I, C.POINTER(_P)]),
     "evs_drafter_set_tensor": (_I, [_P, _I, _P, C.c_int64]),
     "evs_drafter_finalize": (_I, [_P]),

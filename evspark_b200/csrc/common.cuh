@@ -28,6 +28,8 @@ enum EvsKernelId {
   EVS_K_VERIFY = 5,
   EVS_K_DRAFT = 6,
   EVS_K_ROW = 7,
+  EVS_K_Q4_CACHE = 8,
+  EVS_K_Q4_ATTN = 9,
 };
 
 __device__ __forceinline__ void evs_record_error(EvsDevErr* e, int code, int where, int info) {

@@ -1,0 +1,48 @@
+// Device views of the paged 4-bit KV cache, shared by q4_cache.cu and q4_attention.cu.
+#pragma once
+
+#include "common.cuh"
+
+struct Q4CacheDev {
+  uint8_t* pool;
+  EvsDevErr* err;
+  int64_t pages;
+  int P, G, D;
+  int block_bytes;  // one page of one head
+  __host__ __device__ uint8_t* block(int64_t page, int head) const {
+    return pool + (static_cast<size_t>(page) * G + head) * block_bytes;
+  }
+};
+
+struct Q4RowsDev {
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* counts;  // null: every row has T new tokens
+  int64_t table_stride;
+  int max_pages, B, T;
+};
+
+// a [B, T, heads, D] tensor: strides in elements, D contiguous
+struct Q4Tensor {
+  void* p;
+  int64_t sb, st, sh;
+};
+
+// row b's length and its new tokens; false when they lie outside the page table's positions or T
+__device__ __forceinline__ bool q4_row(const Q4RowsDev& r, int b, int* len, int* count, int P) {
+  *len = r.lengths[b];
+  *count = r.counts != nullptr ? r.counts[b] : r.T;
+  return *len >= 0 && *count >= 0 && *count <= r.T &&
+         static_cast<int64_t>(*len) + *count <= static_cast<int64_t>(r.max_pages) * P;
+}
+
+// page of position pos (inside the table), or -1 when the table's entry is no page of the pool
+__device__ __forceinline__ int64_t q4_page(const Q4CacheDev& c, const Q4RowsDev& r, int b, int64_t pos) {
+  const int32_t id = __ldg(r.table + b * r.table_stride + pos / c.P);
+  return id >= 0 && id < c.pages ? id : -1;
+}
+
+int q4_check_cache(const evs_q4_cache* c);
+int q4_check_rows(const evs_q4_cache* c, const evs_q4_rows* r);
+Q4CacheDev q4_cache_dev(const evs_q4_cache* c);
+Q4RowsDev q4_rows_dev(const evs_q4_rows* r);

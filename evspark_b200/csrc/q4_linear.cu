@@ -1,0 +1,358 @@
+// Tokens times a weight held in 4 bits: y[m][n] = sum_k x[m][k] (c[n][k] - 8) s[k / group][n].
+//
+//   codes  uint8 [N][Kp / 2], two input features per byte (even one in the low half), Kp = K rounded
+//          up to 128 with codes of 8 (zeros) behind K
+//   scales bf16 [Kp / group][N]
+#include <algorithm>
+
+#include "internal.hpp"
+#include "q4.cuh"
+
+namespace {
+
+constexpr int LIN_WARPS = 8;
+constexpr int LIN_THREADS = 32 * LIN_WARPS;
+constexpr int LIN_ROWS = 128;     // weight rows per CTA: four warps of 32 rows
+constexpr int LIN_KW = 2;         // warps that share a row tile and take every other K block
+constexpr int LIN_TOKENS = 64;    // tokens per CTA at most
+constexpr int LIN_CLUSTER = 8;    // CTAs of one output tile at most (splits of K)
+
+// x staged in shared memory in the order in which the products read it: per (K block, 8-token
+// tile, part) four 16-byte words per lane; lane (n, c) word w holds features 32 c + 8 w .. + 7 of
+// token n as pairs (0,4) (1,5) (2,6) (3,7), the order in which q4_word decodes a weight word.
+__device__ __forceinline__ uint4 pair_up(uint4 v) {
+  return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                    __byte_perm(v.y, v.w, 0x7632));
+}
+
+template <typename TX>
+__device__ __forceinline__ void stage_x(uint4* xs, const TX* __restrict__ x, int64_t ldx, int M, int K, int m0, int NT,
+                                        int kb0, int nkb, bool vec) {
+  constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
+  const int units = nkb * NT * 8 * 16;  // (token, 8 features)
+  for (int i = threadIdx.x; i < units; i += LIN_THREADS) {
+    const int u = i & 15, n = (i >> 4) % (8 * NT), kb = (i >> 4) / (8 * NT);
+    const int k = (kb0 + kb) * Q4_KBLOCK + 8 * u;
+    const int c = u >> 2, w = u & 3;
+    uint4* dst = xs + ((static_cast<size_t>(kb) * NT + (n >> 3)) * NP * 4 + w) * 32 + (n & 7) * 4 + c;
+    const bool row = m0 + n < M;
+    const TX* src = x + static_cast<int64_t>(m0 + n) * ldx + k;
+    if constexpr (NP == 1) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row && vec && k + 8 <= K) {
+        v = *reinterpret_cast<const uint4*>(src);
+      } else if (row) {
+        uint32_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = k + j < K ? __bfloat16_as_ushort(src[j]) : 0u;
+        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+      }
+      *dst = pair_up(v);
+    } else {
+      uint32_t p[8][3];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q4_parts(row && k + j < K ? src[j] : 0.f, p[j]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        dst[q * 4 * 32] = make_uint4(p[0][q] | p[4][q] << 16, p[1][q] | p[5][q] << 16, p[2][q] | p[6][q] << 16,
+                                     p[3][q] | p[7][q] << 16);
+    }
+  }
+}
+
+struct LinTile {  // one warp's share of a K block: 32 rows x 128 features
+  uint4 w[4];     // rows g, g + 8, g + 16, g + 24, features 32 c .. 32 c + 31
+  uint32_t s[4];
+};
+
+__device__ __forceinline__ void load_tile(LinTile& t, const uint8_t* const (&row)[4], const uint16_t* sc, int N, int r0,
+                                          int group, int kb, int c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4* p = reinterpret_cast<const uint4*>(row[i] + static_cast<size_t>(kb) * (Q4_KBLOCK / 2));
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(t.w[i].x), "=r"(t.w[i].y), "=r"(t.w[i].z), "=r"(t.w[i].w)
+                 : "l"(p));
+  }
+  const int gi = (kb * Q4_KBLOCK + 32 * c) / group;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t.s[i] = __ldg(sc + static_cast<size_t>(gi) * N + min(r0 + 8 * i, N - 1));
+}
+
+// grid (K splits = cluster, row tiles, token tiles)
+template <typename TX, typename TO, int NT>
+__global__ void __launch_bounds__(LIN_THREADS)
+    q4_linear_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint8_t* __restrict__ codes,
+                     const uint16_t* __restrict__ scales, int N, int K, int group, TO* __restrict__ out, int64_t ldo,
+                     int chunk_kb, int vec) {
+  constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
+  extern __shared__ __align__(16) unsigned char lin_sm[];
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int wr = warp & 3, wk = warp >> 2;
+  const int S = gridDim.x, rank = blockIdx.x;
+  const int n0 = blockIdx.y * LIN_ROWS, m0 = blockIdx.z * LIN_TOKENS;
+  const int KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
+  const int kb_begin = static_cast<int>(static_cast<int64_t>(KB) * rank / S);
+  const int kb_end = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / S);
+  const int r0 = n0 + 32 * wr + g;
+  const size_t row_bytes = static_cast<size_t>(KB) * (Q4_KBLOCK / 2);
+  const uint8_t* row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) row[i] = codes + static_cast<size_t>(min(r0 + 8 * i, N - 1)) * row_bytes + 16 * c;
+
+  float acc[2][NT][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+
+  uint4* xs = reinterpret_cast<uint4*>(lin_sm);
+  pdl_wait();
+  for (int kc = kb_begin; kc < kb_end; kc += chunk_kb) {
+    const int nkb = min(chunk_kb, kb_end - kc);
+    __syncthreads();
+    stage_x<TX>(xs, x, ldx, M, K, m0, NT, kc, nkb, vec != 0);
+    __syncthreads();
+    for (int kb = wk; kb < nkb; kb += LIN_KW) {
+      LinTile t;
+      load_tile(t, row, scales, N, r0, group, kc + kb, c);
+      Q4Scale s[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = q4_scale(t.s[i] | t.s[i] << 16);
+      const uint4* xb = xs + static_cast<size_t>(kb) * NT * NP * 4 * 32 + lane;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t a[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q4_word((&t.w[i].x)[w], s[i], a[i]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int q = NP - 1; q >= 0; --q) {
+            const uint4 b = xb[((j * NP + q) * 4 + w) * 32];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              q4_mma(acc[i][j], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1], b.x, b.y);
+              q4_mma(acc[i][j], a[2 * i][2], a[2 * i + 1][2], a[2 * i][3], a[2 * i + 1][3], b.z, b.w);
+            }
+          }
+      }
+    }
+  }
+  // sums over the two K warps and the cluster's splits, in that order: red[wk][token][row]
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(lin_sm);
+  constexpr int RL = LIN_ROWS + 4;
+  constexpr int TOK = 8 * NT;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(wk * TOK + 8 * j + 2 * c + (e & 1)) * RL + 32 * wr + 16 * i + g + 8 * (e >> 1)] = acc[i][j][e];
+  if (S > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  const int tokens = min(TOK, M - m0);
+  for (int i = rank * LIN_THREADS + threadIdx.x; i < tokens * LIN_ROWS; i += S * LIN_THREADS) {
+    const int tok = i / LIN_ROWS, r = i % LIN_ROWS;
+    if (n0 + r >= N) continue;
+    float sum = 0.f;
+    for (int p = 0; p < S; ++p) {
+      uint32_t a;
+      float v0, v1;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(red + tok * RL + r)), "r"(p));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v0) : "r"(a) : "memory");
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v1) : "r"(a + TOK * RL * 4) : "memory");
+      sum += v0 + v1;
+    }
+    out[static_cast<int64_t>(m0 + tok) * ldo + n0 + r] = from_f32<TO>(sum);
+  }
+  // no CTA of the cluster leaves while another still reads its sums
+  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename TX, typename TO, int NT>
+int launch_linear_nt(const void* x, int64_t ldx, int M, const void* codes, const void* scales, int N, int K, int group,
+                     void* out, int64_t ldo, cudaStream_t st, bool pdl) {
+  constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
+  const int tiles = (N + LIN_ROWS - 1) / LIN_ROWS, KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
+  // splits of K from N and K alone, so that a token's sums do not depend on the other tokens
+  int S = 1;
+  while (S < LIN_CLUSTER && tiles * S < 296 && KB / (2 * S) >= 4) S *= 2;
+  const int block_bytes = NT * NP * 2048;  // staged x of one K block
+  const int slice = (KB + S - 1) / S;
+  // an even number of blocks, so that the two K warps take the same blocks at every chunk size
+  int chunk = std::max(2, 49152 / block_bytes) & ~1;
+  chunk = std::min(chunk, slice);
+  const int smem = std::max(chunk * block_bytes, 2 * 8 * NT * (LIN_ROWS + 4) * 4);
+  auto* kern = q4_linear_kernel<TX, TO, NT>;
+  static std::atomic<unsigned long long> done{0};
+  EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), 200 * 1024));
+  const int vec = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(TX)) % 16 == 0) ? 1 : 0;
+  const int ztiles = (M + LIN_TOKENS - 1) / LIN_TOKENS;
+  EVS_CHECK_ARG(tiles <= 65535 && ztiles <= 65535, "q4 linear: too many rows or tokens");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(S, tiles, ztiles);
+  cfg.blockDim = dim3(LIN_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  EVS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<const TX*>(x), ldx, M, static_cast<const uint8_t*>(codes),
+                                  static_cast<const uint16_t*>(scales), N, K, group, static_cast<TO*>(out), ldo, chunk,
+                                  vec));
+  evs_count_launch(1);
+  return EVS_OK;
+}
+
+template <typename TX, typename TO>
+int launch_linear_t(const void* x, int64_t ldx, int M, const void* codes, const void* scales, int N, int K, int group,
+                    void* out, int64_t ldo, cudaStream_t st, bool pdl) {
+  if (M <= 8) return launch_linear_nt<TX, TO, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  if (M <= 16) return launch_linear_nt<TX, TO, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  if (M <= 32) return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  return launch_linear_nt<TX, TO, 8>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+}
+
+// one warp per (row, group): codes and scale of the group's features (K padded with zeros)
+template <typename TW>
+__global__ void q4_quantize_kernel(const TW* __restrict__ w, int64_t ldw, int N, int K, int group,
+                                   uint8_t* __restrict__ codes, uint16_t* __restrict__ scales) {
+  const int groups = (K + Q4_KBLOCK - 1) / Q4_KBLOCK * Q4_KBLOCK / group;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
+  if (i >= static_cast<int64_t>(N) * groups) return;
+  const int n = static_cast<int>(i / groups), gi = static_cast<int>(i % groups), lane = threadIdx.x & 31;
+  const int per = group / 32;  // 1, 2 or 4 features a lane
+  float v[4];
+  float m = 0.f;
+  bool bad = false;
+  for (int j = 0; j < per; ++j) {
+    const int k = gi * group + lane * per + j;
+    v[j] = k < K ? to_f32<TW>(w[static_cast<int64_t>(n) * ldw + k]) : 0.f;
+    bad |= !(fabsf(v[j]) <= 3.4e38f);
+    m = fmaxf(m, fabsf(v[j]));
+  }
+  m = warp_max(m);
+  const uint32_t s = __any_sync(0xffffffffu, bad) ? 0x7FC0u : q4_scale_bits(static_cast<double>(m));
+  uint32_t c[4];
+  for (int j = 0; j < per; ++j) c[j] = q4_code(static_cast<double>(v[j]), s);
+  uint8_t* dst = codes + static_cast<size_t>(n) * (groups * static_cast<size_t>(group) / 2) + static_cast<size_t>(gi) * (group / 2);
+  if (per == 1) {
+    const uint32_t other = __shfl_down_sync(0xffffffffu, c[0], 1);
+    if ((lane & 1) == 0) dst[lane / 2] = static_cast<uint8_t>(c[0] | other << 4);
+  } else {
+    for (int j = 0; j < per; j += 2) dst[(lane * per + j) / 2] = static_cast<uint8_t>(c[j] | c[j + 1] << 4);
+  }
+  if (lane == 0) scales[static_cast<size_t>(gi) * N + n] = static_cast<uint16_t>(s);
+}
+
+// one thread per byte: two values of a row
+template <typename TO>
+__global__ void q4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, int N, int K,
+                                     int group, TO* __restrict__ out, int64_t ldo) {
+  const int n = blockIdx.y;
+  const size_t row_bytes = static_cast<size_t>((K + Q4_KBLOCK - 1) / Q4_KBLOCK) * (Q4_KBLOCK / 2);
+  const int j = blockIdx.x * blockDim.x + threadIdx.x;
+  const int k = 2 * j;
+  if (k >= K) return;
+  for (int r = n; r < N; r += gridDim.y) {
+    const uint32_t b = codes[r * row_bytes + j];
+    const float s = __uint_as_float(static_cast<uint32_t>(scales[static_cast<size_t>(k / group) * N + r]) << 16);
+    out[r * ldo + k] = from_f32<TO>((static_cast<int>(b & 15u) - 8) * s);
+    if (k + 1 < K) out[r * ldo + k + 1] = from_f32<TO>((static_cast<int>(b >> 4) - 8) * s);
+  }
+}
+
+int check_weight(const void* codes, const void* scales, int N, int K, int group) {
+  EVS_CHECK_ARG(codes && scales, "null argument");
+  EVS_CHECK_ARG(N >= 1 && K >= 1 && K <= (1 << 24), "q4 weight: N and K must be at least 1 (K at most 2^24)");
+  EVS_CHECK_ARG(group == 32 || group == 64 || group == 128, "q4 weight: group must be 32, 64 or 128");
+  EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "q4 weight: codes must be 16-byte aligned");
+  EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(scales) % 2 == 0, "q4 weight: scales must be 2-byte aligned");
+  return EVS_OK;
+}
+
+}  // namespace
+
+int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
+                     int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl) {
+  if (x_dtype == EVS_DTYPE_BF16) {
+    if (out_dtype == EVS_DTYPE_BF16)
+      return launch_linear_t<__nv_bfloat16, __nv_bfloat16>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+    return launch_linear_t<__nv_bfloat16, float>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  }
+  if (out_dtype == EVS_DTYPE_BF16)
+    return launch_linear_t<float, __nv_bfloat16>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  return launch_linear_t<float, float>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+}
+
+extern "C" {
+
+int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
+                  int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st) {
+  EVS_CHECK_ARG(x && out, "null argument");
+  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_CHECK_ARG(x_dtype == EVS_DTYPE_BF16 || x_dtype == EVS_DTYPE_FP32, "q4 linear: x must be fp32 or bf16");
+  EVS_CHECK_ARG(out_dtype == EVS_DTYPE_BF16 || out_dtype == EVS_DTYPE_FP32, "q4 linear: out must be fp32 or bf16");
+  EVS_CHECK_ARG(M >= 1 && ldx >= K && ldo >= N, "q4 linear: needs M >= 1, ldx >= K and ldo >= N");
+  const size_t xa = x_dtype == EVS_DTYPE_BF16 ? 2 : 4, oa = out_dtype == EVS_DTYPE_BF16 ? 2 : 4;
+  EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(x) % xa == 0 && reinterpret_cast<uintptr_t>(out) % oa == 0,
+                "q4 linear: misaligned pointer");
+  return launch_q4_linear(x, x_dtype, ldx, M, codes, scales, N, K, group, out, out_dtype, ldo, st, false);
+}
+
+int evs_q4_quantize(const void* w, int dtype, int64_t ldw, int N, int K, int group, void* codes, void* scales,
+                    cudaStream_t st) {
+  EVS_CHECK_ARG(w != nullptr, "null argument");
+  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 quantize: w must be fp32 or bf16");
+  EVS_CHECK_ARG(ldw >= K, "q4 quantize: needs ldw >= K");
+  const int64_t groups = static_cast<int64_t>(N) * ((K + Q4_KBLOCK - 1) / Q4_KBLOCK * Q4_KBLOCK / group);
+  const int64_t blocks = (groups + 7) / 8;
+  EVS_CHECK_ARG(blocks <= INT32_MAX, "q4 quantize: too many groups");
+  if (dtype == EVS_DTYPE_BF16)
+    q4_quantize_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(w), ldw, N, K, group, static_cast<uint8_t*>(codes), static_cast<uint16_t*>(scales));
+  else
+    q4_quantize_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, st>>>(
+        static_cast<const float*>(w), ldw, N, K, group, static_cast<uint8_t*>(codes), static_cast<uint16_t*>(scales));
+  EVS_CUDA_TRY(cudaGetLastError());
+  evs_count_launch(1);
+  return EVS_OK;
+}
+
+int evs_q4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
+                      int64_t ldo, cudaStream_t st) {
+  EVS_CHECK_ARG(out != nullptr, "null argument");
+  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_CHECK_ARG(out_dtype == EVS_DTYPE_BF16 || out_dtype == EVS_DTYPE_FP32, "q4 dequantize: out must be fp32 or bf16");
+  EVS_CHECK_ARG(ldo >= K, "q4 dequantize: needs ldo >= K");
+  dim3 grid(((K + 1) / 2 + 255) / 256, std::min(N, 65535));
+  if (out_dtype == EVS_DTYPE_BF16)
+    q4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes),
+                                                              static_cast<const uint16_t*>(scales), N, K, group,
+                                                              static_cast<__nv_bfloat16*>(out), ldo);
+  else
+    q4_dequantize_kernel<float><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes),
+                                                      static_cast<const uint16_t*>(scales), N, K, group,
+                                                      static_cast<float*>(out), ldo);
+  EVS_CUDA_TRY(cudaGetLastError());
+  evs_count_launch(1);
+  return EVS_OK;
+}
+
+}  // extern "C"

@@ -213,6 +213,72 @@ EVS_API int evs_gemm_bf16(const void* W, const void* X, float* out, int N, int K
 EVS_API int evs_gemm_bf16_noalloc(const void* W, const void* X, float* out, int N, int K, int M,
                                   cudaStream_t stream);
 
+/* ---- 4-bit weights and KV cache (no counterpart in the reference) ----
+ * Format: a group of values shares a bf16 scale s = absmax / 7 rounded to five significant bits; a
+ * code c in 1..15 stands for (c - 8) s, exact in bf16; codes come two per byte, the even value in
+ * the low half.  A group with absmax / 7 < 2^-120 is held as zeros; one with a NaN, an infinity or
+ * absmax / 7 > 2^120 is held as NaN.  Foreign weights and pools must keep the form (scales of at
+ * most five significant bits, not negative, at most 2^120); it is not checked.
+ *
+ * Weight [N, K]: codes uint8 [N, Kp / 2] with Kp = K rounded up to 128 (code 8 behind K), 16-byte
+ * aligned; scales bf16 [Kp / group, N]; group 32, 64 or 128 input features. */
+/* w [N, K] (fp32 or bf16, row stride ldw elements) -> codes, scales */
+EVS_API int evs_q4_quantize(const void* w, int dtype, int64_t ldw, int N, int K, int group, void* codes, void* scales,
+                            cudaStream_t stream);
+EVS_API int evs_q4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
+                              int64_t ldo, cudaStream_t stream);
+/* out[m][n] = sum_k x[m][k] w[n][k], sums in fp32; x [M, K] and out [M, N] fp32 or bf16, row strides
+ * ldx and ldo in elements.  A row of out does not depend on M or on the other rows of x. */
+EVS_API int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N,
+                          int K, int group, void* out, int out_dtype, int64_t ldo, cudaStream_t stream);
+
+/* Paged KV cache: pool uint8 [num_pages, kv_heads, block], 16-byte aligned; a block holds page_size
+ * tokens of one head: K codes [P, D / 2] | V codes [P, D / 2] | K scales bf16 [D / 32, P] | V scales
+ * [D / 32, P].  head_dim 32, 64 or 128; page_size a multiple of 16.  err: optional device int32[3]
+ * (zeroed by the caller) that receives the first failure {code, kernel id, row}. */
+typedef struct evs_q4_cache {
+  void* pool;
+  int32_t* err;
+  int64_t num_pages;
+  int32_t page_size, kv_heads, head_dim;
+} evs_q4_cache;
+/* The rows of one call, all device memory: page_table int32 [batch, max_pages] (row stride
+ * table_stride), lengths int32 [batch] (tokens before this call), counts int32 [batch] (new tokens
+ * of each row, at most tokens) or NULL (tokens each).  Row b's new token t < counts[b] sits at
+ * position lengths[b] + t, in page page_table[b][position / page_size]; tokens t >= counts[b] are
+ * padding: nothing is read or written for them.  A row whose lengths and counts lie outside the
+ * table, or a page id outside the pool, sets err and is skipped (attention: NaN). */
+typedef struct evs_q4_rows {
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* counts;
+  int64_t table_stride;
+  int32_t max_pages, batch, tokens;
+} evs_q4_rows;
+/* Rotates k (rotate-half, angle position * rope_base^(-2 j / D)) and stores k and v; with q != NULL
+ * also q_out = rotated q.  Tensors [batch, tokens, heads, D] of one dtype (fp32 or bf16), strides in
+ * elements for the first three dimensions, D contiguous.  Two rows that append to the same slot of
+ * the same page in one call race. */
+EVS_API int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const void* k, const int64_t* k_strides,
+                             const void* v, const int64_t* v_strides, const void* q, const int64_t* q_strides,
+                             void* q_out, const int64_t* q_out_strides, int n_heads, int dtype, double rope_base,
+                             cudaStream_t stream);
+/* the values the cache holds at positions lengths[b] .. lengths[b] + counts[b] - 1 (counts NULL: tokens) */
+EVS_API int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, const int64_t* k_strides, void* v,
+                           const int64_t* v_strides, int dtype, cudaStream_t stream);
+/* Causal attention of the new tokens over the cache (they are appended already): token t of row b
+ * sees positions 0 .. lengths[b] + t.  q and out [batch, tokens, n_heads, D] (fp32 or bf16, out of
+ * q's dtype), already rotated; n_heads a multiple of kv_heads (query head h reads kv head
+ * h / (n_heads / kv_heads)).  max_length >= max(lengths + counts) bounds the launch (0: the whole
+ * table).  workspace: device scratch of at least evs_q4_attention_workspace bytes, one per call in
+ * flight.  A token's result depends on its position, its q and the keys it sees alone: not on the
+ * batch, the other tokens, max_length, the page size or the workspace. */
+EVS_API int64_t evs_q4_attention_workspace(const evs_q4_cache* cache, const evs_q4_rows* rows, int n_heads,
+                                           int max_length);
+EVS_API int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const void* q, const int64_t* q_strides,
+                             int n_heads, float scale, int max_length, void* out, const int64_t* out_strides, int dtype,
+                             void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
 /* ---- γ-parallel drafter (fp32; evspark/train/drafter.py Drafter parameters) ---- */
 typedef struct evs_drafter_config {
   int32_t d_model, n_layers, n_heads, gamma, n_inject, target_hidden, vocab_size, mask_id, ctx_window,

@@ -1,0 +1,382 @@
+"""The 4-bit operators on the device against their definitions in 64 bits (tests/_q4_ref.py)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests import _q4_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def q4():
+    from evspark_b200 import q4 as m
+
+    return m
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def randn(*shape, seed=0, dtype=F32):
+    return torch.randn(*shape, generator=gen(seed), device=DEV).to(dtype)
+
+
+# ---- weights -------------------------------------------------------------------------------
+@pytest.mark.parametrize("n,k,group,dtype", [(1, 1, 32, F32), (5, 31, 32, BF), (33, 128, 64, BF), (16, 129, 128, F32),
+                                             (130, 704, 32, BF), (64, 1000, 64, F32)])
+def test_quantize_matches_the_format(q4, n, k, group, dtype):
+    w = randn(n, k, seed=n + k, dtype=dtype) * torch.exp(randn(n, 1, seed=1) * 3).to(dtype)
+    w[0, :] = 0
+    qw = q4.quantize_weight(w, group)
+    kp = q4.padded_features(k)
+    padded = torch.zeros(n, kp, dtype=torch.float64, device=DEV)
+    padded[:, :k] = w.double()
+    codes, scales = R.quantize(padded, group)
+    assert torch.equal(qw.codes, R.pack(codes))
+    assert torch.equal(qw.scales.double(), scales.t())
+    want = R.held(padded, group)[:, :k]
+    assert torch.equal(qw.dequantize(F32).double(), want)
+    assert torch.equal(qw.dequantize(BF).double(), want)  # held values are exact in bf16
+
+
+def test_quantize_special_groups(q4):
+    w = torch.ones(8, 128, device=DEV)
+    w[1, 3] = math.nan
+    w[2, 40] = math.inf
+    w[3, 70] = -math.inf
+    w[4] *= 2.0 ** -121
+    w[5, :32] = 3e38
+    w[6, 5] = 2.5 * 2 ** -7  # ties go to even
+    d = q4.quantize_weight(w, 32).dequantize(F32)
+    assert d[1, :32].isnan().all() and d[2, 32:64].isnan().all() and d[3, 64:96].isnan().all()
+    assert d[5, :32].isnan().all() and (d[4] == 0).all()
+    assert torch.equal(d[0].double(), R.held(w[0].double(), 32))
+    assert int(d.isnan().sum()) == 4 * 32
+
+
+LINEAR = [(1, 128, 128, 128, BF), (1, 4096, 4096, 128, BF), (8, 33, 65, 32, BF), (9, 1, 1, 32, F32), (13, 704, 256, 64, F32),
+          (16, 257, 1408, 64, BF), (17, 130, 2816, 128, BF), (33, 1003, 717, 32, F32), (64, 384, 4096, 64, BF),
+          (65, 200, 512, 128, BF), (200, 129, 300, 32, F32), (3, 128, 22528, 128, BF)]
+
+
+@pytest.mark.parametrize("m,n,k,group,dtype", LINEAR)
+def test_linear(q4, m, n, k, group, dtype):
+    w = q4.quantize_weight(randn(n, k, seed=3) * k ** -0.5, group)
+    x = randn(m, k, seed=4, dtype=dtype)
+    held = w.dequantize(F32).double()
+    want = x.double() @ held.t()
+    bound = R.linear_bound(x, held)
+    got = q4.q4_linear(x, w)
+    assert got.dtype == F32 and got.shape == (m, n)
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+    got16 = q4.q4_linear(x, w, out_dtype=BF)
+    assert bool(((got16.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all())
+    # a row's bits do not depend on the other rows
+    for r in {0, m // 2, m - 1}:
+        assert torch.equal(q4.q4_linear(x[r:r + 1], w), got[r:r + 1])
+
+
+def test_linear_strides_and_outputs(q4):
+    w = q4.quantize_weight(randn(96, 200, seed=5), 64)
+    big = randn(12, 433, seed=6, dtype=BF)
+    want = q4.q4_linear(big[:, 1:201].contiguous(), w)
+    assert torch.equal(q4.q4_linear(big[:, 1:201], w), want)  # rows at odd offsets
+    assert torch.equal(q4.q4_linear(big[::3, 1:201], w), want[::3])
+    assert torch.equal(q4.q4_linear(big[:, 1:201].unflatten(0, (3, 4)), w), want.unflatten(0, (3, 4)))
+    assert torch.equal(q4.q4_linear(big[0, 1:201], w), want[0])
+    t = randn(200, 12, seed=6, dtype=BF)
+    assert torch.equal(q4.q4_linear(t.t(), w), q4.q4_linear(t.t().contiguous(), w))
+    out = torch.full((14, 96), 7.0, device=DEV)
+    assert q4.q4_linear(big[:, 1:201], w, out=out[1:13]) is not None
+    assert torch.equal(out[1:13], want) and bool((out[0] == 7).all()) and bool((out[13] == 7).all())
+    assert q4.q4_linear(big[:0, 1:201], w).shape == (0, 96)
+
+
+def test_linear_non_finite_rows_stay_in_their_rows(q4):
+    w = q4.quantize_weight(randn(40, 128, seed=7), 128)
+    x = randn(5, 128, seed=8)
+    clean = q4.q4_linear(x, w)
+    x[1, 0], x[3, 127] = math.nan, math.inf
+    got = q4.q4_linear(x, w)
+    assert torch.equal(got[[0, 2, 4]], clean[[0, 2, 4]])
+    assert bool(got[1].isnan().all()) and not bool(got[3].isfinite().all())
+
+
+# ---- cache ---------------------------------------------------------------------------------
+def make_rows(q4, ends, page, G, D, seed=0, extra=2, fill=0xFF):
+    """A pool of garbage (codes of 15, NaN scales) and scattered pages for rows that reach ``ends`` tokens."""
+    need = [max(1, -(-e // page)) for e in ends]
+    total = sum(need) + extra
+    cache = q4.Q4Cache(total, G, D, page_size=page, device=DEV)
+    cache.pool.fill_(fill)
+    perm = torch.randperm(total, generator=torch.Generator().manual_seed(seed)).tolist()
+    table = torch.full((len(ends), max(need)), -1, dtype=torch.int32)
+    for b, n in enumerate(need):
+        table[b, :n] = torch.tensor([perm.pop() for _ in range(n)], dtype=torch.int32)
+    return cache, table.to(DEV)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def fill_cache(q4, cache, table, starts, ends, G, D, seed=0, dtype=BF):
+    """Append random keys and values for positions [0, ends[b]); returns the held values per row."""
+    T = max(ends)
+    k, v = randn(len(ends), T, G, D, seed=seed + 1, dtype=dtype), randn(len(ends), T, G, D, seed=seed + 2, dtype=dtype)
+    q4.q4_kv_append(cache, table, i32([0] * len(ends)), k, v, counts=i32(ends))
+    kk, vv = q4.q4_kv_read(cache, table, i32([0] * len(ends)), T, counts=i32(ends))
+    return kk, vv
+
+
+@pytest.mark.parametrize("D,G,H,page,dtype", [(128, 4, 4, 64, BF), (128, 2, 6, 16, F32), (64, 3, 15, 48, BF),
+                                              (64, 1, 8, 128, F32), (32, 8, 8, 32, F32), (32, 5, 5, 16, BF)])
+def test_append_rotates_quantises_and_pages(q4, D, G, H, page, dtype):
+    starts, counts, T = [0, 1, page - 1, 777, 262000, 5], [7, 3, 7, 5, 6, 0], 7
+    ends = [s + c for s, c in zip(starts, counts)]
+    cache, table = make_rows(q4, ends, page, G, D)
+    before = cache.pool.clone()
+    qkv = randn(6, T, (H + 2 * G) * D, seed=11, dtype=dtype)
+    q = qkv[..., :H * D].unflatten(-1, (H, D))
+    k = qkv[..., H * D:(H + G) * D].unflatten(-1, (G, D))
+    v = qkv[..., (H + G) * D:].unflatten(-1, (G, D))
+    q_out = torch.full((6, T, H, D), 7.0, dtype=dtype, device=DEV)
+    q4.q4_kv_append(cache, table, i32(starts), k, v, q=q, counts=i32(counts), q_out=q_out)
+    cache.check()
+    codes = page * D // 2
+    touched = torch.zeros_like(before, dtype=torch.bool)
+    for b, (s, c) in enumerate(zip(starts, counts)):
+        assert bool((q_out[b, c:] == 7).all())  # padding is left as it was
+        if c == 0:
+            continue
+        pos = torch.arange(s, s + c, device=DEV)
+        want_q = R.rotate(q[b, :c], pos)
+        # one rounding to the type (by way of fp32)
+        assert bool(((q_out[b, :c].double() - want_q).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * want_q.abs()
+                     + 2.0 ** -40).all())
+        for what, x in enumerate((R.rotate(k[b, :c], pos), v[b, :c].double())):
+            cc, ss = R.quantize(x, 32)
+            for i in range(c):
+                p, slot = int(table[b, (s + i) // page]), (s + i) % page
+                blk = cache.pool[p]
+                at = what * codes + slot * D // 2
+                assert torch.equal(blk[:, at:at + D // 2], R.pack(cc[i]))
+                touched[p, :, at:at + D // 2] = True
+                sc = blk[:, 2 * codes + what * (page * D // 16):][:, :page * D // 16].contiguous().view(BF)
+                assert torch.equal(sc.view(G, D // 32, page)[:, :, slot].double(), ss[i])
+                for grp in range(D // 32):
+                    o = 2 * codes + what * (page * D // 16) + 2 * (grp * page + slot)
+                    touched[p, :, o:o + 2] = True
+    assert torch.equal(cache.pool[~touched], before[~touched])  # nothing else was written
+
+
+def test_append_special_values(q4):
+    cache, table = make_rows(q4, [8], 16, 1, 64)
+    k, v = randn(1, 8, 1, 64, seed=1), randn(1, 8, 1, 64, seed=2)
+    v[0, 1, 0, 5], v[0, 2, 0, 40], v[0, 3] = math.nan, math.inf, 0
+    k[0, 4, 0, 0], v[0, 5, 0, :32], v[0, 6, 0, 32:] = math.nan, 3e38, 2.0 ** -130
+    q4.q4_kv_append(cache, table, i32([0]), k, v)
+    kk, vv = q4.q4_kv_read(cache, table, i32([0]), 8, dtype=F32)
+    assert bool(vv[0, 1, 0, :32].isnan().all()) and bool(vv[0, 1, 0, 32:].isfinite().all())
+    assert bool(vv[0, 2, 0, 32:].isnan().all()) and bool((vv[0, 3] == 0).all())
+    assert bool(kk[0, 4].isnan().all())  # the rotation carries the NaN into the pair's other half
+    assert bool(vv[0, 5, 0, :32].isnan().all()) and bool((vv[0, 6, 0, 32:] == 0).all())
+
+
+def test_append_unaligned_views_and_default_q_out(q4):
+    cache, table = make_rows(q4, [20], 16, 2, 64)
+    big = randn(1, 5, 2, 67, seed=3, dtype=BF)
+    k, v, q = big[..., 1:65], big[..., 2:66], big[..., 3:67]
+    a = q4.q4_kv_append(cache, table, i32([13]), k, v, q=q)
+    pool = cache.pool.clone()
+    cache.pool.fill_(0xFF)
+    qq = q.contiguous()
+    b = q4.q4_kv_append(cache, table, i32([13]), k.contiguous(), v.contiguous(), q=qq, q_out=qq)  # in place
+    assert torch.equal(a, b) and torch.equal(pool, cache.pool)
+
+
+ATTEND = [  # starts, T, counts, H, G, D, page, dtype
+    ([0], 1, None, 1, 1, 32, 16, F32),
+    ([0, 1, 15, 16, 17], 1, None, 4, 4, 64, 16, BF),
+    ([0, 3, 62, 63, 64, 250, 255, 256], 13, None, 2, 2, 128, 64, BF),
+    ([5, 100, 31, 700], 7, [7, 0, 3, 1], 10, 2, 64, 48, F32),
+    ([1023, 2], 13, [13, 4], 16, 2, 128, 32, BF),
+    ([300], 5, None, 20, 1, 32, 16, BF),
+    ([40], 3, None, 34, 2, 128, 128, F32),
+    ([4090], 13, None, 3, 1, 32, 64, BF),
+    ([4095, 4096, 10], 2, None, 2, 1, 32, 64, F32),
+    ([65530], 13, None, 1, 1, 32, 128, F32),
+    ([70000, 20], 2, None, 2, 1, 32, 128, BF),
+]
+
+
+@pytest.mark.parametrize("starts,T,counts,H,G,D,page,dtype", ATTEND)
+def test_attention(q4, starts, T, counts, H, G, D, page, dtype):
+    counts = counts or [T] * len(starts)
+    ends = [s + c for s, c in zip(starts, counts)]
+    cache, table = make_rows(q4, ends, page, G, D, seed=H)
+    k, v = fill_cache(q4, cache, table, starts, ends, G, D, seed=T, dtype=dtype)
+    q = randn(len(starts), T, H, D, seed=9, dtype=dtype) * 2
+    out = torch.full((len(starts), T, H, D), 7.0, dtype=dtype, device=DEV)
+    q4.q4_attention(q, cache, table, i32(starts), counts=i32(counts), out=out)
+    cache.check()
+    for b, (s, c) in enumerate(zip(starts, counts)):
+        assert bool((out[b, c:] == 7).all())
+        if c == 0:
+            continue
+        want, av, mag = R.attend(q[b, :c], k[b, :s + c].double(), v[b, :s + c].double(), s, D ** -0.5)
+        bound = R.attend_bound(want, av, mag, s + c, D, dtype)
+        err = (out[b, :c].double() - want).abs()
+        assert bool((err <= bound).all()), (b, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("start,T,H,G,D,dtype", [(250, 13, 8, 2, 64, BF), (4088, 16, 3, 1, 32, BF), (1000, 9, 6, 2, 128, F32),
+                                                 (65529, 13, 1, 1, 32, BF)])
+def test_attention_bits_depend_on_the_token_alone(q4, start, T, H, G, D, dtype):
+    """A verify block, single steps, another batch, page size, bound and strides give the same bits."""
+    end = start + T
+    cache, table = make_rows(q4, [end, 40, end], 64, G, D)
+    k, v = randn(3, end, G, D, seed=1, dtype=dtype), randn(3, end, G, D, seed=2, dtype=dtype)
+    k[2], v[2] = k[0], v[0]
+    q4.q4_kv_append(cache, table, i32([0, 0, 0]), k, v, counts=i32([end, 40, end]))
+    q = randn(3, T, H, D, seed=3, dtype=dtype) * 2
+    q[2] = q[0]
+    block = q4.q4_attention(q, cache, table, i32([start, 20, start]), counts=i32([T, 5, T]))
+    assert torch.equal(block[0], block[2])
+    for t in (0, 1, T // 2, T - 1):
+        step = q4.q4_attention(q[:1, t:t + 1], cache, table[:1], i32([start + t]), max_length=start + t + 1)
+        assert torch.equal(step[0, 0], block[0, t]), t
+    other, ot = make_rows(q4, [end], 16, G, D, seed=5)
+    q4.q4_kv_append(other, ot, i32([0]), k[:1], v[:1])
+    wide = torch.zeros(1, T, H, D + 3, dtype=dtype, device=DEV)
+    wide[..., 1:D + 1] = q[0]
+    got = q4.q4_attention(wide[..., 1:D + 1], other, ot, i32([start]), out=wide[..., 2:D + 2].clone()[..., :D])
+    assert torch.equal(got[0], block[0])
+
+
+def test_attention_nan_keys_and_values_reach_only_who_sees_them(q4):
+    D, G, T, start = 64, 1, 6, 60
+    cache, table = make_rows(q4, [start + T], 16, G, D)
+    k, v = randn(1, start + T, G, D, seed=1), randn(1, start + T, G, D, seed=2)
+    q4.q4_kv_append(cache, table, i32([0]), k, v)
+    q = randn(1, T, 2, D, seed=3)
+    clean = q4.q4_attention(q, cache, table, i32([start]))
+    vb, kb = v.clone(), k.clone()
+    vb[0, start + 2, 0, 40] = math.nan  # the token at start + 2, second group of features
+    kb[0, start + 4, 0, 1] = math.inf
+    q4.q4_kv_append(cache, table, i32([0]), kb, vb)
+    got = q4.q4_attention(q, cache, table, i32([start]))
+    assert torch.equal(got[0, :2], clean[0, :2])
+    assert bool(got[0, 2:4, :, 32:].isnan().all()) and torch.equal(got[0, 2:4, :, :32], clean[0, 2:4, :, :32])
+    assert bool(got[0, 4:].isnan().all())
+
+
+def test_attention_scale_and_sharp_scores(q4):
+    """Scores far apart (one key takes all the weight) and a scale of the caller's."""
+    D, end = 128, 600
+    cache, table = make_rows(q4, [end], 64, 2, D)
+    k, v = fill_cache(q4, cache, table, [end - 4], [end], 2, D)
+    q = randn(1, 4, 4, D, seed=5) * 30
+    out = q4.q4_attention(q, cache, table, i32([end - 4]), scale=0.7)
+    want, av, mag = R.attend(q[0], k[0].double(), v[0].double(), end - 4, 0.7)
+    bound = R.attend_bound(want, av, mag, end, D, F32)
+    assert bool(((out[0].double() - want).abs() <= bound).all())
+
+
+def test_bad_pages_and_lengths_are_reported_not_followed(q4):
+    cache, table = make_rows(q4, [40, 40, 40, 40], 16, 1, 64, fill=0)
+    k, v = randn(4, 40, 1, 64, seed=1), randn(4, 40, 1, 64, seed=2)
+    q4.q4_kv_append(cache, table, i32([0] * 4), k, v)
+    q = randn(4, 2, 1, 64, seed=3)
+    good = q4.q4_attention(q, cache, table, i32([38] * 4))
+    cache.check()
+    bad = table.clone()
+    bad[1, 1] = cache.num_pages
+    bad[2, 0] = -7
+    lengths = i32([38, 38, 38, 47])
+    got = q4.q4_attention(q, cache, bad, lengths)
+    assert torch.equal(got[0], good[0]) and bool(got[1:].isnan().all())
+    with pytest.raises(RuntimeError, match="page table|pool"):
+        cache.check()
+    cache.check()  # read once
+    before = cache.pool.clone()
+    q4.q4_kv_append(cache, bad, i32([0, 16, 0, -1]), k[:, :1], v[:, :1], counts=i32([0, 1, 1, 1]))
+    assert torch.equal(before, cache.pool)
+    with pytest.raises(RuntimeError):
+        cache.check()
+    assert bool(q4.q4_attention(q, cache, table, lengths, counts=i32([2, 3, 2, 2]))[1].isnan().all())
+    with pytest.raises(RuntimeError):
+        cache.check()
+    # a bound below the true length is noted, and that row's result is NaN
+    long, lt = make_rows(q4, [600], 16, 1, 32)
+    q4.q4_kv_append(long, lt, i32([0]), randn(1, 600, 1, 32), randn(1, 600, 1, 32))
+    assert bool(q4.q4_attention(randn(1, 1, 1, 32), long, lt, i32([599]), max_length=256).isnan().all())
+    with pytest.raises(RuntimeError):
+        long.check()
+
+
+def test_together_in_a_captured_graph_on_another_stream(q4):
+    """A decode step of projection, append, attention and projection, captured and replayed with new inputs."""
+    d, H, G, D, T = 256, 4, 2, 64, 3
+    w_qkv = q4.quantize_weight(randn((H + 2 * G) * D, d, seed=1) * d ** -0.5, 64)
+    w_o = q4.quantize_weight(randn(d, H * D, seed=2) * d ** -0.5, 64)
+    cache, table = make_rows(q4, [200, 200], 16, G, D)
+    lengths = i32([90, 0])
+
+    def step(x):
+        qkv = q4.q4_linear(x, w_qkv, out_dtype=BF).unflatten(-1, (H + 2 * G, D))
+        q = q4.q4_kv_append(cache, table, lengths, qkv[:, :, H:H + G], qkv[:, :, H + G:], q=qkv[:, :, :H])
+        a = q4.q4_attention(q, cache, table, lengths)
+        return q4.q4_linear(a.flatten(2), w_o)
+
+    q4.q4_kv_append(cache, table, i32([0, 0]), randn(2, 90, G, D, seed=4, dtype=BF), randn(2, 90, G, D, seed=5, dtype=BF))
+    xs = [randn(2, T, d, seed=10 + i, dtype=BF) for i in range(4)]
+    want = []
+    for i, x in enumerate(xs):
+        lengths.copy_(i32([90 + T * i, T * i]))
+        want.append(step(x).clone())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    x = xs[0].clone()
+    with torch.cuda.stream(side):
+        step(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            y = step(x)
+        for i in range(4):
+            x.copy_(xs[i])
+            lengths.copy_(i32([90 + T * i, T * i]))
+            g.replay()
+            assert torch.equal(y, want[i]), i
+    torch.cuda.current_stream().wait_stream(side)
+    cache.check()
+    # and in 64 bits, from what the cache holds: the attention's inputs are the kernel's own
+    assert bool(want[-1].isfinite().all())
+
+
+def test_large_pool_offsets(q4):
+    """Pages beyond 2^31 bytes of the pool."""
+    page, G, D = 128, 8, 128
+    block = q4.Q4Cache.block_bytes(D, page)
+    pages = (2 ** 32) // (G * block) + 3
+    cache = q4.Q4Cache(pages, G, D, page_size=page, device=DEV)
+    k, v = randn(1, 130, G, D, seed=1, dtype=BF), randn(1, 130, G, D, seed=2, dtype=BF)
+    far, near = i32([[pages - 1, pages - 2]]), i32([[0, 1]])
+    for t in (far, near):
+        q4.q4_kv_append(cache, t, i32([0]), k, v)
+    q = randn(1, 2, G, D, seed=3, dtype=BF)
+    assert torch.equal(q4.q4_attention(q, cache, far, i32([128])), q4.q4_attention(q, cache, near, i32([128])))
+    a, b = (q4.q4_kv_read(cache, t, i32([0]), 130) for t in (far, near))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    cache.check()
