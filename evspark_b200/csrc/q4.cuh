@@ -41,25 +41,24 @@ __device__ __forceinline__ Q4Scale q4_scale(uint32_t s2) {
   return {q4_mul2(s2, 0x41804180u), q4_mul2(s2, 0xC1C0C1C0u)};
 }
 
-// codes at bits SHIFT.. of both halves of w -> the pair of values
-template <int SHIFT>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w, const Q4Scale& s) {
-  const uint32_t t = SHIFT < 3 ? w << (3 - SHIFT) : w >> (SHIFT - 3);
-  return q4_fma2((t & 0x00780078u) | 0x3F803F80u, s.mul, s.add);
+// codes at bits 3 .. 6 of both halves of t -> the pair of values
+__device__ __forceinline__ uint32_t q4_value(uint32_t t, const Q4Scale& s) {
+  uint32_t m;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(t), "r"(0x00780078u), "r"(0x3F803F80u));  // (t & mask) | 1.0
+  return q4_fma2(m, s.mul, s.add);
 }
 // eight codes of one word -> value pairs (0,4) (1,5) (2,6) (3,7)
 __device__ __forceinline__ void q4_word(uint32_t w, const Q4Scale& s, uint32_t (&v)[4]) {
-  v[0] = q4_pair<0>(w, s);
-  v[1] = q4_pair<4>(w, s);
-  v[2] = q4_pair<8>(w, s);
-  v[3] = q4_pair<12>(w, s);
+  v[0] = q4_value(w << 3, s);
+  v[1] = q4_value(w >> 1, s);
+  v[2] = q4_value(w >> 5, s);
+  v[3] = q4_value(w >> 9, s);
 }
 
 // d += a b, one m16n8k16 tensor-core product (bf16 operands, fp32 sums)
 __device__ __forceinline__ void q4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));

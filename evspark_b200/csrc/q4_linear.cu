@@ -4,6 +4,7 @@
 //          up to 128 with codes of 8 (zeros) behind K
 //   scales bf16 [Kp / group][N]
 #include <algorithm>
+#include <cstring>
 
 #include "internal.hpp"
 #include "q4.cuh"
@@ -12,50 +13,64 @@ namespace {
 
 constexpr int LIN_WARPS = 8;
 constexpr int LIN_THREADS = 32 * LIN_WARPS;
-constexpr int LIN_ROWS = 128;     // weight rows per CTA: four warps of 32 rows
-constexpr int LIN_KW = 2;         // warps that share a row tile and take every other K block
-constexpr int LIN_TOKENS = 64;    // tokens per CTA at most
 constexpr int LIN_CLUSTER = 8;    // CTAs of one output tile at most (splits of K)
 
 // x staged in shared memory in the order in which the products read it: per (K block, 8-token
-// tile, part) four 16-byte words per lane; lane (n, c) word w holds features 32 c + 8 w .. + 7 of
-// token n as pairs (0,4) (1,5) (2,6) (3,7), the order in which q4_word decodes a weight word.
+// tile, part) four words of 16 bytes per lane; lane (n, c) word w holds features 32 c + 8 w .. + 7 of
+// token n as pairs (0,4) (1,5) (2,6) (3,7), the order in which q4_word decodes a weight word.  Word w
+// of lane l sits at l ^ 2 w, so that the eight lanes of one store phase (two c, four w) meet eight
+// different 16-byte bank groups; reads stay a permutation of 32 lanes.
 __device__ __forceinline__ uint4 pair_up(uint4 v) {
   return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                     __byte_perm(v.y, v.w, 0x7632));
 }
 
-template <typename TX>
-__device__ __forceinline__ void stage_x(uint4* xs, const TX* __restrict__ x, int64_t ldx, int M, int K, int m0, int NT,
-                                        int kb0, int nkb, bool vec) {
-  constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
-  const int units = nkb * NT * 8 * 16;  // (token, 8 features)
-  for (int i = threadIdx.x; i < units; i += LIN_THREADS) {
-    const int u = i & 15, n = (i >> 4) % (8 * NT), kb = (i >> 4) / (8 * NT);
-    const int k = (kb0 + kb) * Q4_KBLOCK + 8 * u;
-    const int c = u >> 2, w = u & 3;
-    uint4* dst = xs + ((static_cast<size_t>(kb) * NT + (n >> 3)) * NP * 4 + w) * 32 + (n & 7) * 4 + c;
-    const bool row = m0 + n < M;
-    const TX* src = x + static_cast<int64_t>(m0 + n) * ldx + k;
-    if constexpr (NP == 1) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (row && vec && k + 8 <= K) {
-        v = *reinterpret_cast<const uint4*>(src);
-      } else if (row) {
-        uint32_t e[8];
+template <typename TX, int NT>
+__device__ __forceinline__ void stage_x(uint4* xs, const TX* __restrict__ x, int64_t ldx, int M, int K, int m0, int kb0,
+                                        int nkb, bool vec) {
+  constexpr int NP = sizeof(TX) == 2 ? 1 : 3, NR = NP == 1 ? 1 : 2;
+  constexpr int TPB = LIN_THREADS / 16;                   // tokens that the CTA loads at once
+  constexpr int KSTEP = TPB > 8 * NT ? TPB / (8 * NT) : 1;  // ... or K blocks
+  constexpr int BATCH = NP == 1 ? 4 : 2;                  // loads of a thread in flight
+  const int u = threadIdx.x & 15, c = u >> 2, w = u & 3, row = threadIdx.x >> 4;
+  for (int n = row % (8 * NT); n < 8 * NT; n += TPB) {
+    const bool live = m0 + n < M;
+    const TX* src = x + static_cast<int64_t>(m0 + n) * ldx + 8 * u;
+    uint4* dst = xs + ((n >> 3) * NP * 4 + w) * 32 + (((n & 7) * 4 + c) ^ (2 * w));
+    for (int kb = row / (8 * NT); kb < nkb; kb += BATCH * KSTEP) {
+      uint4 raw[BATCH][NR];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = k + j < K ? __bfloat16_as_ushort(src[j]) : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+      for (int r = 0; r < BATCH; ++r) {
+        const int k0 = (kb0 + kb + r * KSTEP) * Q4_KBLOCK, k = k0 + 8 * u;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) raw[r][h] = make_uint4(0u, 0u, 0u, 0u);
+        if (kb + r * KSTEP >= nkb || !live) continue;
+        if (vec && k + 8 <= K) {
+#pragma unroll
+          for (int h = 0; h < NR; ++h) raw[r][h] = reinterpret_cast<const uint4*>(src + k0)[h];
+        } else if (k < K) {
+          TX e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = k + j < K ? src[k0 + j] : from_f32<TX>(0.f);
+          memcpy(raw[r], e, sizeof(e));
+        }
       }
-      *dst = pair_up(v);
-    } else {
-      uint32_t p[8][3];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q4_parts(row && k + j < K ? src[j] : 0.f, p[j]);
+      for (int r = 0; r < BATCH; ++r) {
+        if (kb + r * KSTEP >= nkb) break;
+        uint4* d = dst + (kb + r * KSTEP) * (NT * NP * 4 * 32);
+        if constexpr (NP == 1) {
+          *d = pair_up(raw[r][0]);
+        } else {
+          uint32_t p[8][3];
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
-        dst[q * 4 * 32] = make_uint4(p[0][q] | p[4][q] << 16, p[1][q] | p[5][q] << 16, p[2][q] | p[6][q] << 16,
-                                     p[3][q] | p[7][q] << 16);
+          for (int j = 0; j < 8; ++j) q4_parts(__uint_as_float((&raw[r][j >> 2].x)[j & 3]), p[j]);
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            d[q * 4 * 32] = make_uint4(p[0][q] | p[4][q] << 16, p[1][q] | p[5][q] << 16, p[2][q] | p[6][q] << 16,
+                                       p[3][q] | p[7][q] << 16);
+        }
+      }
     }
   }
 }
@@ -65,41 +80,53 @@ struct LinTile {  // one warp's share of a K block: 32 rows x 128 features
   uint32_t s[4];
 };
 
-__device__ __forceinline__ void load_tile(LinTile& t, const uint8_t* const (&row)[4], const uint16_t* sc, int N, int r0,
-                                          int group, int kb, int c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint4* p = reinterpret_cast<const uint4*>(row[i] + static_cast<size_t>(kb) * (Q4_KBLOCK / 2));
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(t.w[i].x), "=r"(t.w[i].y), "=r"(t.w[i].z), "=r"(t.w[i].w)
-                 : "l"(p));
-  }
-  const int gi = (kb * Q4_KBLOCK + 32 * c) / group;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) t.s[i] = __ldg(sc + static_cast<size_t>(gi) * N + min(r0 + 8 * i, N - 1));
+// the weight streams through once: no space in L1
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+  uint4 v;
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
-// grid (K splits = cluster, row tiles, token tiles)
-template <typename TX, typename TO, int NT>
-__global__ void __launch_bounds__(LIN_THREADS)
+// grid (K splits = cluster, row tiles, token tiles).  Registers hold the next two K blocks' codes
+// while one is multiplied; the first ones are on their way before x is staged.
+template <typename TX, typename TO, int NT, int KW>
+__global__ void __launch_bounds__(LIN_THREADS, NT <= 2 ? 2 : 1)
     q4_linear_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint8_t* __restrict__ codes,
-                     const uint16_t* __restrict__ scales, int N, int K, int group, TO* __restrict__ out, int64_t ldo,
-                     int chunk_kb, int vec) {
+                     const uint16_t* __restrict__ scales, int N, int K, int group_shift, TO* __restrict__ out,
+                     int64_t ldo, int chunk_kb, int vec, uint32_t red_offset) {
   constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
+  constexpr int LIN_ROWS = 32 * LIN_WARPS / KW, LIN_KW = KW;
   extern __shared__ __align__(16) unsigned char lin_sm[];
+  cluster_arrive_relaxed();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int wr = warp & 3, wk = warp >> 2;
+  const int wr = warp % (LIN_WARPS / KW), wk = warp / (LIN_WARPS / KW);
   const int S = gridDim.x, rank = blockIdx.x;
-  const int n0 = blockIdx.y * LIN_ROWS, m0 = blockIdx.z * LIN_TOKENS;
+  const int n0 = blockIdx.y * LIN_ROWS, m0 = blockIdx.z * 8 * NT;
   const int KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
   const int kb_begin = static_cast<int>(static_cast<int64_t>(KB) * rank / S);
   const int kb_end = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / S);
-  const int r0 = n0 + 32 * wr + g;
   const size_t row_bytes = static_cast<size_t>(KB) * (Q4_KBLOCK / 2);
-  const uint8_t* row[4];
+  // 32-bit offsets from the row tile's uniform base (its rows span less than 2^32 bytes)
+  const uint8_t* base = codes + static_cast<size_t>(n0) * row_bytes;
+  const uint8_t* sbase = reinterpret_cast<const uint8_t*>(scales + n0);
+  uint32_t off[4], soff[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) row[i] = codes + static_cast<size_t>(min(r0 + 8 * i, N - 1)) * row_bytes + 16 * c;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t r = min(32 * wr + g + 8 * i, N - 1 - n0);
+    off[i] = r * static_cast<uint32_t>(row_bytes) + 16 * c;
+    soff[i] = 2 * r;
+  }
+  auto load = [&](LinTile& t, int kb) {
+    if (kb >= kb_end) return;
+    const uint32_t so = static_cast<uint32_t>((kb * Q4_KBLOCK + 32 * c) >> group_shift) * (2u * N);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.w[i] = ld_stream(base + (off[i] + static_cast<uint32_t>(kb) * (Q4_KBLOCK / 2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.s[i] = __ldg(reinterpret_cast<const uint16_t*>(sbase + (soff[i] + so)));
+  };
 
   float acc[2][NT][4];
 #pragma unroll
@@ -109,20 +136,31 @@ __global__ void __launch_bounds__(LIN_THREADS)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
 
+  LinTile t0, t1;
+  load(t0, kb_begin + wk);
+  load(t1, kb_begin + wk + LIN_KW);
   uint4* xs = reinterpret_cast<uint4*>(lin_sm);
   pdl_wait();
   for (int kc = kb_begin; kc < kb_end; kc += chunk_kb) {
     const int nkb = min(chunk_kb, kb_end - kc);
+    if (kc != kb_begin) __syncthreads();
+    stage_x<TX, NT>(xs, x, ldx, M, K, m0, kc, nkb, vec != 0);
     __syncthreads();
-    stage_x<TX>(xs, x, ldx, M, K, m0, NT, kc, nkb, vec != 0);
-    __syncthreads();
-    for (int kb = wk; kb < nkb; kb += LIN_KW) {
-      LinTile t;
-      load_tile(t, row, scales, N, r0, group, kc + kb, c);
+    auto multiply = [&](const LinTile& t, int kb) {
       Q4Scale s[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] = q4_scale(t.s[i] | t.s[i] << 16);
-      const uint4* xb = xs + static_cast<size_t>(kb) * NT * NP * 4 * 32 + lane;
+      const uint4* xb = xs + kb * NT * NP * 4 * 32;
+      // three-part fp32 rows: a block's 24 product steps are summed apart, as each step truncates
+      float part[2][NT][4];
+      if constexpr (NP > 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[i][j][e] = 0.f;
+      }
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         uint32_t a[4][4];
@@ -132,71 +170,98 @@ __global__ void __launch_bounds__(LIN_THREADS)
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int q = NP - 1; q >= 0; --q) {
-            const uint4 b = xb[((j * NP + q) * 4 + w) * 32];
+            const uint4 b = xb[((j * NP + q) * 4 + w) * 32 + (lane ^ (2 * w))];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              q4_mma(acc[i][j], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1], b.x, b.y);
-              q4_mma(acc[i][j], a[2 * i][2], a[2 * i + 1][2], a[2 * i][3], a[2 * i + 1][3], b.z, b.w);
+              float(&d)[4] = NP > 1 ? part[i][j] : acc[i][j];
+              q4_mma(d, a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1], b.x, b.y);
+              q4_mma(d, a[2 * i][2], a[2 * i + 1][2], a[2 * i][3], a[2 * i + 1][3], b.z, b.w);
             }
           }
       }
+      if constexpr (NP > 1) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] += part[i][j][e];
+      }
+    };
+    // a tile's registers are loaded again as soon as it is multiplied (no copies: a move of a
+    // register that a load still fills would wait for it); chunks hold an even number of tiles a warp
+    for (int kb = wk; kb < nkb; kb += 2 * LIN_KW) {
+      multiply(t0, kb);
+      load(t0, kc + kb + 2 * LIN_KW);
+      if (kb + LIN_KW < nkb) {
+        multiply(t1, kb + LIN_KW);
+        load(t1, kc + kb + 3 * LIN_KW);
+      }
     }
   }
-  // sums over the two K warps and the cluster's splits, in that order: red[wk][token][row]
-  __syncthreads();
-  float* red = reinterpret_cast<float*>(lin_sm);
-  constexpr int RL = LIN_ROWS + 4;
+  // Sums over the K warps and the cluster's splits, in that order.  Rank r owns RC rows of the output
+  // tile; every CTA pushes its sums into the owner's [split][K warp][token][row] slots, which alias
+  // nothing that a slower CTA still reads, so one cluster barrier is enough.
   constexpr int TOK = 8 * NT;
+  const int RC = (LIN_ROWS + S - 1) / S;
+  const uint32_t red = smem_u32(lin_sm) + red_offset;
+  cluster_wait();  // every CTA of the cluster has started
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        red[(wk * TOK + 8 * j + 2 * c + (e & 1)) * RL + 32 * wr + 16 * i + g + 8 * (e >> 1)] = acc[i][j][e];
-  if (S > 1) {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  } else {
-    __syncthreads();
-  }
-  const int tokens = min(TOK, M - m0);
-  for (int i = rank * LIN_THREADS + threadIdx.x; i < tokens * LIN_ROWS; i += S * LIN_THREADS) {
-    const int tok = i / LIN_ROWS, r = i % LIN_ROWS;
-    if (n0 + r >= N) continue;
-    float sum = 0.f;
-    for (int p = 0; p < S; ++p) {
+    for (int h = 0; h < 2; ++h) {
+      const int r = 32 * wr + 16 * i + 8 * h + g, owner = r / RC;
       uint32_t a;
-      float v0, v1;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(red + tok * RL + r)), "r"(p));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v0) : "r"(a) : "memory");
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v1) : "r"(a + TOK * RL * 4) : "memory");
-      sum += v0 + v1;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;"
+          : "=r"(a)
+          : "r"(red + 4 * (((rank * KW + wk) * TOK + 2 * c) * RC + r - owner * RC)), "r"(owner));
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a + 4 * (8 * j + e) * RC), "f"(acc[i][j][2 * h + e])
+                       : "memory");
     }
-    out[static_cast<int64_t>(m0 + tok) * ldo + n0 + r] = from_f32<TO>(sum);
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const float* mine = reinterpret_cast<const float*>(lin_sm + red_offset);
+  const int tokens = min(TOK, M - m0), first = rank * RC, own_rows = min(RC, min(LIN_ROWS, N - n0) - first);
+  for (int i = threadIdx.x; i < tokens * own_rows; i += LIN_THREADS) {
+    const int tok = i / own_rows, r = i - tok * own_rows;
+    float v[LIN_CLUSTER][KW];
+#pragma unroll
+    for (int p = 0; p < LIN_CLUSTER; ++p)
+#pragma unroll
+      for (int q = 0; q < KW; ++q) v[p][q] = p < S ? mine[((p * KW + q) * TOK + tok) * RC + r] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int p = 0; p < LIN_CLUSTER; ++p)
+      if (p < S) {
+        float part = v[p][0];
+#pragma unroll
+        for (int q = 1; q < KW; ++q) part += v[p][q];
+        sum += part;
+      }
+    out[static_cast<int64_t>(m0 + tok) * ldo + n0 + first + r] = from_f32<TO>(sum);
   }
-  // no CTA of the cluster leaves while another still reads its sums
-  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename TX, typename TO, int NT>
-int launch_linear_nt(const void* x, int64_t ldx, int M, const void* codes, const void* scales, int N, int K, int group,
-                     void* out, int64_t ldo, cudaStream_t st, bool pdl) {
-  constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
-  const int tiles = (N + LIN_ROWS - 1) / LIN_ROWS, KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
-  // splits of K from N and K alone, so that a token's sums do not depend on the other tokens
-  int S = 1;
-  while (S < LIN_CLUSTER && tiles * S < 296 && KB / (2 * S) >= 4) S *= 2;
+template <typename TX, typename TO, int NT, int KW>
+int launch_linear_kw(const void* x, int64_t ldx, int M, const void* codes, const void* scales, int N, int K, int group,
+                     void* out, int64_t ldo, int S, cudaStream_t st, bool pdl) {
+  constexpr int NP = sizeof(TX) == 2 ? 1 : 3, ROWS = 32 * LIN_WARPS / KW;
+  const int tiles = (N + ROWS - 1) / ROWS, KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
   const int block_bytes = NT * NP * 2048;  // staged x of one K block
   const int slice = (KB + S - 1) / S;
-  // an even number of blocks, so that the two K warps take the same blocks at every chunk size
-  int chunk = std::max(2, 49152 / block_bytes) & ~1;
+  // a multiple of 2 KW blocks: whichever the chunk, a K warp takes the same blocks in the same registers
+  int chunk = std::max(2 * KW, (NT <= 2 ? 81920 : 131072) / block_bytes / (2 * KW) * (2 * KW));
   chunk = std::min(chunk, slice);
-  const int smem = std::max(chunk * block_bytes, 2 * 8 * NT * (LIN_ROWS + 4) * 4);
-  auto* kern = q4_linear_kernel<TX, TO, NT>;
+  const int red_offset = chunk * block_bytes;
+  const int smem = red_offset + S * KW * 8 * NT * ((ROWS + S - 1) / S) * 4;
+  auto* kern = q4_linear_kernel<TX, TO, NT, KW>;
   static std::atomic<unsigned long long> done{0};
   EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), 200 * 1024));
   const int vec = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(TX)) % 16 == 0) ? 1 : 0;
-  const int ztiles = (M + LIN_TOKENS - 1) / LIN_TOKENS;
+  const int ztiles = (M + 8 * NT - 1) / (8 * NT);
   EVS_CHECK_ARG(tiles <= 65535 && ztiles <= 65535, "q4 linear: too many rows or tokens");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, tiles, ztiles);
@@ -213,10 +278,24 @@ int launch_linear_nt(const void* x, int64_t ldx, int M, const void* codes, const
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
   EVS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<const TX*>(x), ldx, M, static_cast<const uint8_t*>(codes),
-                                  static_cast<const uint16_t*>(scales), N, K, group, static_cast<TO*>(out), ldo, chunk,
-                                  vec));
+                                  static_cast<const uint16_t*>(scales), N, K, group == 32 ? 5 : (group == 64 ? 6 : 7),
+                                  static_cast<TO*>(out), ldo, chunk, vec, static_cast<uint32_t>(red_offset)));
   evs_count_launch(1);
   return EVS_OK;
+}
+
+template <typename TX, typename TO, int NT>
+int launch_linear_nt(const void* x, int64_t ldx, int M, const void* codes, const void* scales, int N, int K, int group,
+                     void* out, int64_t ldo, cudaStream_t st, bool pdl) {
+  const int KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
+  // From N and K alone, so that a token's sums do not depend on the other tokens: 256 rows per CTA
+  // where that leaves enough CTAs, and as many splits of K as keep every cluster resident at once
+  // (two CTAs an SM; clusters of up to eight pack into about 264 of the 296 places).
+  const int KW = N >= 6400 ? 1 : 2;
+  const int tiles = (N + 256 / KW - 1) / (256 / KW);
+  const int S = std::max(1, std::min({LIN_CLUSTER, 264 / tiles, KB / KW}));
+  if (KW == 1) return launch_linear_kw<TX, TO, NT, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, S, st, pdl);
+  return launch_linear_kw<TX, TO, NT, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, S, st, pdl);
 }
 
 template <typename TX, typename TO>
@@ -224,7 +303,9 @@ int launch_linear_t(const void* x, int64_t ldx, int M, const void* codes, const 
                     void* out, int64_t ldo, cudaStream_t st, bool pdl) {
   if (M <= 8) return launch_linear_nt<TX, TO, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
   if (M <= 16) return launch_linear_nt<TX, TO, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
-  if (M <= 32) return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  // tokens beyond one tile's read the weight again; three-part fp32 rows leave no room for 64 of them
+  if (M <= 32 || sizeof(TX) == 4)
+    return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
   return launch_linear_nt<TX, TO, 8>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
 }
 

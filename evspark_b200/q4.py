@@ -44,14 +44,21 @@ def _need_cuda(t: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} must be a CUDA tensor")
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() builds a Stream object: 2 us a call
+_fns: dict = {}
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """One library call on the current stream of ``device``."""
-    fn = getattr(N.lib(), name)
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(N.lib(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = fn(*args, _raw_stream(index))
     if status:
         N.check(status, name)
 
@@ -83,6 +90,7 @@ class Q4Weight:
             raise ValueError("Q4Weight: codes and scales on different devices")
         _need_cuda(codes, "Q4Weight: codes")
         self.codes, self.scales, self.shape, self.group = codes, scales, (n, k), int(group)
+        self._args = (codes.data_ptr(), scales.data_ptr(), n, k, self.group)
 
     @property
     def device(self) -> torch.device:
@@ -131,31 +139,30 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
     block: every 64 rows read the weight once."""
     n, k = w.shape
     dt = _dtype(x, "q4_linear: x")
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"q4_linear: x must be [..., {k}], got {tuple(x.shape)}")
-    if x.device != w.codes.device:
-        raise ValueError(f"q4_linear: x on {x.device}, the weight on {w.codes.device}")
+    shape, dev = x.shape, w.codes.device
+    if not shape or shape[-1] != k:
+        raise ValueError(f"q4_linear: x must be [..., {k}], got {tuple(shape)}")
+    if x.device != dev:
+        raise ValueError(f"q4_linear: x on {x.device}, the weight on {dev}")
     if out is not None:
-        if out.shape != (*x.shape[:-1], n) or out.device != x.device or not out.is_contiguous():
+        if out.shape != (*shape[:-1], n) or out.device != dev or not out.is_contiguous():
             raise ValueError(f"q4_linear: out must be a contiguous [..., {n}] tensor of x's batch shape and device")
-        _dtype(out, "q4_linear: out")
+        odt = _dtype(out, "q4_linear: out")
     else:
-        if out_dtype not in _DT:
+        odt = _DT.get(out_dtype)
+        if odt is None:
             raise ValueError(f"q4_linear: out_dtype must be bf16 or fp32, got {out_dtype}")
-        out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
-    if x.numel() == 0:
+        out = torch.empty((*shape[:-1], n), dtype=out_dtype, device=dev)
+    m = x.numel() // k
+    if m == 0:
         return out
-    if x.dim() == 1:
-        ldx = k
-        if k > 1 and x.stride(0) != 1:
+    ldx = k
+    if not x.is_contiguous():
+        if len(shape) == 2 and x.stride(1) == 1 and x.stride(0) >= k:
+            ldx = x.stride(0)
+        else:
             x = x.contiguous()
-    elif x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= k:
-        ldx = x.stride(0)
-    else:
-        x = x.contiguous()
-        ldx = k
-    _call(x.device, "evs_q4_linear", x.data_ptr(), dt, ldx, x.numel() // k, w.codes.data_ptr(), w.scales.data_ptr(), n,
-          k, w.group, out.data_ptr(), _DT[out.dtype], n)
+    _call(dev, "evs_q4_linear", x.data_ptr(), dt, ldx, m, *w._args, out.data_ptr(), odt, n)
     return out
 
 
@@ -209,6 +216,7 @@ class Q4Cache:
         self._err = torch.zeros(3, dtype=torch.int32, device=pool.device)
         self._desc = N.Q4CacheDesc(pool.data_ptr(), self._err.data_ptr(), num_pages, page_size, kv_heads, head_dim)
         self._ref = C.addressof(self._desc)
+        self._workspace: dict = {}  # attention workspace bytes by call sizes
 
     @property
     def device(self) -> torch.device:
@@ -223,9 +231,11 @@ class Q4Cache:
                              f"or a page id outside the pool [evs status {code}, kernel {where}]")
 
 
+_Strides = C.c_int64 * 3
+
+
 def _strides(t: torch.Tensor):
-    s = t.stride()
-    return (C.c_int64 * 3)(s[0], s[1], s[2])
+    return _Strides(*t.stride()[:3])
 
 
 def _rows(cache: Q4Cache, page_table, lengths, counts, batch: int, tokens: int, what: str):
@@ -345,7 +355,13 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
         return out
     ml = 0 if max_length is None else int(max_length)
     rp = C.byref(rows)
-    need = N.lib().evs_q4_attention_workspace(cache._ref, rp, H, ml)
+    sizes = (B, T, H, ml or rows.max_pages * cache.page_size)
+    need = cache._workspace.get(sizes)
+    if need is None:
+        need = N.lib().evs_q4_attention_workspace(cache._ref, rp, H, ml)
+        if len(cache._workspace) >= 256:
+            cache._workspace.clear()
+        cache._workspace[sizes] = need
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(dev, "evs_q4_attention", cache._ref, rp, q.data_ptr(), _strides(q), H,
           cache.head_dim ** -0.5 if scale is None else float(scale), ml, out.data_ptr(), _strides(out), dt,
