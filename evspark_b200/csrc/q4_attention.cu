@@ -4,12 +4,13 @@
 // Split-KV. A warp takes a unit of consecutive keys for a tile of 16 query rows (a row is one token
 // of one query head of the kv head) and runs an online softmax over it; the four units of a CTA are
 // folded in order, and a second kernel folds the CTAs' partial results in order.  The unit's length
-// depends on the row's own position alone (64 keys below 4096, 256 below 65536, else 1024), so a
+// depends on the row's own position alone (64 keys below 4096, 256 below 131072, else 512), so a
 // token's result does not depend on what else is in the call: verify blocks and single steps agree
 // bit for bit.
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "internal.hpp"
 #include "q4.cuh"
@@ -20,12 +21,13 @@ namespace {
 constexpr int QA_WARPS = 4;
 constexpr int QA_THREADS = 32 * QA_WARPS;
 constexpr int QA_ROWS = 16;
-constexpr int QA_STEP = 32;  // keys per online-softmax step of a warp
+constexpr int NS = 2;           // 16-key chunks per online-softmax step of a warp
+constexpr int QA_STEP = 16 * NS;
 
 // length class of a position, and keys per CTA of a class
-__host__ __device__ constexpr int qa_class(int64_t pos) { return pos < 4096 ? 0 : (pos < 65536 ? 1 : 2); }
-__host__ __device__ constexpr int64_t qa_class_end(int cl) { return cl == 0 ? 4096 : (cl == 1 ? 65536 : (1ll << 40)); }
-__host__ __device__ constexpr int qa_cta_keys(int cl) { return 256 << (2 * cl); }
+__host__ __device__ constexpr int qa_class(int64_t pos) { return pos < 4096 ? 0 : (pos < 131072 ? 1 : 2); }
+__host__ __device__ constexpr int64_t qa_class_end(int cl) { return cl == 0 ? 4096 : (cl == 1 ? 131072 : (1ll << 40)); }
+__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 256 : (cl == 1 ? 1024 : 2048); }
 // partial results of one row for lengths up to bound
 inline int qa_slots(int64_t bound) {
   int n = 1;
@@ -36,18 +38,6 @@ inline int qa_slots(int64_t bound) {
   }
   return n;
 }
-
-template <int DH>
-struct KTile {  // 32 keys: per 16-key chunk two 8-key tiles, features c DH / 4 .. of one key each
-  uint32_t w[2][2][DH / 32];
-  uint32_t s[2][2];
-};
-template <int DH>
-struct VTile {  // 32 keys: per 16-key chunk the features g DH / 8 .. of the keys 4 c .. 4 c + 3
-  static constexpr int NW = DH / 64 > 0 ? DH / 64 : 1;
-  uint32_t w[2][4][NW];
-  uint32_t s[2][2];
-};
 
 template <int NW>
 __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
@@ -66,16 +56,46 @@ __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
 // carries into the sign bit)
 __device__ __forceinline__ uint32_t scales_nan(uint32_t s2) { return (s2 + 0x00800080u) & 0x80008000u; }
 
+// 2^x to two units in the last place, 0 below 2^-126
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int qa_parts_q(size_t elem) { return elem == 2 ? 1 : 3; }  // bf16 parts of a query value
+constexpr int qa_parts_p(size_t elem) { return elem == 2 ? 2 : 3; }  // ... and of a probability
+
+// The K codes and scales of 32 keys, as one thread multiplies them: per 16-key chunk two 8-key tiles,
+// of which it holds key 4 (g / 2) + g % 2 + 2 u, features c DH / 4 .. + DH / 4 - 1.
+template <int DH>
+struct KTile {
+  uint32_t w[NS][2][DH / 32];
+  uint32_t s[NS][2];
+};
+// The V codes and scales: per 16-key chunk the keys 4 c .. 4 c + 3, features g DH / 8 .. + DH / 8 - 1.
+template <int DH>
+struct VTile {
+  static constexpr int NW = DH / 64 > 0 ? DH / 64 : 1;
+  uint32_t w[NS][4][NW];
+  uint32_t s[NS][2];
+};
+
+// floats of the staged queries
 template <typename T, int DH>
-__global__ void __launch_bounds__(QA_THREADS)
+__host__ __device__ constexpr int qa_q_floats() {
+  return qa_parts_q(sizeof(T)) * 2 * (DH / 32) * 32 * 4;
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
     q4_attn_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, int grp, int t0, int tc, int tiles, float scale_log2,
                    int nslots, float* __restrict__ part_o, float2* __restrict__ part_s) {
-  constexpr int NQ = sizeof(T) == 2 ? 1 : 3;  // bf16 parts of a query value
-  constexpr int NP = sizeof(T) == 2 ? 2 : 3;  // bf16 parts of a probability
-  constexpr int KW = DH / 32;                 // code words per thread and key (K)
-  constexpr int VN = DH / 8;                  // 8-feature tiles of the output
+  constexpr int NQ = qa_parts_q(sizeof(T)), NP = qa_parts_p(sizeof(T));
+  constexpr int KW = DH / 32;  // code words per thread and key (K)
+  constexpr int VN = DH / 8;   // 8-feature tiles of the output
   pdl_trigger();
-  extern __shared__ __align__(16) float qa_sm[];  // [warp][16][DH + 2]
+  extern __shared__ __align__(16) float qa_sm[];  // the queries, then [warp][16][DH + 2] results
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
   pdl_wait();
@@ -87,90 +107,101 @@ __global__ void __launch_bounds__(QA_THREADS)
   const int first = t0 + tile * QA_ROWS / grp;
   const int last = min(min(t0 + (tile * QA_ROWS + QA_ROWS - 1) / grp, t0 + tc - 1), count - 1);
   if (first > last) return;
-  const int64_t pmax = static_cast<int64_t>(len) + last;
-  const int cl0 = qa_class(static_cast<int64_t>(len) + first), cl1 = qa_class(pmax);
+  const int pmin = len + first, pmax = len + last;
+  const int cl0 = qa_class(pmin), cl1 = qa_class(pmax);
   if (static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl0) > pmax) return;
 
-  // this thread's two rows: tokens and positions (-1: no token)
-  int tok[2], pos[2];
+  // Queries as product operands: step 2 w covers the feature pairs (0,4) (1,5) of the word 8 w ..,
+  // step 2 w + 1 the pairs (2,6) (3,7), as q4_word decodes the keys; qs[part][step][lane].
+  uint4* qs = reinterpret_cast<uint4*>(qa_sm);
+  for (int i = threadIdx.x; i < 32 * KW; i += QA_THREADS) {
+    const int l = i & 31, w = i >> 5, lg = l >> 2, lc = l & 3;
+    uint32_t e[2][8][3];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = tile * QA_ROWS + g + 8 * i;
-    tok[i] = t0 + r / grp;
-    pos[i] = r < tc * grp && tok[i] < count ? len + tok[i] : -1;
-  }
-  // queries as product operands: step 2 w covers the feature pairs (0,4) (1,5) of the word 8 w ..,
-  // step 2 w + 1 the pairs (2,6) (3,7), as q4_word decodes the keys
-  uint32_t qa[NQ][2 * KW][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = tile * QA_ROWS + g + 8 * i;
-    const T* src = static_cast<const T*>(q.p) + b * q.sb + tok[i] * q.st + (kvh * grp + r % grp) * q.sh + c * (DH / 4);
-#pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      uint32_t e[8][3];
+    for (int h = 0; h < 2; ++h) {
+      const int r = tile * QA_ROWS + lg + 8 * h, t = t0 + r / grp;
+      const bool live = r < tc * grp && t < count;
+      const T* src =
+          static_cast<const T*>(q.p) + b * q.sb + t * q.st + (kvh * grp + r % grp) * q.sh + lc * (DH / 4) + 8 * w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (NQ == 1)
-          e[j][0] = pos[i] >= 0 ? __bfloat16_as_ushort(src[8 * w + j]) : 0u;
+          e[h][j][0] = live ? __bfloat16_as_ushort(src[j]) : 0u;
         else
-          q4_parts(pos[i] >= 0 ? to_f32<T>(src[8 * w + j]) : 0.f, e[j]);
-      }
-#pragma unroll
-      for (int p = 0; p < NQ; ++p) {
-        qa[p][2 * w][i] = e[0][p] | e[4][p] << 16;
-        qa[p][2 * w][2 + i] = e[1][p] | e[5][p] << 16;
-        qa[p][2 * w + 1][i] = e[2][p] | e[6][p] << 16;
-        qa[p][2 * w + 1][2 + i] = e[3][p] | e[7][p] << 16;
+          q4_parts(live ? to_f32<T>(src[j]) : 0.f, e[h][j]);
       }
     }
+#pragma unroll
+    for (int p = 0; p < NQ; ++p)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        qs[(p * 2 * KW + 2 * w + s) * 32 + l] =
+            make_uint4(e[0][2 * s][p] | e[0][2 * s + 4][p] << 16, e[1][2 * s][p] | e[1][2 * s + 4][p] << 16,
+                       e[0][2 * s + 1][p] | e[0][2 * s + 5][p] << 16, e[1][2 * s + 1][p] | e[1][2 * s + 5][p] << 16);
   }
-  const int64_t trow = b * rows.table_stride;
-  const int k_scales = cache.P * DH, v_codes = cache.P * (DH / 2), v_scales = k_scales + cache.P * (DH / 16);
-  const int kg = c * (DH / 4) / 32, vg = g * (DH / 8) / 32;  // this thread's scale groups
+  __syncthreads();
+
+  const int32_t* table = rows.table + b * rows.table_stride;
+  const int P = cache.P;
+  // byte offsets inside a block: this thread's K features and scale group, V features and scale group
+  const uint32_t k_off = c * (DH / 8) + (4 * (g >> 1) + (g & 1)) * (DH / 2);
+  const uint32_t ks_off = P * DH + 2 * ((c * (DH / 4) / 32) * P + 4 * (g >> 1) + (g & 1));
+  const uint32_t v_off = P * (DH / 2) + g * (DH / 16) + 4 * c * (DH / 2);
+  const uint32_t vs_off = P * DH + P * (DH / 16) + 2 * ((g * (DH / 8) / 32) * P + 4 * c);
+  const uint8_t* head_base = cache.block(0, kvh);
+  const size_t page_bytes = static_cast<size_t>(cache.G) * cache.block_bytes;
 
   for (int cl = cl0; cl <= cl1; ++cl) {
-    const int64_t kend64 = min(pmax, qa_class_end(cl) - 1) + 1;  // keys seen by some row of the class
+    const int kall = static_cast<int>(min(static_cast<int64_t>(pmax), qa_class_end(cl) - 1)) + 1;  // keys of the class
     const int unit = qa_cta_keys(cl) / QA_WARPS;
-    const int64_t kbeg64 = static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl) + warp * unit;
-    if (static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl) >= kend64) continue;
-    const int kbeg = static_cast<int>(kbeg64), kend = static_cast<int>(min(kend64, kbeg64 + unit));
+    if (static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl) >= kall) continue;
+    const int kbeg = blockIdx.x * qa_cta_keys(cl) + warp * unit, kend = min(kall, kbeg + unit);
+    // keys that every row of the class sees need no mask; rows of no token (or another class) take
+    // part unmasked, their results are dropped
+    const int clear = max(pmin, cl == 0 ? 0 : static_cast<int>(qa_class_end(cl - 1))) + 1;
     int lim[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) lim[i] = pos[i] >= 0 && qa_class(pos[i]) == cl ? pos[i] : -1;
+    for (int i = 0; i < 2; ++i) {
+      const int r = tile * QA_ROWS + g + 8 * i, t = t0 + r / grp;
+      lim[i] = r < tc * grp && t < count && qa_class(len + t) == cl ? len + t : INT32_MAX;
+    }
 
     float o[VN][4], m[2], l[2];
 #pragma unroll
     for (int n = 0; n < VN; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    m[0] = m[1] = -CUDART_INF_F;
-    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) m[i] = -CUDART_INF_F, l[i] = 0.f;
 
-    int page_of = -1;  // lane's page id of the 16-key chunk (step & ~15) * 2 + lane
+    // Pages: lane i holds the page id of the 16-key chunk 32 j + i of the unit (j: the last load);
+    // the slot of a chunk inside its page goes along.
+    int page_of = -1;
     auto load_pages = [&](int key) {
       const int kk = key + 16 * lane;
-      page_of = -1;
-      if (kk < kend) page_of = __ldg(rows.table + trow + kk / cache.P);
+      page_of = kk < kend ? __ldg(table + kk / P) : -1;
     };
-    // the block of the 16-key chunk starting at key, or null (no keys there, or a bad page)
-    auto chunk_of = [&](int key, int sub) -> const uint8_t* {
-      const int idx = ((key - kbeg) >> 4) + sub;
-      const int id = __shfl_sync(0xffffffffu, page_of, idx & 31);
-      if (key + 16 * sub >= kend || id < 0 || id >= cache.pages) return nullptr;
-      return cache.block(id, kvh);
-    };
+    auto page_at = [&](int key, int sub) { return __shfl_sync(0xffffffffu, page_of, (((key - kbeg) >> 4) + sub) & 31); };
     KTile<DH> kt;
+    VTile<DH> vt;
+    bool bad = false;
+    // pages of the step that the next V load reads, and of the step after
+    int vpage[NS], kpage[NS], slot[NS];
+    auto next_slot = [&](int s) { return s + 16 == P ? 0 : s + 16; };
     auto load_k = [&](int key) {
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const uint8_t* blk = chunk_of(key, sub);
-        const int slot0 = (key + 16 * sub) % cache.P;
+      for (int sub = 0; sub < NS; ++sub) {
+        const int id = kpage[sub];
+        const bool in = key + 16 * sub < kend;
+        if (in && static_cast<uint32_t>(id) < static_cast<uint32_t>(cache.pages)) {
+          const uint8_t* blk = head_base + id * page_bytes;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int slot = slot0 + 4 * (g >> 1) + (g & 1) + 2 * u;
-          if (blk != nullptr) {
-            ld_words<KW>(kt.w[sub][u], blk + slot * (DH / 2) + c * (DH / 8));
-            kt.s[sub][u] = __ldg(reinterpret_cast<const uint16_t*>(blk + k_scales) + kg * cache.P + slot);
-          } else {
+          for (int u = 0; u < 2; ++u) {
+            ld_words<KW>(kt.w[sub][u], blk + (k_off + (slot[sub] + 2 * u) * (DH / 2)));
+            kt.s[sub][u] = __ldg(reinterpret_cast<const uint16_t*>(blk + (ks_off + 2 * (slot[sub] + 2 * u))));
+          }
+        } else {
+          bad |= in;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
 #pragma unroll
             for (int w = 0; w < KW; ++w) kt.w[sub][u][w] = 0u;
             kt.s[sub][u] = 0x7FC0u;  // keys without a page: a NaN score for whoever sees them
@@ -178,22 +209,21 @@ __global__ void __launch_bounds__(QA_THREADS)
         }
       }
     };
-    VTile<DH> vt;
     auto load_v = [&](int key) {
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        const uint8_t* blk = chunk_of(key, sub);
-        const int slot = (key + 16 * sub) % cache.P + 4 * c;
-        if (blk != nullptr) {
+      for (int sub = 0; sub < NS; ++sub) {
+        const int id = vpage[sub];
+        if (key + 16 * sub < kend && static_cast<uint32_t>(id) < static_cast<uint32_t>(cache.pages)) {
+          const uint8_t* blk = head_base + id * page_bytes;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint8_t* p = blk + v_codes + (slot + j) * (DH / 2) + g * (DH / 16);
+            const uint8_t* p = blk + (v_off + (slot[sub] + j) * (DH / 2));
             if constexpr (DH == 32)
               vt.w[sub][j][0] = __ldg(reinterpret_cast<const uint16_t*>(p));
             else
               ld_words<VTile<DH>::NW>(vt.w[sub][j], p);
           }
-          const uint2 s = __ldg(reinterpret_cast<const uint2*>(blk + v_scales + 2 * (vg * cache.P + slot)));
+          const uint2 s = __ldg(reinterpret_cast<const uint2*>(blk + (vs_off + 2 * slot[sub])));
           vt.s[sub][0] = s.x, vt.s[sub][1] = s.y;
         } else {
 #pragma unroll
@@ -207,62 +237,86 @@ __global__ void __launch_bounds__(QA_THREADS)
 
     if (kbeg < kend) {
       load_pages(kbeg);
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) {
+        slot[sub] = sub == 0 ? kbeg % P : next_slot(slot[sub - 1]);
+        kpage[sub] = page_at(kbeg, sub);
+      }
       load_k(kbeg);
     }
     for (int key = kbeg; key < kend; key += QA_STEP) {
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) vpage[sub] = kpage[sub];
       load_v(key);
-      float s[2][2][4];
+      float s[NS][2][4];
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+        for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          s[sub][u][0] = s[sub][u][1] = s[sub][u][2] = s[sub][u][3] = 0.f;
-          const Q4Scale ks = q4_scale(kt.s[sub][u] | kt.s[sub][u] << 16);
+          for (int u = 0; u < 2; ++u) s[sub][u][0] = s[sub][u][1] = s[sub][u][2] = s[sub][u][3] = 0.f;
+      Q4Scale ks[NS][2];
 #pragma unroll
-          for (int w = 0; w < KW; ++w) {
-            uint32_t kv[4];
-            q4_word(kt.w[sub][u][w], ks, kv);
+      for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-            for (int p = NQ - 1; p >= 0; --p) {
-              q4_mma(s[sub][u], qa[p][2 * w][0], qa[p][2 * w][1], qa[p][2 * w][2], qa[p][2 * w][3], kv[0], kv[1]);
-              q4_mma(s[sub][u], qa[p][2 * w + 1][0], qa[p][2 * w + 1][1], qa[p][2 * w + 1][2], qa[p][2 * w + 1][3],
-                     kv[2], kv[3]);
+        for (int u = 0; u < 2; ++u) ks[sub][u] = q4_scale(kt.s[sub][u] | kt.s[sub][u] << 16);
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        uint32_t kv[NS][2][4];
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) q4_word(kt.w[sub][u][w], ks[sub][u], kv[sub][u]);
+#pragma unroll
+          for (int p = NQ - 1; p >= 0; --p)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 a = qs[(p * 2 * KW + 2 * w + h) * 32 + lane];
+#pragma unroll
+              for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  q4_mma(s[sub][u], a.x, a.y, a.z, a.w, kv[sub][u][2 * h], kv[sub][u][2 * h + 1]);
             }
-          }
-        }
+      }
       const int next = key + QA_STEP;
-      const VTile<DH> vc = vt;
-      bool bad_page = false;
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-        bad_page |= key + 16 * sub < kend && chunk_of(key, sub) == nullptr;
-      if (bad_page && lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
       if (next < kend) {
         if (((next - kbeg) & 511) == 0) load_pages(next);
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub) {
+          slot[sub] = next_slot(slot[sub == 0 ? NS - 1 : sub - 1]);
+          kpage[sub] = page_at(next, sub);
+        }
         load_k(next);
       }
-      // scores to probabilities: thread's keys of a chunk are 4 c + 2 u + (0, 1)
-      float mx[2] = {m[0], m[1]};
+      const bool masked = key + QA_STEP > clear;
+      if (masked) {  // thread's keys of a chunk are 4 c + 2 u + (0, 1)
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+          for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int kk = key + 16 * sub + 4 * c + 2 * u + (e & 1);
-            const float v = kk <= lim[e >> 1] ? s[sub][u][e] * scale_log2 : -CUDART_INF_F;
-            s[sub][u][e] = v;
-            mx[e >> 1] = fmaxf(mx[e >> 1], v);
-          }
+              for (int e = 0; e < 4; ++e)
+                if (key + 16 * sub + 4 * c + 2 * u + (e & 1) > lim[e >> 1]) s[sub][u][e] = -CUDART_INF_F;
+      }
+      float mx[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mx[i] = m[i];
+#pragma unroll
+        for (int sub = 0; sub < NS; ++sub)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[sub][u][e]);
+      bool moved = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        moved |= mx[i] != m[i];
       }
-      if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float a = mx[i] == m[i] ? 1.f : exp2f(m[i] - mx[i]);
+          const float a = mx[i] == m[i] ? 1.f : ex2((m[i] - mx[i]) * scale_log2);
           m[i] = mx[i];
           l[i] *= a;
 #pragma unroll
@@ -272,16 +326,19 @@ __global__ void __launch_bounds__(QA_THREADS)
           }
         }
       }
-      const float mu[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0], m[1] == -CUDART_INF_F ? 0.f : m[1]};
+      float mu[2];
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        // probabilities as bf16 parts: a[p] = keys (4 c, 4 c + 1) of rows g, g + 8, then (4 c + 2, 4 c + 3)
+      for (int i = 0; i < 2; ++i) mu[i] = m[i] == -CUDART_INF_F ? 0.f : -m[i] * scale_log2;
+#pragma unroll
+      for (int sub = 0; sub < NS; ++sub) {
+        // probabilities as bf16 parts: keys (4 c, 4 c + 1) of rows g, g + 8, then (4 c + 2, 4 c + 3)
         uint32_t pa[NP][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p0 = exp2f(s[sub][u][2 * i] - mu[i]), p1 = exp2f(s[sub][u][2 * i + 1] - mu[i]);
+            const float p0 = ex2(fmaf(s[sub][u][2 * i], scale_log2, mu[i]));
+            const float p1 = ex2(fmaf(s[sub][u][2 * i + 1], scale_log2, mu[i]));
             l[i] += p0 + p1;
             float r0 = p0, r1 = p1;
 #pragma unroll
@@ -294,10 +351,10 @@ __global__ void __launch_bounds__(QA_THREADS)
               }
             }
           }
-        uint32_t vs[2] = {vc.s[sub][0], vc.s[sub][1]};
-        // keys behind the last visible one hold whatever the page held: their scale becomes 0
-        const int k4 = key + 16 * sub + 4 * c;
-        if (k4 + 4 > kend) {
+        uint32_t vs[2] = {vt.s[sub][0], vt.s[sub][1]};
+        if (masked) {
+          // keys behind the last visible one hold whatever the page held: their scale becomes 0
+          const int k4 = key + 16 * sub + 4 * c;
           if (k4 >= kend) vs[0] &= 0xFFFF0000u;
           if (k4 + 1 >= kend) vs[0] &= 0x0000FFFFu;
           if (k4 + 2 >= kend) vs[1] &= 0xFFFF0000u;
@@ -334,19 +391,19 @@ __global__ void __launch_bounds__(QA_THREADS)
         for (int n4 = 0; n4 < VN / 4; ++n4) {
           const int w = n4 >> 1;
           const uint32_t sel = (n4 & 1) ? 0x7632u : 0x5410u;
-          const uint32_t t01 = __byte_perm(vc.w[sub][0][w], vc.w[sub][1][w], sel);
-          const uint32_t t23 = __byte_perm(vc.w[sub][2][w], vc.w[sub][3][w], sel);
           uint32_t b01[4], b23[4];
-          q4_word(t01, s01, b01);
-          q4_word(t23, s23, b23);
+          q4_word(__byte_perm(vt.w[sub][0][w], vt.w[sub][1][w], sel), s01, b01);
+          q4_word(__byte_perm(vt.w[sub][2][w], vt.w[sub][3][w], sel), s23, b23);
+          // the parts of one output tile apart from each other: a product takes 20 cycles to follow itself
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p)
-              q4_mma(o[4 * n4 + j], pa[p][0], pa[p][1], pa[p][2], pa[p][3], b01[j], b23[j]);
+            for (int j = 0; j < 4; ++j)
+                q4_mma(o[4 * n4 + j], pa[p][0], pa[p][1], pa[p][2], pa[p][3], b01[j], b23[j]);
         }
       }
     }
+    if (__any_sync(0xffffffffu, bad) && lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
@@ -354,42 +411,40 @@ __global__ void __launch_bounds__(QA_THREADS)
     }
     // the four units folded in order
     constexpr int LD = DH + 2;
-    float* mine = qa_sm + warp * QA_ROWS * LD;
+    float* res = qa_sm + qa_q_floats<T, DH>();
+    float* mine = res + warp * QA_ROWS * LD;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float* row = mine + (g + 8 * i) * LD;
 #pragma unroll
-      for (int n = 0; n < VN; ++n) {
-        row[2 * c * VN + n] = o[n][2 * i];
-        row[(2 * c + 1) * VN + n] = o[n][2 * i + 1];
+      for (int n = 0; n < VN; n += 2) {
+        *reinterpret_cast<float2*>(row + 2 * c * VN + n) = make_float2(o[n][2 * i], o[n + 1][2 * i]);
+        *reinterpret_cast<float2*>(row + (2 * c + 1) * VN + n) = make_float2(o[n][2 * i + 1], o[n + 1][2 * i + 1]);
       }
-      if (c == 0) {
-        row[DH] = m[i];
-        row[DH + 1] = l[i];
-      }
+      if (c == 0) *reinterpret_cast<float2*>(row + DH) = make_float2(m[i] * scale_log2, l[i]);
     }
     __syncthreads();
     for (int r = warp; r < QA_ROWS; r += QA_WARPS) {
       const int R = tile * QA_ROWS + r, t = t0 + R / grp;
-      if (R >= tc * grp || t >= count || qa_class(static_cast<int64_t>(len) + t) != cl) continue;
+      if (R >= tc * grp || t >= count || qa_class(len + t) != cl) continue;
       float mw[QA_WARPS], big = -CUDART_INF_F;
 #pragma unroll
       for (int w = 0; w < QA_WARPS; ++w) {
-        mw[w] = qa_sm[(w * QA_ROWS + r) * LD + DH];
+        mw[w] = res[(w * QA_ROWS + r) * LD + DH];
         big = fmaxf(big, mw[w]);
       }
       float sum = 0.f, f[QA_WARPS];
 #pragma unroll
       for (int w = 0; w < QA_WARPS; ++w) {
-        f[w] = mw[w] == -CUDART_INF_F ? 0.f : exp2f(mw[w] - big);
-        sum += qa_sm[(w * QA_ROWS + r) * LD + DH + 1] * f[w];
+        f[w] = mw[w] == -CUDART_INF_F ? 0.f : ex2(mw[w] - big);
+        sum += res[(w * QA_ROWS + r) * LD + DH + 1] * f[w];
       }
       const size_t prow =
           ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots + blockIdx.x;
       for (int d = lane; d < DH; d += 32) {
         float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < QA_WARPS; ++w) acc += qa_sm[(w * QA_ROWS + r) * LD + d] * f[w];
+        for (int w = 0; w < QA_WARPS; ++w) acc += res[(w * QA_ROWS + r) * LD + d] * f[w];
         part_o[prow * DH + d] = acc;
       }
       if (lane == 0) part_s[prow] = make_float2(big, sum);
@@ -401,7 +456,7 @@ __global__ void __launch_bounds__(QA_THREADS)
 // One warp per output row: the CTAs' partial results folded in order.
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS)
-    q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int tc, int tiles, int nslots,
+    q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int tc, int prows, int nslots,
                       const float* __restrict__ part_o, const float2* __restrict__ part_s) {
   pdl_trigger();
   pdl_wait();
@@ -419,7 +474,7 @@ __global__ void __launch_bounds__(QA_THREADS)
   }
   const int64_t pos = static_cast<int64_t>(len) + t;
   const int n = static_cast<int>(pos / qa_cta_keys(qa_class(pos))) + 1;
-  const size_t prow = ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots;
+  const size_t prow = ((static_cast<size_t>(b) * cache.G + kvh) * static_cast<size_t>(prows) + R) * nslots;
   if (n > nslots) {  // max_length was below this row's length
     for (int d = lane; d < DH; d += 32) dst[d] = from_f32<T>(CUDART_NAN_F);
     if (lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
@@ -434,7 +489,7 @@ __global__ void __launch_bounds__(QA_THREADS)
 #pragma unroll 4
   for (int x = 0; x < n; ++x) {
     const float2 st = part_s[prow + x];
-    const float f = st.x == -CUDART_INF_F ? 0.f : exp2f(st.x - big);
+    const float f = st.x == -CUDART_INF_F ? 0.f : ex2(st.x - big);
     sum += st.y * f;
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) acc[d] += part_o[(prow + x) * DH + 32 * d + lane] * f;
@@ -443,28 +498,31 @@ __global__ void __launch_bounds__(QA_THREADS)
   for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
 }
 
+inline int64_t padded_rows(int64_t rows) { return (rows + QA_ROWS - 1) / QA_ROWS * QA_ROWS; }
+
 template <typename T, int DH>
 int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& out, int H, float scale,
                 int64_t bound, float* ws, int64_t ws_floats, cudaStream_t st, bool pdl) {
   const int grp = H / c.G, nslots = qa_slots(bound);
   auto* kern = q4_attn_kernel<T, DH>;
-  const int smem = QA_WARPS * QA_ROWS * (DH + 2) * 4;
+  const int smem = (qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2)) * 4;
   static std::atomic<unsigned long long> done{0};
   EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
   // tokens per pass: as many as the workspace holds partial results for
   const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
-  const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles per pass
-  int tokens = static_cast<int>(std::min<int64_t>(r.T, fit * QA_ROWS / grp));
-  EVS_CHECK_RANGE(fit >= 1 && tokens >= 1, "q4 attention: the workspace is too small");
+  const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles
+  const int tokens = static_cast<int>(std::min<int64_t>(r.T, fit * QA_ROWS / grp));
+  EVS_CHECK_RANGE(tokens >= 1, "q4 attention: the workspace is too small");
   for (int t0 = 0; t0 < r.T; t0 += tokens) {
     const int tc = std::min(tokens, r.T - t0);
-    const int tiles = (tc * grp + QA_ROWS - 1) / QA_ROWS;
+    const int prows = static_cast<int>(padded_rows(static_cast<int64_t>(tc) * grp)), tiles = prows / QA_ROWS;
     float* po = ws;
-    float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * tiles * QA_ROWS * nslots * DH);
+    float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * prows * nslots * DH);
     EVS_CUDA_TRY(evs_launch(kern, dim3(nslots, c.G * tiles, r.B), dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc,
                             tiles, scale * 1.4426950408889634f, nslots, po, ps));
+    // the combine may start while the last tiles run (it waits for them before it reads)
     EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3((tc * grp + QA_WARPS - 1) / QA_WARPS, c.G, r.B),
-                            dim3(QA_THREADS), 0, st, pdl, c, r, out, grp, t0, tc, tiles, nslots,
+                            dim3(QA_THREADS), 0, st, true, c, r, out, grp, t0, tc, prows, nslots,
                             static_cast<const float*>(po), static_cast<const float2*>(ps)));
     evs_count_launch(2);
   }
@@ -494,13 +552,12 @@ int launch_q4_attention(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor&
 }
 
 int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound) {
-  // all row tiles in one pass where that takes at most 256 MiB, else as many as fit
+  // every row in one pass where that takes at most 256 MiB, else as many as fit (a token at least)
   const int grp = H / G;
-  const int64_t per_tile = static_cast<int64_t>(B) * G * QA_ROWS * qa_slots(bound) * (D + 2) * 4;
-  const int64_t least = (std::max(grp, 1) + QA_ROWS - 1) / QA_ROWS;  // one token
-  const int64_t all = (static_cast<int64_t>(T) * grp + QA_ROWS - 1) / QA_ROWS;
-  const int64_t want = std::min(all, std::max<int64_t>(least, (256ll << 20) / per_tile));
-  return want * per_tile;
+  const int64_t per_row = static_cast<int64_t>(B) * G * qa_slots(bound) * (D + 2) * 4;
+  const int64_t all = padded_rows(static_cast<int64_t>(T) * grp), least = padded_rows(grp);
+  const int64_t fit = (256ll << 20) / per_row / QA_ROWS * QA_ROWS;
+  return std::min(all, std::max(least, fit)) * per_row;
 }
 
 extern "C" {
@@ -522,6 +579,7 @@ int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 attention: q must be fp32 or bf16");
   EVS_CHECK_ARG(n_heads >= cache->kv_heads && n_heads % cache->kv_heads == 0,
                 "q4 attention: n_heads must be a multiple of kv_heads");
+  EVS_CHECK_ARG(scale > 0.f && std::isfinite(scale), "q4 attention: scale must be positive");
   EVS_CHECK_ARG(max_length >= 0, "q4 attention: max_length must not be negative");
   EVS_CHECK_ARG(cache->kv_heads <= 65535 && rows->batch <= 65535, "q4 attention: too many heads or rows");
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "q4 attention: the workspace must be 16-byte aligned");

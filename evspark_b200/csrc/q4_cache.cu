@@ -9,6 +9,7 @@
 // read-modify-write.  Page ids and lengths are checked before any access: a bad one is recorded in
 // the cache's error word and the token is skipped.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "internal.hpp"
@@ -18,6 +19,7 @@
 namespace {
 
 constexpr int APP_THREADS = 256;
+constexpr int FEW_TOKENS = 296;  // two CTAs an SM
 constexpr int FREQ_MAX = 64;  // head_dim / 2 at most
 
 struct RopeFreq {
@@ -65,17 +67,45 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec) {
   }
 }
 
-// One CTA per (token, block of head rows).  D / 16 threads per head row, each holding the features
-// 8 i .. 8 i + 7 of the row's lower half and of its upper half (the pairs that the rotation turns).
-// Rows 0 .. H - 1 are queries, then G keys, then G values.
+// Scale and codes of a group are decided in fp32 wherever that cannot differ from 64 bits, else in 64
+// bits.  Scale: t = absmax / 7 in fp32 is within 2^-22 of the exact quotient, so its five-bit rounding
+// is the exact one unless the dropped 19 bits lie within 4 units of a half (one group in 2^15).
+// Codes: the quotient x / s, corrected once by its exact remainder, is within 2^-23 of the exact one
+// (|x / s| < 8), and is a half exactly where x is; its rounding is the exact one unless it lies within
+// 2^-15 of a half.  Values, which are x themselves, may sit on a half (bf16 ones often do: x has eight
+// bits and s five, so x / s is a half or 2^-6 away from one); keys, rotated in 64 bits, are looked at
+// again there.
+__device__ __forceinline__ bool scale_clear(float absmax) {
+  const float t = absmax * (1.f / 7.f);
+  return (__float_as_uint(t) & 0x7FFFFu) - 0x3FFFCu > 8u && t >= 2.f * Q4_TINY && t <= 0.5f * Q4_HUGE;
+}
+__device__ __forceinline__ uint32_t scale_bits_fast(float absmax) {
+  return (__float_as_uint(absmax * (1.f / 7.f)) + 0x40000u) >> 19 << 3;  // five significant bits, as bf16 bits
+}
+// code of x under scale s (inv = 1 / s to 2^-22), and the largest distance from its code's value so
+// far (a half of a value is no distance); adding 1.5 2^23 leaves the rounded quotient in the low bits
+__device__ __forceinline__ uint32_t code_fast(float x, float s, float inv, bool value, float& far) {
+  float q = x * inv;
+  q = fmaf(fmaf(-q, s, x), inv, q);
+  q = fminf(fmaxf(q, -7.25f), 7.25f);
+  const float y = q + 12582912.f, d = fabsf(q - (y - 12582912.f));
+  far = value && d == 0.5f ? far : fmaxf(far, d);
+  return __float_as_uint(y) - (0x4B400000u - 8u);
+}
+
+// One CTA per token (and block of head rows, where the call has few tokens).  D / 16 threads per head
+// row, each holding the features 8 i .. 8 i + 7 of the row's lower half and of its upper half (the
+// pairs that the rotation turns).  Rows 0 .. H - 1 are queries, then G keys, then G values.  Angles
+// and rotation in 64 bits (2 of the 64 fma a clock that an SM has per value: not what bounds this), so
+// that a key's codes are those of its exact rotation.
 template <typename T>
-__global__ void __launch_bounds__(APP_THREADS)
+__global__ void __launch_bounds__(APP_THREADS, 4)
     q4_append_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, Q4Tensor k, Q4Tensor v, Q4Tensor q_out, int H,
                      int vec, const __grid_constant__ RopeFreq freq) {
   pdl_trigger();
-  __shared__ double cs[FREQ_MAX], sn[FREQ_MAX];
+  __shared__ double2 turn[8][FREQ_MAX / 8];  // cos, sin of feature 8 i + j at [j][i]
   pdl_wait();
-  const int b = blockIdx.x / rows.T, t = blockIdx.x % rows.T;
+  const int b = blockIdx.x / rows.T, t = blockIdx.x - b * rows.T;
   int len, count;
   if (!q4_row(rows, b, &len, &count, cache.P)) {
     if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
@@ -83,80 +113,133 @@ __global__ void __launch_bounds__(APP_THREADS)
   }
   if (t >= count) return;
   const int D = cache.D, half = D / 2, G = cache.G;
-  const int64_t pos = static_cast<int64_t>(len) + t;
-  if (threadIdx.x < half) sincos(static_cast<double>(pos) * freq.f[threadIdx.x], &sn[threadIdx.x], &cs[threadIdx.x]);
-  __syncthreads();
-  const int64_t page = q4_page(cache, rows, b, pos);
-  const int tpr = D / 16, per = APP_THREADS / tpr;
-  const int r = blockIdx.y * per + threadIdx.x / tpr, i = threadIdx.x % tpr;
-  const bool live = r < H + 2 * G;
-  if (page < 0 && threadIdx.x == 0 && blockIdx.y == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
+  const int pos = len + t;
+  const int tpr_log = D == 128 ? 3 : (D == 64 ? 2 : 1), per = APP_THREADS >> tpr_log;
+  const int total = H + 2 * G;
+  const int i = threadIdx.x & ((1 << tpr_log) - 1);
+  int r = blockIdx.y * per + (threadIdx.x >> tpr_log);
+  const T* q_at = static_cast<const T*>(q.p) + b * q.sb + t * q.st + 8 * i;
+  const T* k_at = static_cast<const T*>(k.p) + b * k.sb + t * k.st + 8 * i;
+  const T* v_at = static_cast<const T*>(v.p) + b * v.sb + t * v.st + 8 * i;
   float lo[8], hi[8];
+  auto load = [&](int row) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 0.f;
-  const bool is_q = r < H, is_k = !is_q && r < H + G;
-  const int head = is_q ? r : (is_k ? r - H : r - H - G);
-  if (live) {
-    const Q4Tensor& src = is_q ? q : (is_k ? k : v);
-    const T* p = static_cast<const T*>(src.p) + b * src.sb + t * src.st + head * src.sh + 8 * i;
+    for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 0.f;
+    if (row >= total) return;
+    const T* p = row < H ? q_at + row * q.sh : (row < H + G ? k_at + (row - H) * k.sh : v_at + (row - H - G) * v.sh);
     load8<T>(lo, p, vec != 0);
     load8<T>(hi, p + half, vec != 0);
+  };
+  load(r);  // on its way while the angles are computed
+  if (threadIdx.x < half && static_cast<int>(blockIdx.y) * per < H + G) {
+    double s, c;
+    sincos(static_cast<double>(pos) * freq.f[threadIdx.x], &s, &c);
+    turn[threadIdx.x & 7][threadIdx.x >> 3] = make_double2(c, s);
   }
-  double xl[8], xh[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    xl[j] = lo[j];
-    xh[j] = hi[j];
+  __syncthreads();
+  const int64_t page = q4_page(cache, rows, b, pos);
+  const int slot = pos % cache.P;
+  if (page < 0 && threadIdx.x == 0 && blockIdx.y == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
+  // rows of one pass share the count of passes, so that whole warps meet the shuffles below
+  for (int r0 = blockIdx.y * per; r0 < total; r0 += gridDim.y * per, r += gridDim.y * per) {
+    const bool live = r < total, is_q = r < H, is_k = !is_q && r < H + G;
+    const int head = is_q ? r : (is_k ? r - H : r - H - G);
     if (is_q || is_k) {
-      const double c = cs[8 * i + j], s = sn[8 * i + j];
-      const double a = xl[j] * c - xh[j] * s, d = xh[j] * c + xl[j] * s;
-      xl[j] = a;
-      xh[j] = d;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const double2 cs = turn[j][i];
+        const double a = lo[j], d = hi[j];
+        lo[j] = static_cast<float>(a * cs.x - d * cs.y);
+        hi[j] = static_cast<float>(d * cs.x + a * cs.y);
+      }
     }
-  }
-  if (live && is_q) {
-    T* o = static_cast<T*>(q_out.p) + b * q_out.sb + t * q_out.st + head * q_out.sh + 8 * i;
+    // the values in 64 bits (keys: read and rotated again, where fp32 does not decide)
+    auto exact = [&](int j, double& l, double& h) {
+      l = lo[j];
+      h = hi[j];
+      if (!is_k) return;
+      const double a = to_f32<T>(k_at[head * k.sh + j]), d = to_f32<T>(k_at[head * k.sh + half + j]);
+      const double2 cs = turn[j][i];
+      l = a * cs.x - d * cs.y;
+      h = d * cs.x + a * cs.y;
+    };
+    if (live && is_q) {
+      T* o = static_cast<T*>(q_out.p) + b * q_out.sb + t * q_out.st + head * q_out.sh + 8 * i;
+      store8<T>(o, lo, vec != 0);
+      store8<T>(o + half, hi, vec != 0);
+    }
+    // groups of 32 features: four threads of one half (D = 64, 128), or both halves of two threads (D = 32)
+    auto group_max = [&](auto& ml, auto& mh, auto larger) {
+      if (D == 32) ml = mh = larger(ml, mh);
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        if (D == 32 && o == 2) break;
+        ml = larger(ml, __shfl_xor_sync(0xffffffffu, ml, o));
+        mh = larger(mh, __shfl_xor_sync(0xffffffffu, mh, o));
+      }
+    };
+    // magnitudes as integers: the same order, with every NaN on top
+    uint32_t bl = 0, bh = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      lo[j] = static_cast<float>(xl[j]);
-      hi[j] = static_cast<float>(xh[j]);
+      bl = max(bl, __float_as_uint(lo[j]) & 0x7FFFFFFFu);
+      bh = max(bh, __float_as_uint(hi[j]) & 0x7FFFFFFFu);
     }
-    store8<T>(o, lo, vec != 0);
-    store8<T>(o + half, hi, vec != 0);
-  }
-  // groups of 32 features: four threads of one half (D = 64, 128), or both halves of two threads (D = 32)
-  double ml = 0.0, mh = 0.0;
-  auto larger = [](double a, double o) { return (a != a || a >= o) ? a : o; };  // a NaN wins
+    group_max(bl, bh, [](uint32_t a, uint32_t o) { return max(a, o); });
+    const float ml = __uint_as_float(bl), mh = __uint_as_float(bh);
+    const bool put = live && !is_q && page >= 0;
+    uint32_t sl = scale_bits_fast(ml), sh = scale_bits_fast(mh);
+    if (__any_sync(0xffffffffu, put && !(scale_clear(ml) && scale_clear(mh)))) {
+      double el = 0.0, eh = 0.0;
+      auto larger = [](double a, double o) { return (a != a || a >= o) ? a : o; };  // a NaN wins
+      if (put) {
+        for (int j = 0; j < 8; ++j) {
+          double l, h;
+          exact(j, l, h);
+          el = larger(el, fabs(l));
+          eh = larger(eh, fabs(h));
+        }
+      }
+      group_max(el, eh, larger);
+      sl = q4_scale_bits(el);
+      sh = q4_scale_bits(eh);
+    }
+    if (put) {
+      const float fl = __uint_as_float(sl << 16), fh = __uint_as_float(sh << 16);
+      float il, ih;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(il) : "f"(fl));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ih) : "f"(fh));
+      uint32_t cl = 0, ch = 0;
+      float far = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    ml = larger(ml, fabs(xl[j]));
-    mh = larger(mh, fabs(xh[j]));
-  }
-  if (D == 32) ml = mh = larger(ml, mh);
-  const int width = D == 32 ? 2 : 4;
-  for (int o = 1; o < width; o <<= 1) {
-    ml = larger(ml, __shfl_xor_sync(0xffffffffu, ml, o));
-    mh = larger(mh, __shfl_xor_sync(0xffffffffu, mh, o));
-  }
-  if (!live || is_q || page < 0) return;
-  const uint32_t sl = q4_scale_bits(ml), sh = q4_scale_bits(mh);
-  uint32_t cl = 0, ch = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    cl |= q4_code(xl[j], sl) << (4 * j);
-    ch |= q4_code(xh[j], sh) << (4 * j);
-  }
-  const int slot = static_cast<int>(pos % cache.P);
-  uint8_t* block = cache.block(page, head);
-  uint8_t* codes = block + (is_k ? 0 : cache.P * (D / 2)) + slot * (D / 2);
-  *reinterpret_cast<uint32_t*>(codes + 4 * i) = cl;
-  *reinterpret_cast<uint32_t*>(codes + half / 2 + 4 * i) = ch;
-  uint16_t* scales = reinterpret_cast<uint16_t*>(block + cache.P * D) + (is_k ? 0 : cache.P * (D / 32)) + slot;
-  if (D == 32) {
-    if (i == 0) scales[0] = static_cast<uint16_t>(sl);
-  } else if (i % 4 == 0) {
-    scales[(i / 4) * cache.P] = static_cast<uint16_t>(sl);
-    scales[(i / 4 + D / 64) * cache.P] = static_cast<uint16_t>(sh);
+      for (int j = 0; j < 8; ++j) {
+        cl |= code_fast(lo[j], fl, il, !is_k, far) << (4 * j);
+        ch |= code_fast(hi[j], fh, ih, !is_k, far) << (4 * j);
+      }
+      // a scale of 0 or NaN makes every quotient infinite or NaN: the codes are 8
+      const bool odd = !(ml <= FLT_MAX) || !(mh <= FLT_MAX) || sl == 0u || sh == 0u || sl == 0x7FC0u || sh == 0x7FC0u;
+      if (far >= 0.5f - 0x1p-15f || odd) {
+        cl = ch = 0;
+        for (int j = 0; j < 8; ++j) {
+          double l, h;
+          exact(j, l, h);
+          cl |= q4_code(l, sl) << (4 * j);
+          ch |= q4_code(h, sh) << (4 * j);
+        }
+      }
+      uint8_t* block = cache.block(page, head);
+      uint8_t* codes = block + (is_k ? 0 : cache.P * (D / 2)) + slot * (D / 2);
+      *reinterpret_cast<uint32_t*>(codes + 4 * i) = cl;
+      *reinterpret_cast<uint32_t*>(codes + half / 2 + 4 * i) = ch;
+      uint16_t* scales = reinterpret_cast<uint16_t*>(block + cache.P * D) + (is_k ? 0 : cache.P * (D / 32)) + slot;
+      if (D == 32) {
+        if (i == 0) scales[0] = static_cast<uint16_t>(sl);
+      } else if (i % 4 == 0) {
+        scales[(i / 4) * cache.P] = static_cast<uint16_t>(sl);
+        scales[(i / 4 + D / 64) * cache.P] = static_cast<uint16_t>(sh);
+      }
+    }
+    if (r0 + static_cast<int>(gridDim.y) * per < total) load(r + gridDim.y * per);
   }
 }
 
@@ -166,35 +249,47 @@ __global__ void __launch_bounds__(APP_THREADS)
     q4_read_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor k, Q4Tensor v, int vec) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / rows.T, t = blockIdx.x % rows.T;
+  const int b = blockIdx.x / rows.T, t = blockIdx.x - b * rows.T;
   int len, count;
   if (!q4_row(rows, b, &len, &count, cache.P)) {
     if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
     return;
   }
   if (t >= count) return;
-  const int D = cache.D, G = cache.G, per = D / 8;
-  const int64_t pos = static_cast<int64_t>(len) + t;
+  const int D = cache.D, G = cache.G, log8 = D == 128 ? 4 : (D == 64 ? 3 : 2);
+  const int pos = len + t;
   const int64_t page = q4_page(cache, rows, b, pos);
   if (page < 0) {
     if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
     return;
   }
-  const int slot = static_cast<int>(pos % cache.P);
-  for (int i = threadIdx.x; i < 2 * G * per; i += APP_THREADS) {
-    const bool is_k = i < G * per;
-    const int head = (is_k ? i : i - G * per) / per, w = i % per;
-    const uint8_t* block = cache.block(page, head);
-    const uint32_t codes =
-        *reinterpret_cast<const uint32_t*>(block + (is_k ? 0 : cache.P * (D / 2)) + slot * (D / 2) + 4 * w);
-    const uint16_t sb = (reinterpret_cast<const uint16_t*>(block + cache.P * D))[(is_k ? 0 : cache.P * (D / 32)) +
-                                                                                 (w / 4) * cache.P + slot];
-    const float s = __uint_as_float(static_cast<uint32_t>(sb) << 16);
-    float x[8];
+  const int slot = pos % cache.P, units = 2 * G << log8;
+  const uint8_t* first = cache.block(page, 0);
+  constexpr int BATCH = 4;  // loads of a thread in flight
+  for (int i0 = blockIdx.y * APP_THREADS * BATCH + threadIdx.x; i0 < units; i0 += gridDim.y * APP_THREADS * BATCH) {
+    uint32_t codes[BATCH], sb[BATCH];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (static_cast<int>((codes >> (4 * j)) & 15u) - 8) * s;
-    const Q4Tensor& dst = is_k ? k : v;
-    store8<T>(static_cast<T*>(dst.p) + b * dst.sb + t * dst.st + head * dst.sh + 8 * w, x, vec != 0);
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
+      if (i >= units) continue;
+      const bool is_v = row >= G;
+      const uint8_t* block = first + static_cast<size_t>(is_v ? row - G : row) * cache.block_bytes;
+      codes[u] = __ldg(reinterpret_cast<const uint32_t*>(block + (is_v ? cache.P * (D / 2) : 0) + slot * (D / 2) + 4 * w));
+      sb[u] = __ldg(reinterpret_cast<const uint16_t*>(block + cache.P * D) + (is_v ? cache.P * (D / 32) : 0) +
+                    (w >> 2) * cache.P + slot);
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
+      if (i >= units) break;
+      const float s = __uint_as_float(sb[u] << 16);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = (static_cast<int>((codes[u] >> (4 * j)) & 15u) - 8) * s;
+      const Q4Tensor& dst = row >= G ? v : k;
+      store8<T>(static_cast<T*>(dst.p) + b * dst.sb + t * dst.st + (row >= G ? row - G : row) * dst.sh + 8 * w, x,
+                vec != 0);
+    }
   }
 }
 
@@ -210,7 +305,8 @@ int q4_check_cache(const evs_q4_cache* c) {
   EVS_CHECK_ARG(c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128, "q4 cache: head_dim must be 32, 64 or 128");
   EVS_CHECK_ARG(c->page_size >= 16 && c->page_size <= 4096 && c->page_size % 16 == 0,
                 "q4 cache: page_size must be a multiple of 16 in [16, 4096]");
-  EVS_CHECK_ARG(c->kv_heads >= 1 && c->num_pages >= 1, "q4 cache: needs kv_heads >= 1 and num_pages >= 1");
+  EVS_CHECK_ARG(c->kv_heads >= 1 && c->num_pages >= 1 && c->num_pages <= INT32_MAX,
+                "q4 cache: needs kv_heads >= 1 and num_pages in [1, 2^31)");
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(c->pool) % 16 == 0, "q4 cache: the pool must be 16-byte aligned");
   return EVS_OK;
 }
@@ -267,7 +363,10 @@ int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   RopeFreq f;
   for (int j = 0; j < c.D / 2; ++j) f.f[j] = std::pow(rope_base, -2.0 * j / c.D);
   const int per = APP_THREADS / (c.D / 16);
-  dim3 grid(rows->batch * rows->tokens, (H + 2 * c.G + per - 1) / per);
+  // few tokens: their head rows over several CTAs; many: one CTA a token, so that the angles of a
+  // token are computed once
+  const int tokens = rows->batch * rows->tokens;
+  dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (H + 2 * c.G + per - 1) / per);
   EVS_CHECK_ARG(grid.y <= 65535, "q4 append: too many heads");
   if (dtype == EVS_DTYPE_BF16)
     q4_append_kernel<__nv_bfloat16><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tq, tk, tv, to, H, vec, f);
@@ -288,7 +387,8 @@ int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, 
   const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
   const Q4Tensor tk = tensor_of(k, k_strides), tv = tensor_of(v, v_strides);
   const int vec = vec_ok(tk, el) && vec_ok(tv, el);
-  const int grid = rows->batch * rows->tokens;
+  const int tokens = rows->batch * rows->tokens;
+  const dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS));
   if (dtype == EVS_DTYPE_BF16)
     q4_read_kernel<__nv_bfloat16><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tk, tv, vec);
   else

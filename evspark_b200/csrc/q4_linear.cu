@@ -166,17 +166,25 @@ __global__ void __launch_bounds__(LIN_THREADS, NT <= 2 ? 2 : 1)
         uint32_t a[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) q4_word((&t.w[i].x)[w], s[i], a[i]);
+        // products of one sum apart from each other: a product takes 20 cycles to follow itself
+        constexpr int JB = NT < 2 ? NT : 2;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int j0 = 0; j0 < NT; j0 += JB)
 #pragma unroll
           for (int q = NP - 1; q >= 0; --q) {
-            const uint4 b = xb[((j * NP + q) * 4 + w) * 32 + (lane ^ (2 * w))];
+            uint4 b[JB];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float(&d)[4] = NP > 1 ? part[i][j] : acc[i][j];
-              q4_mma(d, a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1], b.x, b.y);
-              q4_mma(d, a[2 * i][2], a[2 * i + 1][2], a[2 * i][3], a[2 * i + 1][3], b.z, b.w);
-            }
+            for (int j = 0; j < JB; ++j) b[j] = xb[(((j0 + j) * NP + q) * 4 + w) * 32 + (lane ^ (2 * w))];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < JB; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  float(&d)[4] = NP > 1 ? part[i][j0 + j] : acc[i][j0 + j];
+                  q4_mma(d, a[2 * i][2 * h], a[2 * i + 1][2 * h], a[2 * i][2 * h + 1], a[2 * i + 1][2 * h + 1],
+                         h ? b[j].z : b[j].x, h ? b[j].w : b[j].y);
+                }
           }
       }
       if constexpr (NP > 1) {

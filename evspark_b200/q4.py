@@ -344,6 +344,8 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
     if H < 1 or H % cache.kv_heads:
         raise ValueError(f"q4_attention: heads ({H}) must be a multiple of kv_heads ({cache.kv_heads})")
     _heads(q, B, T, H, cache.head_dim, q.dtype, dev, "q4_attention: q")
+    if scale is not None and not 0.0 < scale < float("inf"):
+        raise ValueError(f"q4_attention: scale must be positive and finite, got {scale}")
     if max_length is not None and max_length < 1:
         raise ValueError(f"q4_attention: max_length must be positive, got {max_length}")
     rows = _rows(cache, page_table, lengths, counts, B, T, "q4_attention")
