@@ -76,9 +76,11 @@ _PROTOS = {
     "evs_device_check": (_I, []),
     "evs_model_create": (_I, [C.POINTER(ModelConfig), C.POINTER(_P)]),
     "evs_model_set_tensor": (_I, [_P, _I, _I, _P, C.c_int64]),
+    "evs_model_set_q4": (_I, [_P, _I, _I, _P, _P, _I, _I, _I]),
     "evs_model_finalize": (_I, [_P]),
     "evs_model_destroy": (None, [_P]),
     "evs_state_create": (_I, [_P, _I, _I, _I, C.POINTER(_P)]),
+    "evs_state_create_q4": (_I, [_P, _I, _I, _I, C.POINTER(_P)]),
     "evs_state_tp_handle": (_I, [_P, _P]),
     "evs_state_tp_connect": (_I, [_P, _P, _I]),
     "evs_state_tp_disconnect": (_I, [_P]),

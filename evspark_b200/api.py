@@ -115,14 +115,18 @@ class EvSpark:
     @classmethod
     def load(cls, ckpt: str | None = DEFAULT_CKPT, model_name: str = "evo2_7b", device: str = "cuda:0",
              use_kernels: bool = True, *, seed: int = 20260820, drafter_seed: int = 20260830,
-             max_chunk: int = 32) -> "EvSpark":
+             max_chunk: int = 32, weight_format: str | None = None, weight_group: int = 64,
+             kv_format: str | None = None) -> "EvSpark":
+        """``weight_format="q4"`` / ``kv_format="q4"``: the target's dense projections / KV cache in 4 bits
+        (``TargetModel``)."""
         import torch
 
         from evspark_b200.config import DRAFTERS, target_config
         from evspark_b200.drafter import DeviceDrafter, load_checkpoint, layer_index
-        from evspark_b200.model import TargetModel, require_device
+        from evspark_b200.model import TargetModel, check_formats, require_device
         from evspark_b200.specdec.block.neural_draft import NeuralDraftModel
 
+        check_formats(weight_format, weight_group, kv_format)
         if not use_kernels:
             raise ValueError("evspark_b200 has one compute path: the sm_100a kernels (use_kernels=True)")
         require_device(device)
@@ -137,7 +141,8 @@ class EvSpark:
             layers = DRAFTERS[model_name].inject_layers
         init_on = "cuda" if cfg.d_model >= 1024 else "cpu"
         model = TargetModel.random(cfg, seed=seed, device=device, init_on=init_on,
-                                   capture_layers=tuple(layer_index(n) for n in layers), max_chunk=max_chunk)
+                                   capture_layers=tuple(layer_index(n) for n in layers), max_chunk=max_chunk,
+                                   weight_format=weight_format, weight_group=weight_group, kv_format=kv_format)
         if path is not None and path.is_file():
             drafter, layers, meta = load_checkpoint(str(path), cfg.d_model, device=device)
         else:

@@ -912,6 +912,7 @@ int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, 
   EVS_CHECK_ARG(m->cfg.head_dim >= 32 && m->cfg.head_dim <= 128 && 256 % m->cfg.head_dim == 0,
                 "head_dim must be 32, 64 or 128");
   EVS_CHECK_RANGE(kv_blocks >= 1 && kv_blocks <= s->attn_blocks, "KV length beyond max_seqlen");
+  if (s->kv_q4) return launch_attention_q4(m, s, layer, B, T, splits, kv_blocks * ATTN_BLOCK, st);
   if (m->cfg.dtype == EVS_DTYPE_BF16) return launch_attention_t<__nv_bfloat16>(m, s, layer, B, T, splits, kv_blocks, st);
   return launch_attention_t<float>(m, s, layer, B, T, splits, kv_blocks, st);
 }

@@ -68,7 +68,13 @@ const void** slot_ptr(LayerDev& L, int slot) {
 // out: partial sums [splits][M][N] (s->ws, or a shared buffer of a row-parallel projection)
 int gemm(const evs_model* m, evs_state* s, const CUtensorMap* tA, const CUtensorMap* tA2, const void* W,
          const void* W2, int N, int K, int M, int dual, float* out, size_t out_floats, cudaStream_t st, int* splits,
-         const CUtensorMap* tB_override = nullptr) {
+         const CUtensorMap* tB_override = nullptr, const Q4Mat* q4 = nullptr) {
+  if (q4 != nullptr) {
+    EVS_CHECK_RANGE(static_cast<size_t>(M) * N <= out_floats, "projection workspace too small");
+    *splits = 1;
+    return launch_q4_linear(s->act, m->cfg.dtype, s->ld_act, M, q4->codes, q4->scales, N, K, q4->group, out,
+                            EVS_DTYPE_FP32, N, st, s->use_pdl());
+  }
   GemmPlan p = gemm_plan(m, N, K, M, dual);
   EVS_CHECK_RANGE(static_cast<size_t>(p.splits) * M * N <= out_floats, "split-K workspace too small");
   *splits = p.splits;
@@ -127,21 +133,25 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
   // one projection, timed with its algorithmic bytes (weights + activations in + fp32 partials out)
   const CUtensorMap* w3_act = nullptr;  // set when the w1/w2 projection wrote the fused SwiGLU output
   auto G = [&](const CUtensorMap* tA, const CUtensorMap* tA2, const void* W, const void* W2, int N, int K, int dual,
-               float* out = nullptr, size_t out_floats = 0, const CUtensorMap* tB = nullptr) {
+               float* out = nullptr, size_t out_floats = 0, const CUtensorMap* tB = nullptr,
+               const Q4Mat* q4 = nullptr) {
     const GemmPlan pl = gemm_plan(m, N, K, M, dual);
-    const double bytes = (static_cast<double>(N) * K + static_cast<double>(M) * K) * el + 4.0 * pl.splits * M * N;
+    double bytes = (static_cast<double>(N) * K + static_cast<double>(M) * K) * el + 4.0 * pl.splits * M * N;
+    if (q4 != nullptr)
+      bytes = static_cast<double>(N) * K * (0.5 + 2.0 / q4->group) + static_cast<double>(M) * (K * el + 4.0 * N);
     float* o = out != nullptr ? out : s->ws;
     const size_t of = out != nullptr ? out_floats : s->ws_floats;
     return timed(s, st, EVS_PROF_GEMM, bytes,
-                 [&] { return gemm(m, s, tA, tA2, W, W2, N, K, M, dual, o, of, st, &sp, tB); });
+                 [&] { return gemm(m, s, tA, tA2, W, W2, N, K, M, dual, o, of, st, &sp, tB, q4); });
   };
   // row-parallel projection [d x K] whose partial sums the next residual + RMSNorm adds up: with
   // channel sharding it writes to the shared buffer of reduction `epoch` and signals the peers
   TpPartials parts{};
-  auto RP = [&](const CUtensorMap* tA, const void* W, int K, const CUtensorMap* tB = nullptr) -> int {
+  auto RP = [&](const CUtensorMap* tA, const void* W, int K, const CUtensorMap* tB = nullptr,
+                const Q4Mat* q4 = nullptr) -> int {
     parts = TpPartials{};
     if (!tp) {
-      EVS_TRY(G(tA, nullptr, W, nullptr, d, K, 0, nullptr, 0, tB));
+      EVS_TRY(G(tA, nullptr, W, nullptr, d, K, 0, nullptr, 0, tB, q4));
       parts.R = 1;
       parts.buf[0] = s->ws;
       return EVS_OK;
@@ -166,13 +176,15 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
                 [&] { return launch_embed_norm(m, s, ids, M, static_cast<const float*>(m->L[0].pre_norm), st); }));
   for (int i = 0; i < c.n_layers; ++i) {
     const LayerDev& L = m->L[i];
+    auto q4_of = [&](int slot) { return m->q4 ? &L.q4[slot] : nullptr; };
     if (L.kind == EVS_LAYER_MHA) {
-      EVS_TRY(G(&L.tm_qkv, nullptr, L.w_qkv, nullptr, 3 * dl, d, 0));
-      const double kv_bytes = 2.0 * B * (maxlen + T) * H * Dh * el + 4.0 * sp * M * 3 * dl + 2.0 * M * dl * el;
+      EVS_TRY(G(&L.tm_qkv, nullptr, L.w_qkv, nullptr, 3 * dl, d, 0, nullptr, 0, nullptr, q4_of(EVS_W_QKV)));
+      const double kv_el = s->kv_q4 ? 0.5 + 2.0 / 32 : el;
+      const double kv_bytes = 2.0 * B * (maxlen + T) * H * Dh * kv_el + 4.0 * sp * M * 3 * dl + 2.0 * M * dl * el;
       EVS_TRY(timed(s, st, EVS_PROF_ATTN, kv_bytes, [&] { return launch_attention(m, s, i, B, T, sp, kv_blocks, st); }));
-      EVS_TRY(RP(&L.tm_o, L.w_o, dl));
+      EVS_TRY(RP(&L.tm_o, L.w_o, dl, nullptr, q4_of(EVS_W_O)));
     } else {
-      EVS_TRY(G(&L.tm_in, nullptr, L.w_in, nullptr, 3 * dl, d, 0));
+      EVS_TRY(G(&L.tm_in, nullptr, L.w_in, nullptr, 3 * dl, d, 0, nullptr, 0, nullptr, q4_of(EVS_W_IN)));
       const int K = L.kind == EVS_LAYER_HCM ? c.hcm_filter_length : c.hcs_filter_length;
       const int K0 = c.short_filter_length;
       // u in + y out + outer history read/write + taps; inner FIR history or IIR states
@@ -182,12 +194,12 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
       else
         hb += B * ((K - 1.0 + T) * dl * el) + static_cast<double>(dl) * K * 4;
       EVS_TRY(timed(s, st, EVS_PROF_HYENA, hb, [&] { return launch_hyena(m, s, i, B, T, sp, prefill, retain, st); }));
-      EVS_TRY(RP(&L.tm_out, L.w_out, dl));
+      EVS_TRY(RP(&L.tm_out, L.w_out, dl, nullptr, q4_of(EVS_W_OUT)));
     }
     EVS_TRY(timed(s, st, EVS_PROF_ROW, row_bytes + 4.0 * sp * M * d * parts.R, [&] {
       return launch_res_add_norm(m, s, M, sp, parts, static_cast<const float*>(L.post_norm), -1, T, st);
     }));
-    if (c.dtype == EVS_DTYPE_BF16 && gemm_plan(m, 2 * F, d, M, 1).splits == 1) {
+    if (!m->q4 && c.dtype == EVS_DTYPE_BF16 && gemm_plan(m, 2 * F, d, M, 1).splits == 1) {
       // one split: the w1/w2 projection applies the SwiGLU gate in its epilogue
       const GemmPlan pl = gemm_plan(m, 2 * F, d, M, 1);
       const double bytes = (2.0 * F * d + static_cast<double>(M) * d) * el + M * F * el;
@@ -198,10 +210,10 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
       w3_act = s->tm_gate;
     } else {
       w3_act = nullptr;
-      EVS_TRY(G(&L.tm_w1, &L.tm_w2, L.w1, L.w2, 2 * F, d, 1));
+      EVS_TRY(G(&L.tm_w1, &L.tm_w2, L.w1, L.w2, 2 * F, d, 1, nullptr, 0, nullptr, q4_of(EVS_W_W1)));
       EVS_TRY(timed(s, st, EVS_PROF_ROW, 8.0 * sp * M * F + M * F * el, [&] { return launch_swiglu(m, s, M, sp, st); }));
     }
-    EVS_TRY(RP(&L.tm_w3, L.w3, F, w3_act));
+    EVS_TRY(RP(&L.tm_w3, L.w3, F, w3_act, q4_of(EVS_W_W3)));
     const float* next = static_cast<const float*>(i + 1 < c.n_layers ? m->L[i + 1].pre_norm : m->final_norm);
     EVS_TRY(timed(s, st, EVS_PROF_ROW, row_bytes + 4.0 * sp * M * d * parts.R,
                   [&] { return launch_res_add_norm(m, s, M, sp, parts, next, m->capture_slot(i), T, st); }));
@@ -331,16 +343,54 @@ int evs_model_set_tensor(evs_model* m, int layer, int slot, const void* dev_ptr,
   return EVS_OK;
 }
 
+int evs_model_set_q4(evs_model* m, int layer, int slot, const void* codes, const void* scales, int N, int K, int group) {
+  EVS_CHECK_ARG(m != nullptr, "null argument");
+  EVS_CHECK_ARG(!m->finalized, "model already finalized");
+  EVS_CHECK_ARG(m->tp_world == 1, "4-bit weights need a model without channel sharding");
+  EVS_CHECK_ARG(layer >= 0 && layer < m->cfg.n_layers, "layer index out of range");
+  EVS_TRY(q4_check_weight(codes, scales, N, K, group));
+  const int64_t d = m->cfg.d_model, F = m->cfg.mlp_inner;
+  const bool mha = m->L[layer].kind == EVS_LAYER_MHA;
+  int64_t n = 0, k = d;
+  switch (slot) {
+    case EVS_W_IN: n = mha ? 0 : 3 * d; break;
+    case EVS_W_QKV: n = mha ? 3 * d : 0; break;
+    case EVS_W_OUT: n = mha ? 0 : d; break;
+    case EVS_W_O: n = mha ? d : 0; break;
+    case EVS_W_W1: n = 2 * F; break;
+    case EVS_W_W3: n = d, k = F; break;
+    default: break;
+  }
+  EVS_CHECK_ARG(n > 0, "slot is no dense projection of this layer kind");
+  EVS_CHECK_ARG(N == n && K == k, "4-bit weight does not match the slot shape");
+  m->L[layer].q4[slot] = {codes, scales, N, K, group};
+  return EVS_OK;
+}
+
 int evs_model_finalize(evs_model* m) {
   EVS_CHECK_ARG(m != nullptr, "null model");
   if (m->finalized) return EVS_OK;
   const evs_model_config& c = m->cfg;
   const int d = c.d_model, dl = m->dl, F = m->Fl, V = c.vocab_size;
   EVS_CHECK_ARG(m->embed && m->final_norm, "embed / final_norm not set");
+  // dense projections: all in 4 bits or none (the w1 slot holds w1 and w2)
+  int dense = 0, held = 0;
+  for (int i = 0; i < c.n_layers; ++i)
+    for (int slot : {EVS_W_IN, EVS_W_OUT, EVS_W_QKV, EVS_W_O, EVS_W_W1, EVS_W_W3})
+      if (expected_numel(m, m->L[i].kind, slot) > 0) {
+        ++dense;
+        held += m->L[i].q4[slot].codes != nullptr;
+      }
+  EVS_CHECK_ARG(held == 0 || held == dense, "either every dense projection of the blocks is held in 4 bits or none");
+  m->q4 = held > 0;
+  auto is_q4 = [&](int slot) {
+    return m->q4 && (slot == EVS_W_IN || slot == EVS_W_OUT || slot == EVS_W_QKV || slot == EVS_W_O || slot == EVS_W_W1 ||
+                     slot == EVS_W_W2 || slot == EVS_W_W3);
+  };
   for (int i = 0; i < c.n_layers; ++i) {
     LayerDev& L = m->L[i];
     for (int slot = EVS_W_PRE_NORM; slot < EVS_W_NUM_SLOTS; ++slot) {
-      if (expected_numel(m, L.kind, slot) > 0 && *slot_ptr(L, slot) == nullptr) {
+      if (expected_numel(m, L.kind, slot) > 0 && !is_q4(slot) && *slot_ptr(L, slot) == nullptr) {
         evs_set_last_error(EVS_EINVAL, ("layer " + std::to_string(i) + " slot " + std::to_string(slot) +
                                         " not set").c_str());
         return EVS_EINVAL;
@@ -350,7 +400,7 @@ int evs_model_finalize(evs_model* m) {
       EVS_CUDA_TRY(cudaMalloc(&L.poles, sizeof(float) * dl * c.state_size));
       EVS_TRY(launch_poles(static_cast<const float*>(L.log_poles), L.poles, dl * c.state_size, 0));
     }
-    if (c.dtype == EVS_DTYPE_BF16) {
+    if (c.dtype == EVS_DTYPE_BF16 && !m->q4) {
       // local shapes: column-parallel [3 dl, d] / [Fl, d], row-parallel [d, dl] / [d, Fl]
       if (L.kind == EVS_LAYER_MHA) {
         EVS_TRY(make_tmap_2d_bf16(&L.tm_qkv, L.w_qkv, d, 3 * dl, d * 2, GEMM_BK, GEMM_BM));
@@ -377,8 +427,9 @@ void evs_model_destroy(evs_model* m) {
   delete m;
 }
 
+namespace {
 // Persistent per-row arenas live in one allocation (owned[0]); scratch in owned[1].
-int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, evs_state** out) {
+int create_state(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, bool kv_q4, evs_state** out) {
   EVS_CHECK_ARG(m != nullptr && out != nullptr, "null argument");
   EVS_CHECK_ARG(m->finalized, "model not finalized");
   EVS_CHECK_ARG(max_batch >= 1 && max_seqlen >= 2 && max_chunk >= 1, "bad state sizes");
@@ -386,8 +437,16 @@ int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_
   // d: residual width; dl, H, F: this rank's Hyena channels, heads and MLP features
   const int d = c.d_model, dl = m->dl, F = m->Fl, H = m->Hl, Dh = c.head_dim, S = c.state_size;
   const size_t el = m->elem();
+  if (kv_q4) {
+    EVS_CHECK_ARG(m->tp_world == 1, "a 4-bit KV cache needs a model without channel sharding");
+    EVS_CHECK_ARG(Dh == 32 || Dh == 64 || Dh == 128, "a 4-bit KV cache needs head_dim 32, 64 or 128");
+    EVS_CHECK_ARG(max_seqlen <= (1 << 30) && max_batch <= 65535, "state too large for a 4-bit KV cache");
+  }
   evs_state* s = new evs_state();
   s->m = m;
+  s->kv_q4 = kv_q4;
+  s->kv_pages = (max_seqlen + Q4_STATE_PAGE - 1) / Q4_STATE_PAGE;
+  const size_t q4_row = static_cast<size_t>(s->kv_pages) * H * (Q4_STATE_PAGE * Dh + Q4_STATE_PAGE * Dh / 8);
   s->max_batch = max_batch;
   s->max_seqlen = max_seqlen;
   s->max_chunk = max_chunk;
@@ -419,7 +478,7 @@ int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_
     const int k = c.layer_kind[i];
     o_outer[i] = o_inner[i] = o_iir[i] = o_kv[i] = SIZE_MAX;
     if (k == EVS_LAYER_MHA) {
-      o_kv[i] = take(B * max_seqlen * 2 * H * Dh * el);
+      o_kv[i] = take(kv_q4 ? B * q4_row : B * max_seqlen * 2 * H * Dh * el);
     } else {
       o_outer[i] = take(B * s->cap_outer * 3 * dl * el);
       if (k == EVS_LAYER_HCS) o_inner[i] = take(B * s->cap_hcs * dl * el);
@@ -486,7 +545,12 @@ int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_
   const size_t o_act = take(static_cast<size_t>(s->m_cap) * s->ld_act * el);
   const size_t o_ws = take(s->ws_floats * 4);
   const size_t o_qrot = take(static_cast<size_t>(s->m_cap) * dl * el);
-  const size_t o_part = any_mha ? take(B * H * s->attn_blocks * s->attn_tcap * (Dh + 2) * 4) : SIZE_MAX;
+  s->attn_part_bytes = kv_q4 ? static_cast<size_t>(q4_attention_ws(max_batch, max_chunk, H, Dh, H, max_seqlen))
+                             : B * H * s->attn_blocks * s->attn_tcap * (Dh + 2) * 4;
+  const size_t o_part = any_mha ? take(s->attn_part_bytes) : SIZE_MAX;
+  const size_t o_table = kv_q4 ? take(B * s->kv_pages * sizeof(int32_t)) : SIZE_MAX;
+  const size_t o_zero = kv_q4 ? take(sizeof(int32_t)) : SIZE_MAX;
+  const size_t o_qkv = kv_q4 && any_mha ? take(static_cast<size_t>(s->m_cap) * 3 * dl * el) : SIZE_MAX;
   const size_t o_ids = take(static_cast<size_t>(s->m_cap) * 8);
   const size_t o_gate = c.dtype == EVS_DTYPE_BF16 ? take(static_cast<size_t>(s->m_cap) * F * 2) : SIZE_MAX;
   const size_t o_err = take(sizeof(EvsDevErr));
@@ -508,9 +572,17 @@ int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_
   if (o_part != SIZE_MAX) s->attn_part = reinterpret_cast<float*>(base + o_part);
   s->ids_scratch = reinterpret_cast<int64_t*>(base + o_ids);
   if (o_gate != SIZE_MAX) s->gate = base + o_gate;
+  if (o_qkv != SIZE_MAX) s->qkv = base + o_qkv;
   s->d_err = reinterpret_cast<EvsDevErr*>(base + o_err);
   EVS_CUDA_TRY(cudaMemset(pers, 0, s->owned_bytes[0]));
   EVS_CUDA_TRY(cudaMemset(scr, 0, s->owned_bytes[1]));
+  if (kv_q4) {
+    s->d_table = reinterpret_cast<int32_t*>(base + o_table);
+    s->d_zero = reinterpret_cast<int32_t*>(base + o_zero);
+    std::vector<int32_t> table(B * s->kv_pages);
+    for (size_t i = 0; i < table.size(); ++i) table[i] = static_cast<int32_t>(i);
+    EVS_CUDA_TRY(cudaMemcpy(s->d_table, table.data(), table.size() * sizeof(int32_t), cudaMemcpyHostToDevice));
+  }
   if (m->tp_world > 1) {
     // [buffer 0 | buffer 1 | epoch flag]; its own allocation so that it can be shared over IPC
     const size_t bytes = 2 * s->tp_buf_bytes + 256;
@@ -537,6 +609,15 @@ int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_
   EVS_CUDA_TRY(cudaDeviceSynchronize());
   *out = s;
   return EVS_OK;
+}
+}  // namespace
+
+int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, evs_state** out) {
+  return create_state(m, max_batch, max_seqlen, max_chunk, false, out);
+}
+
+int evs_state_create_q4(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, evs_state** out) {
+  return create_state(m, max_batch, max_seqlen, max_chunk, true, out);
 }
 
 void evs_state_destroy(evs_state* s) {
@@ -610,7 +691,7 @@ int evs_state_reset(evs_state* s, cudaStream_t st) {
 int evs_state_copy(evs_state* dst, const evs_state* src, cudaStream_t st) {
   EVS_CHECK_ARG(dst && src && dst->m == src->m, "states of different models");
   EVS_CHECK_ARG(dst->max_batch == src->max_batch && dst->max_seqlen == src->max_seqlen &&
-                    dst->max_chunk == src->max_chunk,
+                    dst->max_chunk == src->max_chunk && dst->kv_q4 == src->kv_q4,
                 "states of different sizes");
   EVS_CUDA_TRY(cudaMemcpyAsync(dst->owned[0], src->owned[0], src->owned_bytes[0], cudaMemcpyDeviceToDevice, st));
   dst->h_len = src->h_len;
@@ -669,7 +750,11 @@ int copy_row(evs_state* s, int src, int dst, cudaStream_t st) {
       const size_t rb = static_cast<size_t>(s->iir_slots) * d * c.state_size * 4;
       EVS_TRY(cp(hy.s_all, rb, rb));
     }
-    if (s->kv[i]) {
+    if (s->kv[i] && s->kv_q4) {
+      const size_t page = static_cast<size_t>(m->Hl) * (Q4_STATE_PAGE * c.head_dim + Q4_STATE_PAGE * c.head_dim / 8);
+      const int held = (std::min(s->h_len[src], s->max_seqlen) + Q4_STATE_PAGE - 1) / Q4_STATE_PAGE;
+      EVS_TRY(cp(s->kv[i], page * s->kv_pages, page * held));
+    } else if (s->kv[i]) {
       const size_t pos = 2ull * m->Hl * c.head_dim * el;
       EVS_TRY(cp(s->kv[i], pos * s->max_seqlen, pos * std::min(s->h_len[src], s->max_seqlen)));
     }

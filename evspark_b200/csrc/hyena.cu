@@ -978,6 +978,7 @@ int launch_state_export(const evs_state* s, int layer, int which, int row, int w
                                           s->d_len, static_cast<float*>(dst));
   } else if (which == 3) {
     EVS_CHECK_ARG(s->kv[layer] != nullptr, "layer has no KV cache");
+    if (s->kv_q4) return launch_q4_state_read(s, layer, row, width, dst, st);
     const int HD2 = 2 * m->Hl * m->cfg.head_dim;
     if (bf)
       export_kv_kernel<__nv_bfloat16><<<64, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(s->kv[layer]),

@@ -37,6 +37,12 @@ constexpr int EVS_RETAIN_MAX = 64;  // tokens per row of a retained forward (per
 //   IIR per-position states  [B][iir_slots][d][S] fp32        (slot = block index)
 //   KV cache                 [B][Lmax][2][H][Dh]  data dtype
 //   capture ring             [B][ring_len][d]     fp32        (injection-layer outputs)
+// a dense projection held in 4 bits
+struct Q4Mat {
+  const void* codes = nullptr;
+  const void* scales = nullptr;
+  int N = 0, K = 0, group = 0;
+};
 struct LayerDev {
   int kind = 0;
   const void* pre_norm = nullptr;
@@ -56,6 +62,7 @@ struct LayerDev {
   float* poles = nullptr;  // owned: exp(log_poles) fp32 [d, S]
   CUtensorMap tm_in, tm_out, tm_qkv, tm_o, tm_w1, tm_w2, tm_w3;
   int64_t numel[EVS_W_NUM_SLOTS] = {0};
+  Q4Mat q4[EVS_W_NUM_SLOTS];
 };
 
 struct evs_model {
@@ -65,6 +72,7 @@ struct evs_model {
   int tp_world = 1, tp_rank = 0;
   int dl = 0, Hl = 0, Fl = 0;
   bool finalized = false;
+  bool q4 = false;  // the blocks' dense projections are held in 4 bits
   const void* embed = nullptr;
   const void* final_norm = nullptr;
   int64_t embed_numel = 0, final_norm_numel = 0;
@@ -117,6 +125,13 @@ struct evs_state {
   float* ws = nullptr;         // split-K partials [splits][m][n] fp32
   void* qrot = nullptr;        // [m_cap][d] data dtype rotated queries
   float* attn_part = nullptr;  // [B][H][attn_blocks][attn_tcap][Dh+2] fp32
+  // KV cache in 4 bits: kv[layer] is a page pool, row b owns pages b kv_pages .. (Q4_STATE_PAGE tokens each)
+  bool kv_q4 = false;
+  int kv_pages = 0;                // pages per row
+  int32_t* d_table = nullptr;      // [B][kv_pages]
+  int32_t* d_zero = nullptr;       // [1] a start position of 0
+  void* qkv = nullptr;             // [m_cap][3d] data dtype: the qkv projection
+  size_t attn_part_bytes = 0;
   int64_t* ids_scratch = nullptr;  // [m_cap] chunk ids of a strided prefill
   EvsDevErr* d_err = nullptr;
   // channel sharding: partial sums of the row-parallel projections, double-buffered, and an
@@ -235,6 +250,17 @@ int launch_state_export(const evs_state* s, int layer, int which, int row, int w
 // attention: rope + KV append + split-KV partials + ordered combine (output into s->act)
 int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int kv_blocks,
                      cudaStream_t st);
+
+// 4-bit weights and KV cache
+constexpr int Q4_STATE_PAGE = 64;
+int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
+                     int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl);
+int q4_check_weight(const void* codes, const void* scales, int N, int K, int group);
+// rope + append into the 4-bit pages + attention over them (output into s->act); bound >= lengths + T
+int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound,
+                        cudaStream_t st);
+int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound);
+int launch_q4_state_read(const evs_state* s, int layer, int row, int width, void* dst, cudaStream_t st);
 
 // verification
 int launch_transform(const void* logits, int logits_fp64, int rows, int V, double temperature, int top_k,

@@ -560,6 +560,65 @@ int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound) {
   return std::min(all, std::max(least, fit)) * per_row;
 }
 
+namespace {
+// qkv projection: partial sums [splits][M][3d] -> data dtype [M][3d]
+template <typename TD>
+__global__ void __launch_bounds__(256) qkv_collect_kernel(const float* __restrict__ ws, int splits, size_t n,
+                                                          TD* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();
+  const size_t i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  split_sum4<false>(a, ws + i, n, splits);
+  out[i] = from_f32<TD>(a.x);
+  out[i + 1] = from_f32<TD>(a.y);
+  out[i + 2] = from_f32<TD>(a.z);
+  out[i + 3] = from_f32<TD>(a.w);
+}
+
+Q4CacheDev state_cache(const evs_state* s, int layer) {
+  const int D = s->m->cfg.head_dim;
+  return {static_cast<uint8_t*>(s->kv[layer]), s->d_err, static_cast<int64_t>(s->max_batch) * s->kv_pages, Q4_STATE_PAGE,
+          s->m->Hl, D, Q4_STATE_PAGE * D + Q4_STATE_PAGE * D / 8};
+}
+}  // namespace
+
+int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound,
+                        cudaStream_t st) {
+  const int d = m->dl, H = m->Hl, D = m->cfg.head_dim, dtype = m->cfg.dtype;
+  const bool pdl = s->use_pdl();
+  const size_t el = m->elem(), n = static_cast<size_t>(B) * T * 3 * d;
+  const dim3 grid(static_cast<unsigned>((n / 4 + 255) / 256));
+  if (dtype == EVS_DTYPE_BF16)
+    EVS_CUDA_TRY(evs_launch(qkv_collect_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, pdl,
+                            static_cast<const float*>(s->ws), splits, n, static_cast<__nv_bfloat16*>(s->qkv)));
+  else
+    EVS_CUDA_TRY(evs_launch(qkv_collect_kernel<float>, grid, dim3(256), 0, st, pdl, static_cast<const float*>(s->ws),
+                            splits, n, static_cast<float*>(s->qkv)));
+  evs_count_launch(1);
+  const Q4CacheDev c = state_cache(s, layer);
+  const Q4RowsDev r{s->d_table, s->d_len, nullptr, s->kv_pages, s->kv_pages, B, T};
+  char* qkv = static_cast<char*>(s->qkv);
+  const int64_t row = 3ll * d;
+  const Q4Tensor q{qkv, T * row, row, D}, k{qkv + d * el, T * row, row, D}, v{qkv + 2 * d * el, T * row, row, D};
+  const Q4Tensor qr{s->qrot, static_cast<int64_t>(T) * d, d, D};
+  const Q4Tensor out{s->act, static_cast<int64_t>(T) * s->ld_act, s->ld_act, D};
+  EVS_TRY(launch_q4_append(c, r, q, k, v, qr, H, dtype, m->cfg.rope_base, st, pdl));
+  return launch_q4_attention(c, r, qr, out, H, 1.f / std::sqrt(static_cast<float>(D)), bound, s->attn_part,
+                             static_cast<int64_t>(s->attn_part_bytes), dtype, st, pdl);
+}
+
+int launch_q4_state_read(const evs_state* s, int layer, int row, int width, void* dst, cudaStream_t st) {
+  if (width == 0) return EVS_OK;
+  const int H = s->m->Hl, D = s->m->cfg.head_dim;
+  const int64_t t = 2ll * H * D;
+  const Q4RowsDev r{s->d_table + static_cast<size_t>(row) * s->kv_pages, s->d_zero, nullptr, s->kv_pages, s->kv_pages, 1,
+                    width};
+  const Q4Tensor k{dst, width * t, t, D}, v{static_cast<char*>(dst) + H * D * s->m->elem(), width * t, t, D};
+  return launch_q4_read(state_cache(s, layer), r, k, v, s->m->cfg.dtype, st);
+}
+
 extern "C" {
 
 int64_t evs_q4_attention_workspace(const evs_q4_cache* cache, const evs_q4_rows* rows, int n_heads, int max_length) {

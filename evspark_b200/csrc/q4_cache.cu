@@ -337,6 +337,37 @@ Q4RowsDev q4_rows_dev(const evs_q4_rows* r) {
   return {r->page_table, r->lengths, r->counts, r->table_stride, r->max_pages, r->batch, r->tokens};
 }
 
+int launch_q4_append(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& k, const Q4Tensor& v,
+                     const Q4Tensor& q_out, int H, int dtype, double rope_base, cudaStream_t st, bool pdl) {
+  const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
+  const int vec = vec_ok(k, el) && vec_ok(v, el) && vec_ok(q, el) && vec_ok(q_out, el);
+  RopeFreq f;
+  for (int j = 0; j < c.D / 2; ++j) f.f[j] = std::pow(rope_base, -2.0 * j / c.D);
+  const int per = APP_THREADS / (c.D / 16);
+  // few tokens: their head rows over several CTAs; many: one CTA a token, so that the angles of a
+  // token are computed once
+  const int tokens = r.B * r.T;
+  dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (H + 2 * c.G + per - 1) / per);
+  EVS_CHECK_ARG(grid.y <= 65535, "q4 append: too many heads");
+  auto* kern = dtype == EVS_DTYPE_BF16 ? q4_append_kernel<__nv_bfloat16> : q4_append_kernel<float>;
+  EVS_CUDA_TRY(evs_launch(kern, grid, dim3(APP_THREADS), 0, st, pdl, c, r, q, k, v, q_out, H, vec, f));
+  evs_count_launch(1);
+  return EVS_OK;
+}
+
+int launch_q4_read(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& k, const Q4Tensor& v, int dtype,
+                   cudaStream_t st) {
+  const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
+  const int vec = vec_ok(k, el) && vec_ok(v, el);
+  const int tokens = r.B * r.T;
+  const dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS));
+  EVS_CHECK_ARG(grid.y <= 65535, "q4 read: too many heads");
+  auto* kern = dtype == EVS_DTYPE_BF16 ? q4_read_kernel<__nv_bfloat16> : q4_read_kernel<float>;
+  EVS_CUDA_TRY(evs_launch(kern, grid, dim3(APP_THREADS), 0, st, false, c, r, k, v, vec));
+  evs_count_launch(1);
+  return EVS_OK;
+}
+
 namespace {
 Q4Tensor tensor_of(void* p, const int64_t* s) { return {p, s[0], s[1], s[2]}; }
 Q4Tensor tensor_of(const void* p, const int64_t* s) { return {const_cast<void*>(p), s[0], s[1], s[2]}; }
@@ -354,27 +385,10 @@ int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG((q != nullptr) == (q_out != nullptr), "q4 append: q and q_out come together");
   EVS_CHECK_ARG(q == nullptr || (q_strides && q_out_strides && n_heads >= 1), "q4 append: q needs strides and heads");
   EVS_CHECK_ARG(rope_base > 0.0 && std::isfinite(rope_base), "q4 append: rope_base must be positive");
-  const Q4CacheDev c = q4_cache_dev(cache);
-  const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
-  const int H = q != nullptr ? n_heads : 0;
   const Q4Tensor tk = tensor_of(k, k_strides), tv = tensor_of(v, v_strides);
   const Q4Tensor tq = q != nullptr ? tensor_of(q, q_strides) : tk, to = q != nullptr ? tensor_of(q_out, q_out_strides) : tk;
-  const int vec = vec_ok(tk, el) && vec_ok(tv, el) && vec_ok(tq, el) && vec_ok(to, el);
-  RopeFreq f;
-  for (int j = 0; j < c.D / 2; ++j) f.f[j] = std::pow(rope_base, -2.0 * j / c.D);
-  const int per = APP_THREADS / (c.D / 16);
-  // few tokens: their head rows over several CTAs; many: one CTA a token, so that the angles of a
-  // token are computed once
-  const int tokens = rows->batch * rows->tokens;
-  dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (H + 2 * c.G + per - 1) / per);
-  EVS_CHECK_ARG(grid.y <= 65535, "q4 append: too many heads");
-  if (dtype == EVS_DTYPE_BF16)
-    q4_append_kernel<__nv_bfloat16><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tq, tk, tv, to, H, vec, f);
-  else
-    q4_append_kernel<float><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tq, tk, tv, to, H, vec, f);
-  EVS_CUDA_TRY(cudaGetLastError());
-  evs_count_launch(1);
-  return EVS_OK;
+  return launch_q4_append(q4_cache_dev(cache), q4_rows_dev(rows), tq, tk, tv, to, q != nullptr ? n_heads : 0, dtype,
+                          rope_base, st, false);
 }
 
 int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, const int64_t* k_strides, void* v,
@@ -383,19 +397,8 @@ int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, 
   EVS_TRY(q4_check_rows(cache, rows));
   EVS_CHECK_ARG(k && v && k_strides && v_strides, "null argument");
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 read: k and v must be fp32 or bf16");
-  const Q4CacheDev c = q4_cache_dev(cache);
-  const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
-  const Q4Tensor tk = tensor_of(k, k_strides), tv = tensor_of(v, v_strides);
-  const int vec = vec_ok(tk, el) && vec_ok(tv, el);
-  const int tokens = rows->batch * rows->tokens;
-  const dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS));
-  if (dtype == EVS_DTYPE_BF16)
-    q4_read_kernel<__nv_bfloat16><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tk, tv, vec);
-  else
-    q4_read_kernel<float><<<grid, APP_THREADS, 0, st>>>(c, q4_rows_dev(rows), tk, tv, vec);
-  EVS_CUDA_TRY(cudaGetLastError());
-  evs_count_launch(1);
-  return EVS_OK;
+  return launch_q4_read(q4_cache_dev(cache), q4_rows_dev(rows), tensor_of(k, k_strides), tensor_of(v, v_strides), dtype,
+                        st);
 }
 
 }  // extern "C"

@@ -46,3 +46,7 @@ int q4_check_cache(const evs_q4_cache* c);
 int q4_check_rows(const evs_q4_cache* c, const evs_q4_rows* r);
 Q4CacheDev q4_cache_dev(const evs_q4_cache* c);
 Q4RowsDev q4_rows_dev(const evs_q4_rows* r);
+int launch_q4_append(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& k, const Q4Tensor& v,
+                     const Q4Tensor& q_out, int H, int dtype, double rope_base, cudaStream_t st, bool pdl);
+int launch_q4_read(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& k, const Q4Tensor& v, int dtype,
+                   cudaStream_t st);

@@ -366,7 +366,9 @@ __global__ void q4_dequantize_kernel(const uint8_t* __restrict__ codes, const ui
   }
 }
 
-int check_weight(const void* codes, const void* scales, int N, int K, int group) {
+}  // namespace
+
+int q4_check_weight(const void* codes, const void* scales, int N, int K, int group) {
   EVS_CHECK_ARG(codes && scales, "null argument");
   EVS_CHECK_ARG(N >= 1 && K >= 1 && K <= (1 << 24), "q4 weight: N and K must be at least 1 (K at most 2^24)");
   EVS_CHECK_ARG(group == 32 || group == 64 || group == 128, "q4 weight: group must be 32, 64 or 128");
@@ -374,8 +376,6 @@ int check_weight(const void* codes, const void* scales, int N, int K, int group)
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(scales) % 2 == 0, "q4 weight: scales must be 2-byte aligned");
   return EVS_OK;
 }
-
-}  // namespace
 
 int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
                      int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl) {
@@ -394,7 +394,7 @@ extern "C" {
 int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
                   int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st) {
   EVS_CHECK_ARG(x && out, "null argument");
-  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_TRY(q4_check_weight(codes, scales, N, K, group));
   EVS_CHECK_ARG(x_dtype == EVS_DTYPE_BF16 || x_dtype == EVS_DTYPE_FP32, "q4 linear: x must be fp32 or bf16");
   EVS_CHECK_ARG(out_dtype == EVS_DTYPE_BF16 || out_dtype == EVS_DTYPE_FP32, "q4 linear: out must be fp32 or bf16");
   EVS_CHECK_ARG(M >= 1 && ldx >= K && ldo >= N, "q4 linear: needs M >= 1, ldx >= K and ldo >= N");
@@ -407,7 +407,7 @@ int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* co
 int evs_q4_quantize(const void* w, int dtype, int64_t ldw, int N, int K, int group, void* codes, void* scales,
                     cudaStream_t st) {
   EVS_CHECK_ARG(w != nullptr, "null argument");
-  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_TRY(q4_check_weight(codes, scales, N, K, group));
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 quantize: w must be fp32 or bf16");
   EVS_CHECK_ARG(ldw >= K, "q4 quantize: needs ldw >= K");
   const int64_t groups = static_cast<int64_t>(N) * ((K + Q4_KBLOCK - 1) / Q4_KBLOCK * Q4_KBLOCK / group);
@@ -427,7 +427,7 @@ int evs_q4_quantize(const void* w, int dtype, int64_t ldw, int N, int K, int gro
 int evs_q4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
                       int64_t ldo, cudaStream_t st) {
   EVS_CHECK_ARG(out != nullptr, "null argument");
-  EVS_TRY(check_weight(codes, scales, N, K, group));
+  EVS_TRY(q4_check_weight(codes, scales, N, K, group));
   EVS_CHECK_ARG(out_dtype == EVS_DTYPE_BF16 || out_dtype == EVS_DTYPE_FP32, "q4 dequantize: out must be fp32 or bf16");
   EVS_CHECK_ARG(ldo >= K, "q4 dequantize: needs ldo >= K");
   dim3 grid(((K + 1) / 2 + 255) / 256, std::min(N, 65535));

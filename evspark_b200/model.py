@@ -23,6 +23,7 @@ import torch
 
 from . import _native as N
 from .config import HCL, HCM, HCS, LAYER_CODE, MHA, TargetConfig
+from .q4 import quantize_weight
 from .weights import data_dtype, init_target_weights
 
 PARAM_KEYS = ("mha", "hcl", "hcm", "hcs")
@@ -36,6 +37,25 @@ def require_device(device) -> torch.device:
     with torch.cuda.device(device):
         N.call("evs_device_check")
     return device
+
+
+DENSE = ("w_in", "w_out", "w_qkv", "w_o", "w1", "w2", "w3")  # the blocks' dense projections
+
+
+def check_formats(weight_format, weight_group, kv_format, tp=None) -> None:
+    for what, fmt in (("weight_format", weight_format), ("kv_format", kv_format)):
+        if fmt not in (None, "q4"):
+            raise ValueError(f"{what} must be None or 'q4', got {fmt!r}")
+    if weight_group not in (32, 64, 128):
+        raise ValueError(f"weight_group must be 32, 64 or 128, got {weight_group}")
+    if tp and int(tp[1]) > 1 and (weight_format or kv_format):
+        raise ValueError("4-bit weights and KV caches need a model without channel sharding")
+
+
+def interleave_mlp(w1: torch.Tensor, w2: torch.Tensor) -> torch.Tensor:
+    """[F, d] x 2 -> [2F, d]: 64 rows of w1, 64 of w2 and so on (the layout of the gate kernel's input)."""
+    f, d = w1.shape
+    return torch.stack((w1.view(f // 64, 64, d), w2.view(f // 64, 64, d)), 1).reshape(2 * f, d)
 
 
 class _Config:
@@ -60,10 +80,19 @@ class _Config:
 
 class TargetModel:
     def __init__(self, cfg: TargetConfig, weights: dict[str, torch.Tensor], *, capture_layers=(),
-                 device="cuda:0", max_chunk: int = 32, tp: tuple[int, int] | None = None):
+                 device="cuda:0", max_chunk: int = 32, tp: tuple[int, int] | None = None,
+                 weight_format: str | None = None, weight_group: int = 64, kv_format: str | None = None):
         """``tp=(rank, world)`` builds rank ``rank`` of a channel-sharded model: ``weights`` are then this
-        rank's shards (``evspark_b200.tp.shard_target_weights``) and every rank runs the same calls."""
+        rank's shards (``evspark_b200.tp.shard_target_weights``) and every rank runs the same calls.
+
+        ``weight_format="q4"`` holds the blocks' dense projections in 4 bits, one scale per
+        ``weight_group`` input features (embedding, norms and filters stay as they are);
+        ``kv_format="q4"`` makes states with the KV cache in 4 bits (``evspark_b200.q4``).  Both change the
+        model's numbers, and neither changes what a token's numbers depend on: greedy speculative decoding
+        still equals native decoding."""
+        check_formats(weight_format, weight_group, kv_format, tp)
         self.device = require_device(device)
+        self.weight_format, self.kv_format = weight_format, kv_format
         self.cfg = cfg
         self.config = _Config(cfg)
         self.max_chunk = int(max_chunk)
@@ -73,7 +102,16 @@ class TargetModel:
             raise ValueError("at most 4 capture (injection) layers")
         dd = data_dtype(cfg)
         self.weights = {}
+        self.q4_weights = {}
         for k, v in weights.items():
+            if weight_format == "q4" and k.rsplit(".", 1)[-1] in DENSE:
+                if k.endswith(".w2"):
+                    continue  # packed with w1
+                v = v.detach().to(device=self.device, dtype=dd)
+                if k.endswith(".w1"):
+                    v = interleave_mlp(v, weights[k[:-1] + "2"].detach().to(device=self.device, dtype=dd))
+                self.q4_weights[k] = quantize_weight(v, weight_group)
+                continue
             want = torch.float32 if v.dtype == torch.float32 else dd
             self.weights[k] = v.detach().to(device=self.device, dtype=want).contiguous()
         mc = N.ModelConfig()
@@ -99,6 +137,10 @@ class TargetModel:
                     _, li, nm = name.split(".", 2)
                     layer, slot = int(li), N.SLOTS[nm]
                 N.check(N.lib().evs_model_set_tensor(h, layer, slot, t.data_ptr(), t.numel()), name)
+            for name, w in self.q4_weights.items():
+                _, li, nm = name.split(".", 2)
+                N.check(N.lib().evs_model_set_q4(h, int(li), N.SLOTS[nm], w.codes.data_ptr(), w.scales.data_ptr(),
+                                                 *w.shape, w.group), name)
             N.check(N.lib().evs_model_finalize(h), "evs_model_finalize")
 
     @classmethod
@@ -217,8 +259,8 @@ class InferenceParams(dict):
         self.retained_chunk = 0
         h = C.c_void_p()
         with torch.cuda.device(model.device):
-            N.check(N.lib().evs_state_create(model.handle, max_batch, max_seqlen, max_chunk, C.byref(h)),
-                    "evs_state_create")
+            create = "evs_state_create_q4" if model.kv_format == "q4" else "evs_state_create"
+            N.check(getattr(N.lib(), create)(model.handle, max_batch, max_seqlen, max_chunk, C.byref(h)), create)
         self._h = h
         if model.tp_world > 1:  # collective: every rank creates its state in the same order
             from .tp import connect_state

@@ -108,6 +108,12 @@ EVS_API int evs_device_check(void);
  * replaces vortex StripedHyena construction + Evo2 weight loading (evspark/api.py:94-98) */
 EVS_API int evs_model_create(const evs_model_config* cfg, evs_model** out);
 EVS_API int evs_model_set_tensor(evs_model* m, int layer, int slot, const void* dev_ptr, int64_t numel);
+/* A dense projection held in 4 bits instead of evs_model_set_tensor (format: evs_q4_quantize below):
+ * slot EVS_W_IN, EVS_W_OUT, EVS_W_QKV, EVS_W_O, EVS_W_W3, or EVS_W_W1 for w1 and w2 as one weight
+ * [2 F, d] of 64 rows of w1, 64 of w2 and so on.  Every dense projection of the blocks or none; models
+ * without channel sharding.  The caller keeps the memory, as with evs_model_set_tensor. */
+EVS_API int evs_model_set_q4(evs_model* m, int layer, int slot, const void* codes, const void* scales, int N, int K,
+                             int group);
 /* validates every slot, builds TMA tensor maps and derived constants (poles = exp(log_poles)) */
 EVS_API int evs_model_finalize(evs_model* m);
 EVS_API void evs_model_destroy(evs_model* m);
@@ -116,6 +122,9 @@ EVS_API void evs_model_destroy(evs_model* m);
  * replaces model.initialize_inference_params (evspark/specdec/block/loop.py:341).
  * max_chunk bounds the tokens of one evs_forward call (prefill is chunked internally). */
 EVS_API int evs_state_create(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, evs_state** out);
+/* the same with the KV cache in 4 bits (paged as evs_q4_kv_append lays it out, 64 tokens a page; 0.28 of
+ * the bf16 size).  evs_state_export returns the values that the cache holds.  Not with channel sharding. */
+EVS_API int evs_state_create_q4(const evs_model* m, int max_batch, int max_seqlen, int max_chunk, evs_state** out);
 EVS_API void evs_state_destroy(evs_state* s);
 /* zero the lengths of every row (an empty cache; prefill may follow) */
 EVS_API int evs_state_reset(evs_state* s, cudaStream_t stream);
