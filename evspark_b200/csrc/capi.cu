@@ -68,8 +68,20 @@ const void** slot_ptr(LayerDev& L, int slot) {
 // out: partial sums [splits][M][N] (s->ws, or a shared buffer of a row-parallel projection)
 int gemm(const evs_model* m, evs_state* s, const CUtensorMap* tA, const CUtensorMap* tA2, const void* W,
          const void* W2, int N, int K, int M, int dual, float* out, size_t out_floats, cudaStream_t st, int* splits,
-         const CUtensorMap* tB_override = nullptr, const Q4Mat* q4 = nullptr) {
-  if (q4 != nullptr) {
+         const CUtensorMap* tB_override = nullptr, const Q4Mat* q4 = nullptr, bool decode = false) {
+  bool pdl = s->use_pdl();
+  if (q4 != nullptr && decode) {
+    // prefill: the weight decoded once, then the projection of many tokens.  That one starts on its
+    // weight before it waits for earlier kernels, so it is launched after the decoding has finished.
+    EVS_TRY(launch_q4_decode(q4->codes, q4->scales, N, K, q4->group, s->dec, m->cfg.dtype, K, st, pdl));
+    const int d = m->cfg.d_model;
+    tA = &s->tm_dec[K != d ? 3 : (N == 3 * d ? 0 : (N == d ? 1 : 2))];
+    tA2 = nullptr;
+    W = s->dec;
+    W2 = nullptr;
+    dual = 0;
+    pdl = false;
+  } else if (q4 != nullptr) {
     EVS_CHECK_RANGE(static_cast<size_t>(M) * N <= out_floats, "projection workspace too small");
     *splits = 1;
     return launch_q4_linear(s->act, m->cfg.dtype, s->ld_act, M, q4->codes, q4->scales, N, K, q4->group, out,
@@ -83,11 +95,11 @@ int gemm(const evs_model* m, evs_state* s, const CUtensorMap* tA, const CUtensor
         tB_override ? tB_override : (K == m->cfg.d_model ? s->tm_act_d : (K == m->Fl ? s->tm_act_f : s->tm_act_l));
     if (m->tp_world == 1 && gemm_serial(p)) {
       *splits = 1;  // the splits' sum, stored as one split
-      return launch_gemm_tc_serial(tA, tA2, tB, p, out, s->d_err, st, s->use_pdl());
+      return launch_gemm_tc_serial(tA, tA2, tB, p, out, s->d_err, st, pdl);
     }
-    return launch_gemm_tc(tA, tA2, tB, p, out, s->d_err, st, s->use_pdl());
+    return launch_gemm_tc(tA, tA2, tB, p, out, s->d_err, st, pdl);
   }
-  return launch_gemm_simt(W, W2, s->act, s->ld_act, m->cfg.dtype, p, out, st, s->use_pdl());
+  return launch_gemm_simt(W, W2, s->act, s->ld_act, m->cfg.dtype, p, out, st, pdl);
 }
 
 cudaEvent_t take_event(evs_state* s) {
@@ -142,7 +154,7 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
     float* o = out != nullptr ? out : s->ws;
     const size_t of = out != nullptr ? out_floats : s->ws_floats;
     return timed(s, st, EVS_PROF_GEMM, bytes,
-                 [&] { return gemm(m, s, tA, tA2, W, W2, N, K, M, dual, o, of, st, &sp, tB, q4); });
+                 [&] { return gemm(m, s, tA, tA2, W, W2, N, K, M, dual, o, of, st, &sp, tB, q4, prefill != 0); });
   };
   // row-parallel projection [d x K] whose partial sums the next residual + RMSNorm adds up: with
   // channel sharding it writes to the shared buffer of reduction `epoch` and signals the peers
@@ -548,6 +560,7 @@ int create_state(const evs_model* m, int max_batch, int max_seqlen, int max_chun
   s->attn_part_bytes = kv_q4 ? static_cast<size_t>(q4_attention_ws(max_batch, max_chunk, H, Dh, H, max_seqlen))
                              : B * H * s->attn_blocks * s->attn_tcap * (Dh + 2) * 4;
   const size_t o_part = any_mha ? take(s->attn_part_bytes) : SIZE_MAX;
+  const size_t o_dec = m->q4 ? take(static_cast<size_t>(d) * std::max(3 * d, 2 * F) * el) : SIZE_MAX;
   const size_t o_table = kv_q4 ? take(B * s->kv_pages * sizeof(int32_t)) : SIZE_MAX;
   const size_t o_zero = kv_q4 ? take(sizeof(int32_t)) : SIZE_MAX;
   const size_t o_qkv = kv_q4 && any_mha ? take(static_cast<size_t>(s->m_cap) * 3 * dl * el) : SIZE_MAX;
@@ -573,6 +586,7 @@ int create_state(const evs_model* m, int max_batch, int max_seqlen, int max_chun
   s->ids_scratch = reinterpret_cast<int64_t*>(base + o_ids);
   if (o_gate != SIZE_MAX) s->gate = base + o_gate;
   if (o_qkv != SIZE_MAX) s->qkv = base + o_qkv;
+  if (o_dec != SIZE_MAX) s->dec = base + o_dec;
   s->d_err = reinterpret_cast<EvsDevErr*>(base + o_err);
   EVS_CUDA_TRY(cudaMemset(pers, 0, s->owned_bytes[0]));
   EVS_CUDA_TRY(cudaMemset(scr, 0, s->owned_bytes[1]));
@@ -605,6 +619,12 @@ int create_state(const evs_model* m, int max_batch, int max_seqlen, int max_chun
       EVS_TRY(make_tmap_2d_bf16(&s->tm_gate[t], s->gate, F, s->m_cap, static_cast<uint64_t>(F) * 2, GEMM_BK,
                                 GEMM_NT[t]));
     }
+  }
+  if (m->q4 && c.dtype == EVS_DTYPE_BF16) {
+    const int rows[4] = {3 * d, d, 2 * F, d}, cols[4] = {d, d, d, F};
+    for (int k = 0; k < 4; ++k)
+      EVS_TRY(make_tmap_2d_bf16(&s->tm_dec[k], s->dec, cols[k], rows[k], static_cast<uint64_t>(cols[k]) * 2, GEMM_BK,
+                                GEMM_BM));
   }
   EVS_CUDA_TRY(cudaDeviceSynchronize());
   *out = s;

@@ -132,6 +132,9 @@ struct evs_state {
   int32_t* d_zero = nullptr;       // [1] a start position of 0
   void* qkv = nullptr;             // [m_cap][3d] data dtype: the qkv projection
   size_t attn_part_bytes = 0;
+  // 4-bit weights, prefill: a projection's weight decoded to the data dtype, and its maps by shape
+  void* dec = nullptr;
+  CUtensorMap tm_dec[4];  // [3d, d], [d, d], [2F, d], [d, F]
   int64_t* ids_scratch = nullptr;  // [m_cap] chunk ids of a strided prefill
   EvsDevErr* d_err = nullptr;
   // channel sharding: partial sums of the row-parallel projections, double-buffered, and an
@@ -255,6 +258,8 @@ int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, 
 constexpr int Q4_STATE_PAGE = 64;
 int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
                      int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl);
+int launch_q4_decode(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
+                     int64_t ldo, cudaStream_t st, bool pdl);
 int q4_check_weight(const void* codes, const void* scales, int N, int K, int group);
 // rope + append into the 4-bit pages + attention over them (output into s->act); bound >= lengths + T
 int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound,

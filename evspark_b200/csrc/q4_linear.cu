@@ -349,20 +349,36 @@ __global__ void q4_quantize_kernel(const TW* __restrict__ w, int64_t ldw, int N,
   if (lane == 0) scales[static_cast<size_t>(gi) * N + n] = static_cast<uint16_t>(s);
 }
 
-// one thread per byte: two values of a row
+// one thread per 16 codes of a row: 16 values
 template <typename TO>
-__global__ void q4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, int N, int K,
-                                     int group, TO* __restrict__ out, int64_t ldo) {
-  const int n = blockIdx.y;
+__global__ void __launch_bounds__(256)
+    q4_decode_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, int N, int K,
+                     int group_shift, TO* __restrict__ out, int64_t ldo, int vec) {
+  pdl_trigger();
+  pdl_wait();
+  const int units = (K + 15) / 16;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<int64_t>(N) * units) return;
+  const int n = static_cast<int>(i / units), k = static_cast<int>(i - static_cast<int64_t>(n) * units) * 16;
   const size_t row_bytes = static_cast<size_t>((K + Q4_KBLOCK - 1) / Q4_KBLOCK) * (Q4_KBLOCK / 2);
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  const int k = 2 * j;
-  if (k >= K) return;
-  for (int r = n; r < N; r += gridDim.y) {
-    const uint32_t b = codes[r * row_bytes + j];
-    const float s = __uint_as_float(static_cast<uint32_t>(scales[static_cast<size_t>(k / group) * N + r]) << 16);
-    out[r * ldo + k] = from_f32<TO>((static_cast<int>(b & 15u) - 8) * s);
-    if (k + 1 < K) out[r * ldo + k + 1] = from_f32<TO>((static_cast<int>(b >> 4) - 8) * s);
+  const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + n * row_bytes + k / 2));
+  const float s =
+      __uint_as_float(static_cast<uint32_t>(__ldg(scales + static_cast<size_t>(k >> group_shift) * N + n)) << 16);
+  float v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = (static_cast<int>(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u) - 8) * s;
+  TO* dst = out + n * ldo + k;
+  if (vec && k + 16 <= K) {
+    TO t[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = from_f32<TO>(v[j]);
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(t) / 16); ++j)
+      reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(t)[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (k + j < K) dst[j] = from_f32<TO>(v[j]);
   }
 }
 
@@ -371,6 +387,7 @@ __global__ void q4_dequantize_kernel(const uint8_t* __restrict__ codes, const ui
 int q4_check_weight(const void* codes, const void* scales, int N, int K, int group) {
   EVS_CHECK_ARG(codes && scales, "null argument");
   EVS_CHECK_ARG(N >= 1 && K >= 1 && K <= (1 << 24), "q4 weight: N and K must be at least 1 (K at most 2^24)");
+  EVS_CHECK_ARG(static_cast<int64_t>(N) * K <= (1ll << 35), "q4 weight: at most 2^35 values");
   EVS_CHECK_ARG(group == 32 || group == 64 || group == 128, "q4 weight: group must be 32, 64 or 128");
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(codes) % 16 == 0, "q4 weight: codes must be 16-byte aligned");
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(scales) % 2 == 0, "q4 weight: scales must be 2-byte aligned");
@@ -387,6 +404,25 @@ int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void*
   if (out_dtype == EVS_DTYPE_BF16)
     return launch_linear_t<float, __nv_bfloat16>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
   return launch_linear_t<float, float>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+}
+
+int launch_q4_decode(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
+                     int64_t ldo, cudaStream_t st, bool pdl) {
+  const int64_t blocks = (static_cast<int64_t>(N) * ((K + 15) / 16) + 255) / 256;
+  EVS_CHECK_ARG(blocks <= INT32_MAX, "q4 dequantize: too many values");
+  const int shift = group == 32 ? 5 : (group == 64 ? 6 : 7);
+  const size_t el = out_dtype == EVS_DTYPE_BF16 ? 2 : 4;
+  const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && (ldo * el) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (out_dtype == EVS_DTYPE_BF16)
+    EVS_CUDA_TRY(evs_launch(q4_decode_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, pdl,
+                            static_cast<const uint8_t*>(codes), static_cast<const uint16_t*>(scales), N, K, shift,
+                            static_cast<__nv_bfloat16*>(out), ldo, vec));
+  else
+    EVS_CUDA_TRY(evs_launch(q4_decode_kernel<float>, grid, dim3(256), 0, st, pdl, static_cast<const uint8_t*>(codes),
+                            static_cast<const uint16_t*>(scales), N, K, shift, static_cast<float*>(out), ldo, vec));
+  evs_count_launch(1);
+  return EVS_OK;
 }
 
 extern "C" {
@@ -430,18 +466,7 @@ int evs_q4_dequantize(const void* codes, const void* scales, int N, int K, int g
   EVS_TRY(q4_check_weight(codes, scales, N, K, group));
   EVS_CHECK_ARG(out_dtype == EVS_DTYPE_BF16 || out_dtype == EVS_DTYPE_FP32, "q4 dequantize: out must be fp32 or bf16");
   EVS_CHECK_ARG(ldo >= K, "q4 dequantize: needs ldo >= K");
-  dim3 grid(((K + 1) / 2 + 255) / 256, std::min(N, 65535));
-  if (out_dtype == EVS_DTYPE_BF16)
-    q4_dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes),
-                                                              static_cast<const uint16_t*>(scales), N, K, group,
-                                                              static_cast<__nv_bfloat16*>(out), ldo);
-  else
-    q4_dequantize_kernel<float><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(codes),
-                                                      static_cast<const uint16_t*>(scales), N, K, group,
-                                                      static_cast<float*>(out), ldo);
-  EVS_CUDA_TRY(cudaGetLastError());
-  evs_count_launch(1);
-  return EVS_OK;
+  return launch_q4_decode(codes, scales, N, K, group, out, out_dtype, ldo, st, false);
 }
 
 }  // extern "C"

@@ -88,8 +88,9 @@ class TargetModel:
         ``weight_format="q4"`` holds the blocks' dense projections in 4 bits, one scale per
         ``weight_group`` input features (embedding, norms and filters stay as they are);
         ``kv_format="q4"`` makes states with the KV cache in 4 bits (``evspark_b200.q4``).  Both change the
-        model's numbers, and neither changes what a token's numbers depend on: greedy speculative decoding
-        still equals native decoding."""
+        model's numbers; greedy speculative decoding still equals native decoding.  With 4-bit weights a
+        prompt is prefilled on the weights decoded for it (the same held values, summed as the bf16
+        projections sum), so a token's rounding differs between prefill and later forwards."""
         check_formats(weight_format, weight_group, kv_format, tp)
         self.device = require_device(device)
         self.weight_format, self.kv_format = weight_format, kv_format

@@ -488,6 +488,16 @@ def speculative_generate(model, draft, prompt_ids, n_tokens: int, gamma: int, gr
                               emitted_logits=out_logits, rollback=rollback)
 
 
+def _native_prefill(model, prompt: torch.Tensor, ip) -> torch.Tensor:
+    """Consume the prompt, return its last token's logits.  A model with 4-bit weights decodes them for the
+    prompt's projections (other sums than a step's, so other roundings): its last prompt token goes through a
+    step, as it goes through the first verify block of the speculative loop, and the two stay equal."""
+    if getattr(model, "weight_format", None) is not None and prompt.shape[1] > 1:
+        prefill(model, prompt[:, :-1], ip)
+        return step_forward_reference(model, prompt[:, -1:], ip)[0, -1]
+    return prefill(model, prompt, ip)[0, -1]
+
+
 def native_greedy_reference(model, prompt_ids, n_tokens: int, *, record_logits: bool = False):
     """Token-by-token argmax (lowest index on ties) on the same kernels (loop.py:584-624)."""
     device = model.device
@@ -498,7 +508,7 @@ def native_greedy_reference(model, prompt_ids, n_tokens: int, *, record_logits: 
     ip = model.initialize_inference_params(max_seqlen=L + max(n_tokens, 0) + 2, max_chunk=_prefill_chunk(model, L))
     if n_tokens == 0:
         return np.empty(0, dtype=np.int64), ip, None
-    last = prefill(model, prompt, ip)[0, -1]
+    last = _native_prefill(model, prompt, ip)
     emitted = np.empty(n_tokens, dtype=np.int64)
     rows = []
     x = torch.empty(1, 1, dtype=torch.int64, device=device)
@@ -525,7 +535,7 @@ def native_sample_reference(model, prompt_ids, n_tokens: int, rng: np.random.Gen
         return np.empty(0, dtype=np.int64)
     L = int(prompt.shape[1])
     ip = model.initialize_inference_params(max_seqlen=L + n_tokens + 2, max_chunk=_prefill_chunk(model, L))
-    last = prefill(model, prompt, ip)[0, -1]
+    last = _native_prefill(model, prompt, ip)
     emitted = np.empty(n_tokens, dtype=np.int64)
     x = torch.empty(1, 1, dtype=torch.int64, device=device)
 
@@ -550,7 +560,7 @@ def teacher_force_to_spec_state(model, prompt_ids, emitted_ids, *, max_seqlen: i
     emitted = np.asarray(emitted_ids, dtype=np.int64).ravel()
     L, n = int(prompt.shape[1]), int(emitted.size)
     ip = model.initialize_inference_params(max_seqlen=max_seqlen or L + n + 2)
-    prefill(model, prompt, ip)
+    _native_prefill(model, prompt, ip)
     if n > 1:
         step_forward_reference(model, torch.as_tensor(emitted[:-1], device=model.device)[None], ip)
     return ip
