@@ -4,7 +4,7 @@
 // Split-KV. A warp takes a unit of consecutive keys for a tile of 16 query rows (a row is one token
 // of one query head of the kv head) and runs an online softmax over it; the four units of a CTA are
 // folded in order, and a second kernel folds the CTAs' partial results in order.  The unit's length
-// depends on the row's own position alone (64 keys below 4096, 256 below 131072, else 512), so a
+// depends on the row's own position alone (32 keys below 1024, 64 below 4096, 256 below 131072, else 512), so a
 // token's result does not depend on what else is in the call: verify blocks and single steps agree
 // bit for bit.
 #include <math_constants.h>
@@ -21,17 +21,22 @@ namespace {
 constexpr int QA_WARPS = 4;
 constexpr int QA_THREADS = 32 * QA_WARPS;
 constexpr int QA_ROWS = 16;
+constexpr int QA_CLUSTER = 8;  // slots that one cluster folds: contexts of up to 2,048 keys
 constexpr int NS = 2;           // 16-key chunks per online-softmax step of a warp
 constexpr int QA_STEP = 16 * NS;
 
 // length class of a position, and keys per CTA of a class
-__host__ __device__ constexpr int qa_class(int64_t pos) { return pos < 4096 ? 0 : (pos < 131072 ? 1 : 2); }
-__host__ __device__ constexpr int64_t qa_class_end(int cl) { return cl == 0 ? 4096 : (cl == 1 ? 131072 : (1ll << 40)); }
-__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 256 : (cl == 1 ? 1024 : 2048); }
+__host__ __device__ constexpr int qa_class(int64_t pos) {
+  return pos < 1024 ? 0 : (pos < 4096 ? 1 : (pos < 131072 ? 2 : 3));
+}
+__host__ __device__ constexpr int64_t qa_class_end(int cl) {
+  return cl == 0 ? 1024 : (cl == 1 ? 4096 : (cl == 2 ? 131072 : (1ll << 40)));
+}
+__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 2048)); }
 // partial results of one row for lengths up to bound
 inline int qa_slots(int64_t bound) {
   int n = 1;
-  for (int cl = 0; cl < 3; ++cl) {
+  for (int cl = 0; cl < 4; ++cl) {
     const int64_t end = std::min(bound, qa_class_end(cl));
     n = std::max<int64_t>(n, (end + qa_cta_keys(cl) - 1) / qa_cta_keys(cl));
     if (bound <= qa_class_end(cl)) break;
@@ -87,18 +92,17 @@ __host__ __device__ constexpr int qa_q_floats() {
   return qa_parts_q(sizeof(T)) * 2 * (DH / 32) * 32 * 4;
 }
 
-template <typename T, int DH>
-__global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
-    q4_attn_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, int grp, int t0, int tc, int tiles, float scale_log2,
-                   int nslots, float* __restrict__ part_o, float2* __restrict__ part_s) {
+// One CTA's keys for one tile of 16 rows.  FUSED: each row's result stays in shared memory (fin), else it
+// goes to the CTA's slot of the workspace.
+template <typename T, int DH, bool FUSED>
+__device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache, const Q4RowsDev& rows, const Q4Tensor& q,
+                                          int grp, int t0, int tc, int tiles, float scale_log2, int nslots, bool q_vec,
+                                          float* __restrict__ part_o, float2* __restrict__ part_s) {
   constexpr int NQ = qa_parts_q(sizeof(T)), NP = qa_parts_p(sizeof(T));
   constexpr int KW = DH / 32;  // code words per thread and key (K)
   constexpr int VN = DH / 8;   // 8-feature tiles of the output
-  pdl_trigger();
-  extern __shared__ __align__(16) float qa_sm[];  // the queries, then [warp][16][DH + 2] results
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
-  pdl_wait();
   int len, count;
   if (!q4_row(rows, b, &len, &count, cache.P)) {
     if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
@@ -114,28 +118,31 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
   // Queries as product operands: step 2 w covers the feature pairs (0,4) (1,5) of the word 8 w ..,
   // step 2 w + 1 the pairs (2,6) (3,7), as q4_word decodes the keys; qs[part][step][lane].
   uint4* qs = reinterpret_cast<uint4*>(qa_sm);
-  for (int i = threadIdx.x; i < 32 * KW; i += QA_THREADS) {
-    const int l = i & 31, w = i >> 5, lg = l >> 2, lc = l & 3;
+  if (threadIdx.x < 32 * KW) {
     uint32_t e[2][8][3];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = tile * QA_ROWS + lg + 8 * h, t = t0 + r / grp;
-      const bool live = r < tc * grp && t < count;
-      const T* src =
-          static_cast<const T*>(q.p) + b * q.sb + t * q.st + (kvh * grp + r % grp) * q.sh + lc * (DH / 4) + 8 * w;
+      const int r = tile * QA_ROWS + g + 8 * h, t = t0 + r / grp;
+      float qv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) qv[j] = 0.f;
+      if (r < tc * grp && t < count)
+        q4_load8<T>(qv,
+                    static_cast<const T*>(q.p) + b * q.sb + t * q.st + (kvh * grp + r % grp) * q.sh + c * (DH / 4) + 8 * warp,
+                    q_vec);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         if constexpr (NQ == 1)
-          e[h][j][0] = live ? __bfloat16_as_ushort(src[j]) : 0u;
+          e[h][j][0] = __float_as_uint(qv[j]) >> 16;
         else
-          q4_parts(live ? to_f32<T>(src[j]) : 0.f, e[h][j]);
+          q4_parts(qv[j], e[h][j]);
       }
     }
 #pragma unroll
     for (int p = 0; p < NQ; ++p)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        qs[(p * 2 * KW + 2 * w + s) * 32 + l] =
+        qs[(p * 2 * KW + 2 * warp + s) * 32 + lane] =
             make_uint4(e[0][2 * s][p] | e[0][2 * s + 4][p] << 16, e[1][2 * s][p] | e[1][2 * s + 4][p] << 16,
                        e[0][2 * s + 1][p] | e[0][2 * s + 5][p] << 16, e[1][2 * s + 1][p] | e[1][2 * s + 5][p] << 16);
   }
@@ -437,20 +444,107 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
       for (int w = 0; w < QA_WARPS; ++w) {
         f[w] = mw[w] == -CUDART_INF_F ? 0.f : ex2(mw[w] - big);
-        sum += res[(w * QA_ROWS + r) * LD + DH + 1] * f[w];
+        sum = fmaf(res[(w * QA_ROWS + r) * LD + DH + 1], f[w], sum);
       }
-      const size_t prow =
-          ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots + blockIdx.x;
+      float* dst_o;
+      if constexpr (FUSED) {
+        dst_o = res + (QA_WARPS * QA_ROWS + r) * LD;
+        if (lane == 0) *reinterpret_cast<float2*>(dst_o + DH) = make_float2(big, sum);
+      } else {
+        const size_t prow =
+            ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots + blockIdx.x;
+        dst_o = part_o + prow * DH;
+        if (lane == 0) part_s[prow] = make_float2(big, sum);
+      }
       for (int d = lane; d < DH; d += 32) {
         float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < QA_WARPS; ++w) acc += res[(w * QA_ROWS + r) * LD + d] * f[w];
-        part_o[prow * DH + d] = acc;
+        for (int w = 0; w < QA_WARPS; ++w) acc = fmaf(res[(w * QA_ROWS + r) * LD + d], f[w], acc);
+        dst_o[d] = acc;
       }
-      if (lane == 0) part_s[prow] = make_float2(big, sum);
     }
     __syncthreads();
   }
+}
+
+// whether row b's token t is a token, and its position; a row that cannot be read (bad lengths, or beyond
+// the launch's slots) is set to NaN
+template <typename T, int DH>
+__device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDev& rows, int b, int t, int nslots, T* dst,
+                                         int* n) {
+  const int lane = threadIdx.x & 31;
+  int len, count;
+  const bool ok = q4_row(rows, b, &len, &count, cache.P);
+  if (t >= (ok ? count : min(max(count, 0), rows.T))) return false;
+  if (ok) *n = static_cast<int>((static_cast<int64_t>(len) + t) / qa_cta_keys(qa_class(static_cast<int64_t>(len) + t))) + 1;
+  if (ok && *n <= nslots) return true;
+  for (int d = lane; d < DH; d += 32) dst[d] = from_f32<T>(CUDART_NAN_F);
+  if (ok && lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
+  return false;
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
+    q4_attn_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, int grp, int t0, int tc, int tiles, float scale_log2,
+                   int nslots, int q_vec, float* __restrict__ part_o, float2* __restrict__ part_s) {
+  pdl_trigger();
+  extern __shared__ __align__(16) float qa_sm[];  // the queries, then [warp][16][DH + 2] results
+  pdl_wait();
+  attn_tile<T, DH, false>(qa_sm, cache, rows, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec != 0, part_o, part_s);
+}
+
+// Short contexts: the CTAs of a tile are one cluster and fold their results through its shared memory,
+// with the combine kernel's arithmetic and without its launch and the workspace.
+template <typename T, int DH>
+__global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
+    q4_attn_fused_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, Q4Tensor out, int grp, int tiles,
+                         float scale_log2, int q_vec) {
+  pdl_trigger();
+  extern __shared__ __align__(16) float qa_sm[];  // the queries, [warp][16][DH + 2] results, [16][DH + 2] folded
+  pdl_wait();
+  const int nslots = gridDim.x;
+  attn_tile<T, DH, true>(qa_sm, cache, rows, q, grp, 0, rows.T, tiles, scale_log2, nslots, q_vec != 0, nullptr,
+                         nullptr);
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
+  const float* fin = qa_sm + qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2);
+  for (int r = warp * nslots + blockIdx.x; r < QA_ROWS; r += QA_WARPS * nslots) {
+    const int R = tile * QA_ROWS + r, t = R / grp;
+    if (R >= rows.T * grp) break;
+    T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
+    int n;
+    if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) continue;
+    const uint32_t at = smem_u32(fin + r * (DH + 2));
+    float v[QA_CLUSTER][DH / 32], mx[QA_CLUSTER], sm[QA_CLUSTER], big = -CUDART_INF_F;
+#pragma unroll
+    for (int x = 0; x < QA_CLUSTER; ++x)
+      if (x < n) {
+        uint32_t a;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(x));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(mx[x]), "=f"(sm[x]) : "r"(a + 4 * DH) : "memory");
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[x][d]) : "r"(a + 4 * (32 * d + lane)) : "memory");
+        big = fmaxf(big, mx[x]);
+      }
+    float acc[DH / 32], sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d) acc[d] = 0.f;
+#pragma unroll
+    for (int x = 0; x < QA_CLUSTER; ++x)
+      if (x < n) {
+        const float f = mx[x] == -CUDART_INF_F ? 0.f : ex2(mx[x] - big);
+        sum = fmaf(sm[x], f, sum);
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) acc[d] = fmaf(v[x][d], f, acc[d]);
+      }
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
+  }
+  // no CTA of the cluster leaves while another still reads its results
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // One warp per output row: the CTAs' partial results folded in order.
@@ -464,22 +558,10 @@ __global__ void __launch_bounds__(QA_THREADS)
   const int R = blockIdx.x * QA_WARPS + (threadIdx.x >> 5);
   if (R >= tc * grp) return;
   const int t = t0 + R / grp;
-  int len, count;
-  const bool ok = q4_row(rows, b, &len, &count, cache.P);
-  if (t >= (ok ? count : min(max(count, 0), rows.T))) return;
   T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
-  if (!ok) {
-    for (int d = lane; d < DH; d += 32) dst[d] = from_f32<T>(CUDART_NAN_F);
-    return;
-  }
-  const int64_t pos = static_cast<int64_t>(len) + t;
-  const int n = static_cast<int>(pos / qa_cta_keys(qa_class(pos))) + 1;
+  int n;
+  if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) return;
   const size_t prow = ((static_cast<size_t>(b) * cache.G + kvh) * static_cast<size_t>(prows) + R) * nslots;
-  if (n > nslots) {  // max_length was below this row's length
-    for (int d = lane; d < DH; d += 32) dst[d] = from_f32<T>(CUDART_NAN_F);
-    if (lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
-    return;
-  }
   float big = -CUDART_INF_F;
   for (int x = lane; x < n; x += 32) big = fmaxf(big, part_s[prow + x].x);
   big = warp_max(big);
@@ -490,9 +572,9 @@ __global__ void __launch_bounds__(QA_THREADS)
   for (int x = 0; x < n; ++x) {
     const float2 st = part_s[prow + x];
     const float f = st.x == -CUDART_INF_F ? 0.f : ex2(st.x - big);
-    sum += st.y * f;
+    sum = fmaf(st.y, f, sum);
 #pragma unroll
-    for (int d = 0; d < DH / 32; ++d) acc[d] += part_o[(prow + x) * DH + 32 * d + lane] * f;
+    for (int d = 0; d < DH / 32; ++d) acc[d] = fmaf(part_o[(prow + x) * DH + 32 * d + lane], f, acc[d]);
   }
 #pragma unroll
   for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
@@ -500,10 +582,41 @@ __global__ void __launch_bounds__(QA_THREADS)
 
 inline int64_t padded_rows(int64_t rows) { return (rows + QA_ROWS - 1) / QA_ROWS * QA_ROWS; }
 
+// one cluster per tile, no workspace
+inline bool fused_fits(int nslots, int64_t T, int grp, int G) {
+  return nslots <= QA_CLUSTER && padded_rows(T * grp) / QA_ROWS * G <= 65535;
+}
+
 template <typename T, int DH>
 int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& out, int H, float scale,
                 int64_t bound, float* ws, int64_t ws_floats, cudaStream_t st, bool pdl) {
   const int grp = H / c.G, nslots = qa_slots(bound);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  const int q_vec = q4_vec(q, sizeof(T));
+  if (fused_fits(nslots, r.T, grp, c.G)) {
+    auto* kern = q4_attn_fused_kernel<T, DH>;
+    const int smem = (qa_q_floats<T, DH>() + (QA_WARPS + 1) * QA_ROWS * (DH + 2)) * 4;
+    static std::atomic<unsigned long long> done{0};
+    EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
+    const int tiles = static_cast<int>(padded_rows(static_cast<int64_t>(r.T) * grp) / QA_ROWS);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(nslots, c.G * tiles, r.B);
+    cfg.blockDim = dim3(QA_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = nslots;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    EVS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, c, r, q, out, grp, tiles, scale_log2, q_vec));
+    evs_count_launch(1);
+    return EVS_OK;
+  }
   auto* kern = q4_attn_kernel<T, DH>;
   const int smem = (qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2)) * 4;
   static std::atomic<unsigned long long> done{0};
@@ -519,7 +632,7 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
     float* po = ws;
     float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * prows * nslots * DH);
     EVS_CUDA_TRY(evs_launch(kern, dim3(nslots, c.G * tiles, r.B), dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc,
-                            tiles, scale * 1.4426950408889634f, nslots, po, ps));
+                            tiles, scale_log2, nslots, q_vec, po, ps));
     // the combine may start while the last tiles run (it waits for them before it reads)
     EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3((tc * grp + QA_WARPS - 1) / QA_WARPS, c.G, r.B),
                             dim3(QA_THREADS), 0, st, true, c, r, out, grp, t0, tc, prows, nslots,
@@ -554,6 +667,7 @@ int launch_q4_attention(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor&
 int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound) {
   // every row in one pass where that takes at most 256 MiB, else as many as fit (a token at least)
   const int grp = H / G;
+  if (fused_fits(qa_slots(bound), T, grp, G)) return 0;
   const int64_t per_row = static_cast<int64_t>(B) * G * qa_slots(bound) * (D + 2) * 4;
   const int64_t all = padded_rows(static_cast<int64_t>(T) * grp), least = padded_rows(grp);
   const int64_t fit = (256ll << 20) / per_row / QA_ROWS * QA_ROWS;
@@ -624,7 +738,7 @@ extern "C" {
 int64_t evs_q4_attention_workspace(const evs_q4_cache* cache, const evs_q4_rows* rows, int n_heads, int max_length) {
   if (q4_check_cache(cache) != EVS_OK || q4_check_rows(cache, rows) != EVS_OK || n_heads < cache->kv_heads ||
       n_heads % cache->kv_heads != 0 || max_length < 0)
-    return 0;
+    return -1;
   return q4_attention_ws(rows->batch, rows->tokens, cache->kv_heads, cache->head_dim, n_heads,
                          bound_of(cache, rows, max_length));
 }
@@ -634,7 +748,7 @@ int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
                      void* workspace, int64_t workspace_bytes, cudaStream_t st) {
   EVS_TRY(q4_check_cache(cache));
   EVS_TRY(q4_check_rows(cache, rows));
-  EVS_CHECK_ARG(q && out && q_strides && out_strides && workspace, "null argument");
+  EVS_CHECK_ARG(q && out && q_strides && out_strides && (workspace || workspace_bytes == 0), "null argument");
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 attention: q must be fp32 or bf16");
   EVS_CHECK_ARG(n_heads >= cache->kv_heads && n_heads % cache->kv_heads == 0,
                 "q4 attention: n_heads must be a multiple of kv_heads");

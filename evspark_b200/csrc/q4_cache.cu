@@ -27,26 +27,6 @@ struct RopeFreq {
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, bool vec) {
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(p[j]);
-    return;
-  }
-  if constexpr (sizeof(T) == 2) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = (&r.x)[j];
-      v[2 * j] = __uint_as_float(w << 16);
-      v[2 * j + 1] = __uint_as_float(w & 0xFFFF0000u);
-    }
-  } else {
-    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
-  }
-}
-template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec) {
   if (!vec) {
 #pragma unroll
@@ -127,8 +107,8 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
     for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 0.f;
     if (row >= total) return;
     const T* p = row < H ? q_at + row * q.sh : (row < H + G ? k_at + (row - H) * k.sh : v_at + (row - H - G) * v.sh);
-    load8<T>(lo, p, vec != 0);
-    load8<T>(hi, p + half, vec != 0);
+    q4_load8<T>(lo, p, vec != 0);
+    q4_load8<T>(hi, p + half, vec != 0);
   };
   load(r);  // on its way while the angles are computed
   if (threadIdx.x < half && static_cast<int>(blockIdx.y) * per < H + G) {
@@ -293,11 +273,6 @@ __global__ void __launch_bounds__(APP_THREADS)
   }
 }
 
-bool vec_ok(const Q4Tensor& x, size_t el) {
-  return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.sb * el) % 16 == 0 && (x.st * el) % 16 == 0 &&
-         (x.sh * el) % 16 == 0;
-}
-
 }  // namespace
 
 int q4_check_cache(const evs_q4_cache* c) {
@@ -340,9 +315,16 @@ Q4RowsDev q4_rows_dev(const evs_q4_rows* r) {
 int launch_q4_append(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& k, const Q4Tensor& v,
                      const Q4Tensor& q_out, int H, int dtype, double rope_base, cudaStream_t st, bool pdl) {
   const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
-  const int vec = vec_ok(k, el) && vec_ok(v, el) && vec_ok(q, el) && vec_ok(q_out, el);
-  RopeFreq f;
-  for (int j = 0; j < c.D / 2; ++j) f.f[j] = std::pow(rope_base, -2.0 * j / c.D);
+  const int vec = q4_vec(k, el) && q4_vec(v, el) && q4_vec(q, el) && q4_vec(q_out, el);
+  // the frequencies of the last (base, head size), which a caller rarely changes: 64 powers take 2.5 us
+  thread_local double f_base = 0.0;
+  thread_local int f_dim = 0;
+  thread_local RopeFreq f;
+  if (f_base != rope_base || f_dim != c.D) {
+    for (int j = 0; j < c.D / 2; ++j) f.f[j] = std::pow(rope_base, -2.0 * j / c.D);
+    f_base = rope_base;
+    f_dim = c.D;
+  }
   const int per = APP_THREADS / (c.D / 16);
   // few tokens: their head rows over several CTAs; many: one CTA a token, so that the angles of a
   // token are computed once
@@ -358,7 +340,7 @@ int launch_q4_append(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q,
 int launch_q4_read(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& k, const Q4Tensor& v, int dtype,
                    cudaStream_t st) {
   const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
-  const int vec = vec_ok(k, el) && vec_ok(v, el);
+  const int vec = q4_vec(k, el) && q4_vec(v, el);
   const int tokens = r.B * r.T;
   const dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS));
   EVS_CHECK_ARG(grid.y <= 65535, "q4 read: too many heads");

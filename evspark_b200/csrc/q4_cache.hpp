@@ -28,6 +28,32 @@ struct Q4Tensor {
   int64_t sb, st, sh;
 };
 
+// whether eight values at a time can be moved as 16-byte words
+inline bool q4_vec(const Q4Tensor& x, size_t el) {
+  return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.sb * el) % 16 == 0 && (x.st * el) % 16 == 0 &&
+         (x.sh * el) % 16 == 0;
+}
+template <typename T>
+__device__ __forceinline__ void q4_load8(float (&v)[8], const T* p, bool vec) {
+  if (!vec) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(p[j]);
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = (&r.x)[j];
+      v[2 * j] = __uint_as_float(w << 16);
+      v[2 * j + 1] = __uint_as_float(w & 0xFFFF0000u);
+    }
+  } else {
+    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+  }
+}
+
 // row b's length and its new tokens; false when they lie outside the page table's positions or T
 __device__ __forceinline__ bool q4_row(const Q4RowsDev& r, int b, int* len, int* count, int P) {
   *len = r.lengths[b];

@@ -364,8 +364,8 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
         if len(cache._workspace) >= 256:
             cache._workspace.clear()
         cache._workspace[sizes] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     _call(dev, "evs_q4_attention", cache._ref, rp, q.data_ptr(), _strides(q), H,
           cache.head_dim ** -0.5 if scale is None else float(scale), ml, out.data_ptr(), _strides(out), dt,
-          ws.data_ptr(), need)
+          None if ws is None else ws.data_ptr(), max(need, 0))
     return out

@@ -257,6 +257,11 @@ def test_attention_bits_depend_on_the_token_alone(q4, start, T, H, G, D, dtype):
     for t in (0, 1, T // 2, T - 1):
         step = q4.q4_attention(q[:1, t:t + 1], cache, table[:1], i32([start + t]), max_length=start + t + 1)
         assert torch.equal(step[0, 0], block[0, t]), t
+    # a table with room for more (its empty entries are never read) takes the two-kernel path at any length
+    roomy = torch.full((1, 64 + table.shape[1]), -1, dtype=torch.int32, device=DEV)
+    roomy[:, :table.shape[1]] = table[:1]
+    assert torch.equal(q4.q4_attention(q[:1], cache, roomy, i32([start]))[0], block[0])
+    cache.check()
     other, ot = make_rows(q4, [end], 16, G, D, seed=5)
     q4.q4_kv_append(other, ot, i32([0]), k[:1], v[:1])
     wide = torch.zeros(1, T, H, D + 3, dtype=dtype, device=DEV)

@@ -123,12 +123,12 @@ def test_entry_points_refuse_bad_arguments():
 
     for c in [dict(head_dim=48), dict(page_size=24), dict(num_pages=0), dict(kv_heads=0), dict(pool=None), dict(pool=one + 4)]:
         a, w, p = run({**good, **c}, rows)
-        assert a == p == N.EVS_EINVAL and w == 0, c
+        assert a == p == N.EVS_EINVAL and w == -1, c
     for r in [dict(page_table=None), dict(lengths=None), dict(table_stride=2), dict(max_pages=0), dict(batch=0), dict(tokens=0)]:
         a, w, p = run(good, {**rows, **r})
-        assert a == p == N.EVS_EINVAL and w == 0, r
+        assert a == p == N.EVS_EINVAL and w == -1, r
     a, w, p = run(good, {**rows, "max_pages": 1 << 27, "table_stride": 1 << 27})
-    assert a == p == N.EVS_ERANGE and w == 0
+    assert a == p == N.EVS_ERANGE and w == -1
     assert run(good, rows, H=3)[0] == run(good, rows, H=1)[0] == run(good, rows, dtype=5)[0] == N.EVS_EINVAL
     assert run(good, rows, ws=None)[0] == run(good, rows, ws=one + 4)[0] == run(good, rows, ml=-1)[0] == N.EVS_EINVAL
     d, r = N.Q4CacheDesc(**good), N.Q4RowsDesc(**rows)
@@ -139,7 +139,9 @@ def test_entry_points_refuse_bad_arguments():
 def test_workspace_is_bounded_and_covers_a_token():
     d = N.Q4CacheDesc(256, None, 1 << 20, 64, 32, 128)
     lib = N.lib()
-    for tokens, H, ml in [(1, 32, 300), (13, 32, 65549), (1024, 32, 262144), (4096, 256, 262144)]:
+    r = N.Q4RowsDesc(256, 256, None, 4096, 4096, 1, 13)
+    assert lib.evs_q4_attention_workspace(C.byref(d), C.byref(r), 32, 2048) == 0  # one cluster folds it
+    for tokens, H, ml in [(1, 32, 3000), (13, 32, 65549), (1024, 32, 262144), (4096, 256, 262144)]:
         r = N.Q4RowsDesc(256, 256, None, 4096, 4096, 1, tokens)
         w = lib.evs_q4_attention_workspace(C.byref(d), C.byref(r), H, ml)
         assert 0 < w <= 320 << 20
