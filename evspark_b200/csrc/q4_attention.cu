@@ -4,7 +4,7 @@
 // Split-KV. A warp takes a unit of consecutive keys for a tile of 16 query rows (a row is one token
 // of one query head of the kv head) and runs an online softmax over it; the four units of a CTA are
 // folded in order, and a second kernel folds the CTAs' partial results in order.  The unit's length
-// depends on the row's own position alone (32 keys below 1024, 64 below 4096, 256 below 131072, else 512), so a
+// depends on the row's own position alone (32 keys below 1024, 64 below 4096, 256 below 131072, else 1024), so a
 // token's result does not depend on what else is in the call: verify blocks and single steps agree
 // bit for bit.
 #include <math_constants.h>
@@ -32,7 +32,7 @@ __host__ __device__ constexpr int qa_class(int64_t pos) {
 __host__ __device__ constexpr int64_t qa_class_end(int cl) {
   return cl == 0 ? 1024 : (cl == 1 ? 4096 : (cl == 2 ? 131072 : (1ll << 40)));
 }
-__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 2048)); }
+__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 4096)); }
 // partial results of one row for lengths up to bound
 inline int qa_slots(int64_t bound) {
   int n = 1;
@@ -69,7 +69,11 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr int qa_parts_q(size_t elem) { return elem == 2 ? 1 : 3; }  // bf16 parts of a query value
-constexpr int qa_parts_p(size_t elem) { return elem == 2 ? 2 : 3; }  // ... and of a probability
+// ... and of a probability.  One for bf16 queries: the weight of a key is then off by at most 2^-8 of
+// itself, beside outputs that are rounded by as much once more (relative error against 64 bits 1.7e-3
+// to 1.75e-3 at 1,024 keys); a second part cost a third of the products, 170 us instead of 154 at 64k
+// keys and 540 instead of 479 at 262k.  The sums of the weights take them unrounded.
+constexpr int qa_parts_p(size_t elem) { return elem == 2 ? 1 : 3; }
 
 // The K codes and scales of 32 keys, as one thread multiplies them: per 16-key chunk two 8-key tiles,
 // of which it holds key 4 (g / 2) + g % 2 + 2 u, features c DH / 4 .. + DH / 4 - 1.

@@ -20,6 +20,7 @@ counterpart: it runs its target in bf16 (evspark/api.py:94-98).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -44,20 +45,25 @@ def _need_cuda(t: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} must be a CUDA tensor")
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() builds a Stream object: 2 us a call
+# A decode step's calls are a few microseconds long on the device, so the host side counts: the raw stream
+# (current_stream() builds a Stream object, 2 us a call), device indices instead of torch.device objects, and
+# the C structs packed as bytes.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 _fns: dict = {}
+_pack_rows = struct.Struct("@PPPqiii4x").pack  # evs_q4_rows
+_pack_strides = struct.Struct("@3q").pack
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """One library call on the current stream of ``device``."""
+def _call(index: int, name: str, *args) -> None:
+    """One library call on the current stream of device ``index``."""
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(N.lib(), name)
-    index = device.index
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = fn(*args, _raw_stream(index))
     if status:
         N.check(status, name)
@@ -91,6 +97,7 @@ class Q4Weight:
         _need_cuda(codes, "Q4Weight: codes")
         self.codes, self.scales, self.shape, self.group = codes, scales, (n, k), int(group)
         self._args = (codes.data_ptr(), scales.data_ptr(), n, k, self.group)
+        self._index = codes.get_device()
 
     @property
     def device(self) -> torch.device:
@@ -106,7 +113,7 @@ class Q4Weight:
             raise ValueError(f"dequantize: dtype must be bf16 or fp32, got {dtype}")
         n, k = self.shape
         out = torch.empty(n, k, dtype=dtype, device=self.device)
-        _call(self.device, "evs_q4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), n, k, self.group,
+        _call(self._index, "evs_q4_dequantize", self.codes.data_ptr(), self.scales.data_ptr(), n, k, self.group,
               out.data_ptr(), _DT[dtype], k)
         return out
 
@@ -125,7 +132,7 @@ def quantize_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
     kp = padded_features(k)
     codes = torch.empty(n, kp // 2, dtype=torch.uint8, device=w.device)
     scales = torch.empty(kp // group, n, dtype=torch.bfloat16, device=w.device)
-    _call(w.device, "evs_q4_quantize", w.data_ptr(), dt, max(w.stride(0), k), n, k, group, codes.data_ptr(),
+    _call(w.get_device(), "evs_q4_quantize", w.data_ptr(), dt, max(w.stride(0), k), n, k, group, codes.data_ptr(),
           scales.data_ptr())
     return Q4Weight(codes, scales, (n, k), group)
 
@@ -137,22 +144,24 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
     bf16 rows multiply the held weight values exactly; fp32 rows are used at full precision.  A row's
     result does not depend on the other rows.  Meant for the few tokens of a decode step or verify
     block: every 64 rows read the weight once."""
-    n, k = w.shape
-    dt = _dtype(x, "q4_linear: x")
-    shape, dev = x.shape, w.codes.device
+    codes, scales, n, k, group = w._args
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        dt = _dtype(x, "q4_linear: x")
+    shape = x.shape
     if not shape or shape[-1] != k:
         raise ValueError(f"q4_linear: x must be [..., {k}], got {tuple(shape)}")
-    if x.device != dev:
-        raise ValueError(f"q4_linear: x on {x.device}, the weight on {dev}")
+    if x.get_device() != w._index:
+        raise ValueError(f"q4_linear: x on {x.device}, the weight on {w.codes.device}")
     if out is not None:
-        if out.shape != (*shape[:-1], n) or out.device != dev or not out.is_contiguous():
+        if out.shape != shape[:-1] + (n,) or out.get_device() != w._index or not out.is_contiguous():
             raise ValueError(f"q4_linear: out must be a contiguous [..., {n}] tensor of x's batch shape and device")
         odt = _dtype(out, "q4_linear: out")
     else:
         odt = _DT.get(out_dtype)
         if odt is None:
             raise ValueError(f"q4_linear: out_dtype must be bf16 or fp32, got {out_dtype}")
-        out = torch.empty((*shape[:-1], n), dtype=out_dtype, device=dev)
+        out = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
     m = x.numel() // k
     if m == 0:
         return out
@@ -162,7 +171,7 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
             ldx = x.stride(0)
         else:
             x = x.contiguous()
-    _call(dev, "evs_q4_linear", x.data_ptr(), dt, ldx, m, *w._args, out.data_ptr(), odt, n)
+    _call(w._index, "evs_q4_linear", x.data_ptr(), dt, ldx, m, codes, scales, n, k, group, out.data_ptr(), odt, n)
     return out
 
 
@@ -216,6 +225,7 @@ class Q4Cache:
         self._err = torch.zeros(3, dtype=torch.int32, device=pool.device)
         self._desc = N.Q4CacheDesc(pool.data_ptr(), self._err.data_ptr(), num_pages, page_size, kv_heads, head_dim)
         self._ref = C.addressof(self._desc)
+        self._index = pool.get_device()
         self._workspace: dict = {}  # attention workspace bytes by call sizes
 
     @property
@@ -231,38 +241,39 @@ class Q4Cache:
                              f"or a page id outside the pool [evs status {code}, kernel {where}]")
 
 
-_Strides = C.c_int64 * 3
-
-
-def _strides(t: torch.Tensor):
-    return _Strides(*t.stride()[:3])
-
-
 def _rows(cache: Q4Cache, page_table, lengths, counts, batch: int, tokens: int, what: str):
-    dev = cache.pool.device
-    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch
-            or page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1)
-            or (batch > 1 and page_table.stride(0) < page_table.shape[1])):
+    """The checked evs_q4_rows of a call, packed, and its table's positions."""
+    index = cache._index
+    shape, strides = page_table.shape, page_table.stride()
+    if (page_table.dtype != torch.int32 or len(shape) != 2 or shape[0] != batch or shape[1] < 1
+            or (shape[1] > 1 and strides[1] != 1) or (batch > 1 and strides[0] < shape[1])):
         raise ValueError(f"{what}: page_table must be int32 [{batch}, max_pages] with contiguous rows")
     if lengths.dtype != torch.int32 or lengths.shape != (batch,) or not lengths.is_contiguous():
         raise ValueError(f"{what}: lengths must be a contiguous int32 [{batch}] tensor")
-    if page_table.device != dev or lengths.device != dev:
-        raise ValueError(f"{what}: page_table and lengths must be on the cache's device {dev}")
-    cp = None
+    if page_table.get_device() != index or lengths.get_device() != index:
+        raise ValueError(f"{what}: page_table and lengths must be on the cache's device {cache.pool.device}")
+    cp = 0
     if counts is not None:
-        if counts.dtype != torch.int32 or counts.shape != (batch,) or not counts.is_contiguous() or counts.device != dev:
-            raise ValueError(f"{what}: counts must be a contiguous int32 [{batch}] tensor on {dev}")
+        if (counts.dtype != torch.int32 or counts.shape != (batch,) or not counts.is_contiguous()
+                or counts.get_device() != index):
+            raise ValueError(f"{what}: counts must be a contiguous int32 [{batch}] tensor on {cache.pool.device}")
         cp = counts.data_ptr()
-    mp = page_table.shape[1]
-    return N.Q4RowsDesc(page_table.data_ptr(), lengths.data_ptr(), cp, max(page_table.stride(0), mp), mp, batch, tokens)
+    mp = shape[1]
+    if batch > 2 ** 31 - 1 or tokens > 2 ** 31 - 1 or mp > 2 ** 31 - 1:
+        raise ValueError(f"{what}: too large a call")
+    return _pack_rows(page_table.data_ptr(), lengths.data_ptr(), cp, max(strides[0], mp), mp, batch, tokens), \
+        mp * cache.page_size
 
 
-def _heads(t: torch.Tensor, batch: int, tokens: int, heads: int, dim: int, dtype, dev, name: str) -> None:
-    if t.shape != (batch, tokens, heads, dim) or t.dtype != dtype or t.device != dev:
-        raise ValueError(f"{name} must be {dtype} [{batch}, {tokens}, {heads}, {dim}] on {dev}, "
+def _heads(t: torch.Tensor, shape: tuple, dtype, index: int, name: str) -> bytes:
+    """The packed strides of a checked [B, T, heads, D] tensor."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be {dtype} {list(shape)} on cuda:{index}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.stride(3) != 1:
+    sb, st, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
+    return _pack_strides(sb, st, sh)
 
 
 def q4_kv_append(cache: Q4Cache, page_table: torch.Tensor, lengths: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
@@ -278,27 +289,29 @@ def q4_kv_append(cache: Q4Cache, page_table: torch.Tensor, lengths: torch.Tensor
     position * rope_base^(-2 j / D) in fp64 for any position; k is quantised unrounded."""
     if k.dim() != 4:
         raise ValueError(f"q4_kv_append: k must be [B, T, kv_heads, D], got {tuple(k.shape)}")
-    B, T = k.shape[0], k.shape[1]
-    dev, dt = cache.pool.device, _dtype(k, "q4_kv_append: k")
-    _heads(k, B, T, cache.kv_heads, cache.head_dim, k.dtype, dev, "q4_kv_append: k")
-    _heads(v, B, T, cache.kv_heads, cache.head_dim, k.dtype, dev, "q4_kv_append: v")
-    rows = _rows(cache, page_table, lengths, counts, B, T, "q4_kv_append")
-    H = 0
-    qs = qos = None
+    B, T = k.shape[:2]
+    dt, dtype, index, D = _dtype(k, "q4_kv_append: k"), k.dtype, cache._index, cache.head_dim
+    shape = (B, T, cache.kv_heads, D)
+    ks = _heads(k, shape, dtype, index, "q4_kv_append: k")
+    vs = _heads(v, shape, dtype, index, "q4_kv_append: v")
+    rows, _ = _rows(cache, page_table, lengths, counts, B, T, "q4_kv_append")
+    H, qs, qos, qp, qop = 0, None, None, None, None
     if q is not None:
         H = q.shape[2] if q.dim() == 4 else 0
-        _heads(q, B, T, H, cache.head_dim, k.dtype, dev, "q4_kv_append: q")
+        shape = (B, T, H, D)
+        qs = _heads(q, shape, dtype, index, "q4_kv_append: q")
         if q_out is None:
-            q_out = torch.empty(B, T, H, cache.head_dim, dtype=q.dtype, device=dev)
-        else:
-            _heads(q_out, B, T, H, cache.head_dim, k.dtype, dev, "q4_kv_append: q_out")
-        qs, qos = _strides(q), _strides(q_out)
+            q_out = q.new_empty(shape)
+        qos = _heads(q_out, shape, dtype, index, "q4_kv_append: q_out")
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+        if H < 1:
+            raise ValueError("q4_kv_append: q needs at least one head")
     elif q_out is not None:
         raise ValueError("q4_kv_append: q_out without q")
     if B == 0 or T == 0:
         return q_out
-    _call(dev, "evs_q4_kv_append", cache._ref, C.byref(rows), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
-          N.ptr(q), qs, N.ptr(q_out), qos, H, dt, float(rope_base))
+    _call(index, "evs_q4_kv_append", cache._ref, rows, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, qop, qos, H, dt,
+          rope_base)
     return q_out
 
 
@@ -307,20 +320,23 @@ def q4_kv_read(cache: Q4Cache, page_table: torch.Tensor, starts: torch.Tensor, t
                out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values that the cache holds at positions starts[b] .. starts[b] + counts[b] - 1 (counts
     None: ``tokens`` each) -> k, v [B, tokens, kv_heads, D] (padding behind counts[b] is left unwritten)."""
-    B, dev = starts.shape[0] if starts.dim() == 1 else -1, cache.pool.device
+    B, index = starts.shape[0] if starts.dim() == 1 else -1, cache._index
     tokens = int(tokens)
-    rows = _rows(cache, page_table, starts, counts, B, tokens, "q4_kv_read")
+    if tokens < 0:
+        raise ValueError(f"q4_kv_read: tokens must not be negative, got {tokens}")
+    rows, _ = _rows(cache, page_table, starts, counts, B, tokens, "q4_kv_read")
+    shape = (B, tokens, cache.kv_heads, cache.head_dim)
     if out is None:
         if dtype not in _DT:
             raise ValueError(f"q4_kv_read: dtype must be bf16 or fp32, got {dtype}")
-        out = tuple(torch.empty(B, tokens, cache.kv_heads, cache.head_dim, dtype=dtype, device=dev) for _ in range(2))
+        out = tuple(torch.empty(shape, dtype=dtype, device=cache.pool.device) for _ in range(2))
     k, v = out
     dt = _dtype(k, "q4_kv_read: k")
-    _heads(k, B, tokens, cache.kv_heads, cache.head_dim, k.dtype, dev, "q4_kv_read: k")
-    _heads(v, B, tokens, cache.kv_heads, cache.head_dim, k.dtype, dev, "q4_kv_read: v")
+    ks = _heads(k, shape, k.dtype, index, "q4_kv_read: k")
+    vs = _heads(v, shape, k.dtype, index, "q4_kv_read: v")
     if B == 0 or tokens == 0:
         return k, v
-    _call(dev, "evs_q4_kv_read", cache._ref, C.byref(rows), k.data_ptr(), _strides(k), v.data_ptr(), _strides(v), dt)
+    _call(index, "evs_q4_kv_read", cache._ref, rows, k.data_ptr(), ks, v.data_ptr(), vs, dt)
     return k, v
 
 
@@ -339,33 +355,37 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
     batch, the other tokens of the call, max_length or the page size."""
     if q.dim() != 4:
         raise ValueError(f"q4_attention: q must be [B, T, heads, D], got {tuple(q.shape)}")
-    B, T, H = q.shape[0], q.shape[1], q.shape[2]
-    dev, dt = cache.pool.device, _dtype(q, "q4_attention: q")
+    B, T, H, _ = q.shape
+    dt, index = _dtype(q, "q4_attention: q"), cache._index
     if H < 1 or H % cache.kv_heads:
         raise ValueError(f"q4_attention: heads ({H}) must be a multiple of kv_heads ({cache.kv_heads})")
-    _heads(q, B, T, H, cache.head_dim, q.dtype, dev, "q4_attention: q")
-    if scale is not None and not 0.0 < scale < float("inf"):
+    shape = (B, T, H, cache.head_dim)
+    qs = _heads(q, shape, q.dtype, index, "q4_attention: q")
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    elif not 0.0 < scale < float("inf"):
         raise ValueError(f"q4_attention: scale must be positive and finite, got {scale}")
-    if max_length is not None and max_length < 1:
+    if max_length is not None and not 1 <= max_length < 2 ** 31:
         raise ValueError(f"q4_attention: max_length must be positive, got {max_length}")
-    rows = _rows(cache, page_table, lengths, counts, B, T, "q4_attention")
+    rows, positions = _rows(cache, page_table, lengths, counts, B, T, "q4_attention")
     if out is None:
-        out = torch.empty(B, T, H, cache.head_dim, dtype=q.dtype, device=dev)
-    else:
-        _heads(out, B, T, H, cache.head_dim, q.dtype, dev, "q4_attention: out")
+        out = q.new_empty(shape)
+    os_ = _heads(out, shape, q.dtype, index, "q4_attention: out")
     if B == 0 or T == 0:
         return out
-    ml = 0 if max_length is None else int(max_length)
-    rp = C.byref(rows)
-    sizes = (B, T, H, ml or rows.max_pages * cache.page_size)
+    ml = 0 if max_length is None else max_length
+    sizes = (B, T, H, ml or positions)
     need = cache._workspace.get(sizes)
     if need is None:
-        need = N.lib().evs_q4_attention_workspace(cache._ref, rp, H, ml)
+        need = N.lib().evs_q4_attention_workspace(cache._ref, rows, H, ml)
         if len(cache._workspace) >= 256:
             cache._workspace.clear()
         cache._workspace[sizes] = need
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    _call(dev, "evs_q4_attention", cache._ref, rp, q.data_ptr(), _strides(q), H,
-          cache.head_dim ** -0.5 if scale is None else float(scale), ml, out.data_ptr(), _strides(out), dt,
-          None if ws is None else ws.data_ptr(), max(need, 0))
+    ws, wp = None, None
+    if need > 0:
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.pool.device)
+        wp = ws.data_ptr()
+    else:
+        need = 0
+    _call(index, "evs_q4_attention", cache._ref, rows, q.data_ptr(), qs, H, scale, ml, out.data_ptr(), os_, dt, wp, need)
     return out

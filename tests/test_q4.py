@@ -27,14 +27,14 @@ def weight(n=8, k=100, group=32):
     kp = q4.padded_features(k)
     w.codes, w.scales = torch.zeros(n, kp // 2, dtype=torch.uint8), torch.zeros(kp // group, n, dtype=torch.bfloat16)
     w.shape, w.group = (n, k), group
-    w._args = ()
+    w._args, w._index = (0, 0, n, k, group), -1
     return w
 
 
 def cache(pages=4, G=2, D=64, page=16):
     c = q4.Q4Cache.__new__(q4.Q4Cache)
     c.pool = torch.zeros(pages, G, q4.Q4Cache.block_bytes(D, page), dtype=torch.uint8)
-    c.num_pages, c.kv_heads, c.head_dim, c.page_size = pages, G, D, page
+    c.num_pages, c.kv_heads, c.head_dim, c.page_size, c._index = pages, G, D, page, -1
     return c
 
 
