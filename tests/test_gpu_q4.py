@@ -218,6 +218,11 @@ ATTEND = [  # starts, T, counts, H, G, D, page, dtype
     ([4095, 4096, 10], 2, None, 2, 1, 32, 64, F32),
     ([65530], 13, None, 1, 1, 32, 128, F32),
     ([70000, 20], 2, None, 2, 1, 32, 128, BF),
+    # many rows a kv head beyond the fused lengths: warps share the decoding of the keys
+    ([2500, 60, 4090], 13, [13, 5, 13], 16, 2, 128, 64, BF),
+    ([2300], 7, None, 20, 2, 64, 48, F32),
+    ([3001, 0], 16, [16, 9], 12, 3, 32, 16, BF),
+    ([5000], 40, None, 2, 2, 128, 32, F32),
 ]
 
 
@@ -242,7 +247,8 @@ def test_attention(q4, starts, T, counts, H, G, D, page, dtype):
 
 
 @pytest.mark.parametrize("start,T,H,G,D,dtype", [(250, 13, 8, 2, 64, BF), (4088, 16, 3, 1, 32, BF), (1000, 9, 6, 2, 128, F32),
-                                                 (65529, 13, 1, 1, 32, BF)])
+                                                 (65529, 13, 1, 1, 32, BF), (3500, 13, 16, 2, 128, BF),
+                                                 (1020, 12, 20, 2, 32, F32), (131070, 5, 16, 1, 32, BF)])
 def test_attention_bits_depend_on_the_token_alone(q4, start, T, H, G, D, dtype):
     """A verify block, single steps, another batch, page size, bound and strides give the same bits."""
     end = start + T
@@ -270,12 +276,14 @@ def test_attention_bits_depend_on_the_token_alone(q4, start, T, H, G, D, dtype):
     assert torch.equal(got[0], block[0])
 
 
-def test_attention_nan_keys_and_values_reach_only_who_sees_them(q4):
+@pytest.mark.parametrize("H,room", [(2, 0), (2, 200), (12, 200)])  # one cluster; two kernels; shared decoding
+def test_attention_nan_keys_and_values_reach_only_who_sees_them(q4, H, room):
     D, G, T, start = 64, 1, 6, 60
     cache, table = make_rows(q4, [start + T], 16, G, D)
+    table = torch.cat([table, torch.full((1, room), -1, dtype=torch.int32, device=DEV)], 1)
     k, v = randn(1, start + T, G, D, seed=1), randn(1, start + T, G, D, seed=2)
     q4.q4_kv_append(cache, table, i32([0]), k, v)
-    q = randn(1, T, 2, D, seed=3)
+    q = randn(1, T, H, D, seed=3)
     clean = q4.q4_attention(q, cache, table, i32([start]))
     vb, kb = v.clone(), k.clone()
     vb[0, start + 2, 0, 40] = math.nan  # the token at start + 2, second group of features
@@ -321,6 +329,15 @@ def test_bad_pages_and_lengths_are_reported_not_followed(q4):
     with pytest.raises(RuntimeError):
         cache.check()
     assert bool(q4.q4_attention(q, cache, table, lengths, counts=i32([2, 3, 2, 2]))[1].isnan().all())
+    with pytest.raises(RuntimeError):
+        cache.check()
+    # the same with many rows a head and room in the table (shared decoding, two kernels)
+    many = randn(4, 12, 6, 64, seed=4)
+    room = torch.cat([bad, torch.full((4, 200), -1, dtype=torch.int32, device=DEV)], 1)
+    got = q4.q4_attention(many, cache, room, i32([28, 28, 28, -2]))
+    fine = q4.q4_attention(many[:1], cache, table[:1], i32([28]))
+    # row 1 misses its second page (positions 16 .. 31), which every token from 28 on sees
+    assert torch.equal(got[0], fine[0]) and bool(got[1:].isnan().all())
     with pytest.raises(RuntimeError):
         cache.check()
     # a bound below the true length is noted, and that row's result is NaN
