@@ -24,6 +24,10 @@ constexpr int QA_ROWS = 16;
 constexpr int QA_CLUSTER = 8;  // slots that one cluster folds: contexts of up to 2,048 keys
 constexpr int NS = 2;           // 16-key chunks per online-softmax step of a warp
 constexpr int QA_STEP = 16 * NS;
+// A row's sums are taken relative to 2^m; m moves up only when a score passes it by more than this (in
+// powers of two), as moving it costs a product per output. Sums in fp32 and probabilities in bf16 keep
+// their relative accuracy below 2^8.
+constexpr float QA_SLACK = 8.f;
 
 // length class of a position, and keys per CTA of a class
 __host__ __device__ constexpr int qa_class(int64_t pos) {
@@ -308,32 +312,35 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
               for (int e = 0; e < 4; ++e)
                 if (key + 16 * sub + 4 * c + 2 * u + (e & 1) > lim[e >> 1]) s[sub][u][e] = -CUDART_INF_F;
       }
-      float mx[2];
+      float mx[2], a[2] = {1.f, 1.f};
 #pragma unroll
       for (int i = 0; i < 2; ++i) mx[i] = m[i];
 #pragma unroll
-        for (int sub = 0; sub < NS; ++sub)
+      for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[sub][u][e]);
+          for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[sub][u][e]);
       bool moved = false;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
         mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        moved |= mx[i] != m[i];
+        const float grow = (mx[i] - m[i]) * scale_log2;  // NaN while nothing is visible
+        if (grow > QA_SLACK) {
+          moved = true;
+          a[i] = ex2(-grow);
+          m[i] = mx[i];
+        }
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float a = mx[i] == m[i] ? 1.f : ex2((m[i] - mx[i]) * scale_log2);
-          m[i] = mx[i];
-          l[i] *= a;
+          l[i] *= a[i];
 #pragma unroll
           for (int n = 0; n < VN; ++n) {
-            o[n][2 * i] *= a;
-            o[n][2 * i + 1] *= a;
+            o[n][2 * i] *= a[i];
+            o[n][2 * i + 1] *= a[i];
           }
         }
       }
@@ -536,13 +543,22 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) acc[d] = 0.f;
 #pragma unroll
-    for (int x = 0; x < QA_CLUSTER; ++x)
-      if (x < n) {
-        const float f = mx[x] == -CUDART_INF_F ? 0.f : ex2(mx[x] - big);
-        sum = fmaf(sm[x], f, sum);
+    for (int w = 0; w < QA_WARPS; ++w) {
+      float part[DH / 32], ps = 0.f;
 #pragma unroll
-        for (int d = 0; d < DH / 32; ++d) acc[d] = fmaf(v[x][d], f, acc[d]);
-      }
+      for (int d = 0; d < DH / 32; ++d) part[d] = 0.f;
+#pragma unroll
+      for (int x = w; x < QA_CLUSTER; x += QA_WARPS)
+        if (x < n) {
+          const float f = mx[x] == -CUDART_INF_F ? 0.f : ex2(mx[x] - big);
+          ps = fmaf(sm[x], f, ps);
+#pragma unroll
+          for (int d = 0; d < DH / 32; ++d) part[d] = fmaf(v[x][d], f, part[d]);
+        }
+      sum += ps;
+#pragma unroll
+      for (int d = 0; d < DH / 32; ++d) acc[d] += part[d];
+    }
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
   }
@@ -551,20 +567,19 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// One warp per output row: the CTAs' partial results folded in order.
+// One CTA per output row: warp w folds the slots w, w + 4, ... in order, then the four sums in order.
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS)
-    q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int tc, int prows, int nslots,
+    q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int prows, int nslots,
                       const float* __restrict__ part_o, const float2* __restrict__ part_s) {
+  __shared__ float fold[QA_WARPS][DH + 1];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, b = blockIdx.z, kvh = blockIdx.y;
-  const int R = blockIdx.x * QA_WARPS + (threadIdx.x >> 5);
-  if (R >= tc * grp) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.z, kvh = blockIdx.y, R = blockIdx.x;
   const int t = t0 + R / grp;
   T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
   int n;
-  if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) return;
+  if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) return;  // the same for the whole CTA
   const size_t prow = ((static_cast<size_t>(b) * cache.G + kvh) * static_cast<size_t>(prows) + R) * nslots;
   float big = -CUDART_INF_F;
   for (int x = lane; x < n; x += 32) big = fmaxf(big, part_s[prow + x].x);
@@ -572,8 +587,8 @@ __global__ void __launch_bounds__(QA_THREADS)
   float acc[DH / 32], sum = 0.f;
 #pragma unroll
   for (int d = 0; d < DH / 32; ++d) acc[d] = 0.f;
-#pragma unroll 4
-  for (int x = 0; x < n; ++x) {
+#pragma unroll 8
+  for (int x = warp; x < n; x += QA_WARPS) {
     const float2 st = part_s[prow + x];
     const float f = st.x == -CUDART_INF_F ? 0.f : ex2(st.x - big);
     sum = fmaf(st.y, f, sum);
@@ -581,7 +596,15 @@ __global__ void __launch_bounds__(QA_THREADS)
     for (int d = 0; d < DH / 32; ++d) acc[d] = fmaf(part_o[(prow + x) * DH + 32 * d + lane], f, acc[d]);
   }
 #pragma unroll
-  for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
+  for (int d = 0; d < DH / 32; ++d) fold[warp][32 * d + lane] = acc[d];
+  if (lane == 0) fold[warp][DH] = sum;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= DH) return;
+  float v = fold[0][d], w = fold[0][DH];
+#pragma unroll
+  for (int i = 1; i < QA_WARPS; ++i) v += fold[i][d], w += fold[i][DH];
+  dst[d] = from_f32<T>(v / w);
 }
 
 inline int64_t padded_rows(int64_t rows) { return (rows + QA_ROWS - 1) / QA_ROWS * QA_ROWS; }
@@ -638,8 +661,8 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
     EVS_CUDA_TRY(evs_launch(kern, dim3(nslots, c.G * tiles, r.B), dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc,
                             tiles, scale_log2, nslots, q_vec, po, ps));
     // the combine may start while the last tiles run (it waits for them before it reads)
-    EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3((tc * grp + QA_WARPS - 1) / QA_WARPS, c.G, r.B),
-                            dim3(QA_THREADS), 0, st, true, c, r, out, grp, t0, tc, prows, nslots,
+    EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3(tc * grp, c.G, r.B), dim3(QA_THREADS), 0, st, true, c, r,
+                            out, grp, t0, prows, nslots,
                             static_cast<const float*>(po), static_cast<const float2*>(ps)));
     evs_count_launch(2);
   }
