@@ -51,10 +51,11 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec) {
 // bits.  Scale: t = absmax / 7 in fp32 is within 2^-22 of the exact quotient, so its five-bit rounding
 // is the exact one unless the dropped 19 bits lie within 4 units of a half (one group in 2^15).
 // Codes: the quotient x / s, corrected once by its exact remainder, is within 2^-23 of the exact one
-// (|x / s| < 8), and is a half exactly where x is; its rounding is the exact one unless it lies within
-// 2^-15 of a half.  Values, which are x themselves, may sit on a half (bf16 ones often do: x has eight
-// bits and s five, so x / s is a half or 2^-6 away from one); keys, rotated in 64 bits, are looked at
-// again there.
+// (|x / s| < 7.12, so its rounding needs no clamp), and is a half exactly where x is; its rounding is
+// the exact one unless it lies within 2^-15 of a half.  Keys, rotated in 64 bits, are looked at again
+// there.  Values are x themselves and may sit on a half.  Those of bf16 need no look at all: x = a 2^e
+// and s = b 2^f with a < 2^8 and b < 2^5, so a quotient above 0.49 that is not a half is at least
+// 1 / (2 max(b, a / 0.49)) > 2^-11 away from one.
 __device__ __forceinline__ bool scale_clear(float absmax) {
   const float t = absmax * (1.f / 7.f);
   return (__float_as_uint(t) & 0x7FFFFu) - 0x3FFFCu > 8u && t >= 2.f * Q4_TINY && t <= 0.5f * Q4_HUGE;
@@ -62,15 +63,26 @@ __device__ __forceinline__ bool scale_clear(float absmax) {
 __device__ __forceinline__ uint32_t scale_bits_fast(float absmax) {
   return (__float_as_uint(absmax * (1.f / 7.f)) + 0x40000u) >> 19 << 3;  // five significant bits, as bf16 bits
 }
-// code of x under scale s (inv = 1 / s to 2^-22), and the largest distance from its code's value so
-// far (a half of a value is no distance); adding 1.5 2^23 leaves the rounded quotient in the low bits
-__device__ __forceinline__ uint32_t code_fast(float x, float s, float inv, bool value, float& far) {
-  float q = x * inv;
-  q = fmaf(fmaf(-q, s, x), inv, q);
-  q = fminf(fmaxf(q, -7.25f), 7.25f);
-  const float y = q + 12582912.f, d = fabsf(q - (y - 12582912.f));
-  far = value && d == 0.5f ? far : fmaxf(far, d);
-  return __float_as_uint(y) - (0x4B400000u - 8u);
+// Codes of eight values under scale s (inv = 1 / s to 2^-22), value j's at bit 4 j, and the largest
+// distance from a code's value so far.  Adding 1.5 2^23 leaves the rounded quotient in the low bits;
+// the sum's other bits add up to one constant.
+enum Look { LOOK_NONE, LOOK_VALUES, LOOK_ALL };  // distances: none, but exact halves, every one
+template <Look LOOK>
+__device__ __forceinline__ uint32_t codes_fast(const float (&x)[8], float s, float inv, float& far) {
+  constexpr float SHIFT = 12582912.f;
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 7; j >= 0; --j) {
+    float q = x[j] * inv;
+    q = fmaf(fmaf(-q, s, x[j]), inv, q);
+    const float y = q + SHIFT;
+    if constexpr (LOOK != LOOK_NONE) {
+      const float d = fabsf(q - (y - SHIFT));
+      far = LOOK == LOOK_VALUES && d == 0.5f ? far : fmaxf(far, d);
+    }
+    w = w * 16u + __float_as_uint(y);
+  }
+  return w - (0x4B400000u - 8u) * 0x11111111u;
 }
 
 // One CTA per token (and block of head rows, where the call has few tokens).  D / 16 threads per head
@@ -148,6 +160,11 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
       store8<T>(o, lo, vec != 0);
       store8<T>(o + half, hi, vec != 0);
     }
+    const bool put = live && !is_q && page >= 0, more = r0 + static_cast<int>(gridDim.y) * per < total;
+    if (!__any_sync(0xffffffffu, put)) {  // a warp of queries
+      if (more) load(r + gridDim.y * per);
+      continue;
+    }
     // groups of 32 features: four threads of one half (D = 64, 128), or both halves of two threads (D = 32)
     auto group_max = [&](auto& ml, auto& mh, auto larger) {
       if (D == 32) ml = mh = larger(ml, mh);
@@ -158,16 +175,18 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
         mh = larger(mh, __shfl_xor_sync(0xffffffffu, mh, o));
       }
     };
-    // magnitudes as integers: the same order, with every NaN on top
-    uint32_t bl = 0, bh = 0;
+    // magnitudes as integers: the same order, with NaN on top (x 0 is one for a NaN and an infinity)
+    float xl = 0.f, xh = 0.f, zl = 0.f, zh = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      bl = max(bl, __float_as_uint(lo[j]) & 0x7FFFFFFFu);
-      bh = max(bh, __float_as_uint(hi[j]) & 0x7FFFFFFFu);
+      xl = fmaxf(xl, fabsf(lo[j]));
+      xh = fmaxf(xh, fabsf(hi[j]));
+      zl = fmaf(lo[j], 0.f, zl);
+      zh = fmaf(hi[j], 0.f, zh);
     }
+    uint32_t bl = zl == 0.f ? __float_as_uint(xl) : 0x7FC00000u, bh = zh == 0.f ? __float_as_uint(xh) : 0x7FC00000u;
     group_max(bl, bh, [](uint32_t a, uint32_t o) { return max(a, o); });
     const float ml = __uint_as_float(bl), mh = __uint_as_float(bh);
-    const bool put = live && !is_q && page >= 0;
     uint32_t sl = scale_bits_fast(ml), sh = scale_bits_fast(mh);
     if (__any_sync(0xffffffffu, put && !(scale_clear(ml) && scale_clear(mh)))) {
       double el = 0.0, eh = 0.0;
@@ -189,12 +208,15 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
       float il, ih;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(il) : "f"(fl));
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(ih) : "f"(fh));
-      uint32_t cl = 0, ch = 0;
+      uint32_t cl, ch;
       float far = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cl |= code_fast(lo[j], fl, il, !is_k, far) << (4 * j);
-        ch |= code_fast(hi[j], fh, ih, !is_k, far) << (4 * j);
+      if (is_k) {
+        cl = codes_fast<LOOK_ALL>(lo, fl, il, far);
+        ch = codes_fast<LOOK_ALL>(hi, fh, ih, far);
+      } else {
+        constexpr Look LOOK = sizeof(T) == 2 ? LOOK_NONE : LOOK_VALUES;
+        cl = codes_fast<LOOK>(lo, fl, il, far);
+        ch = codes_fast<LOOK>(hi, fh, ih, far);
       }
       // a scale of 0 or NaN makes every quotient infinite or NaN: the codes are 8
       const bool odd = !(ml <= FLT_MAX) || !(mh <= FLT_MAX) || sl == 0u || sh == 0u || sl == 0x7FC0u || sh == 0x7FC0u;
@@ -219,7 +241,7 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
         scales[(i / 4 + D / 64) * cache.P] = static_cast<uint16_t>(sh);
       }
     }
-    if (r0 + static_cast<int>(gridDim.y) * per < total) load(r + gridDim.y * per);
+    if (more) load(r + gridDim.y * per);
   }
 }
 
