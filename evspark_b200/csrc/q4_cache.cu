@@ -113,14 +113,12 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
   const T* q_at = static_cast<const T*>(q.p) + b * q.sb + t * q.st + 8 * i;
   const T* k_at = static_cast<const T*>(k.p) + b * k.sb + t * k.st + 8 * i;
   const T* v_at = static_cast<const T*>(v.p) + b * v.sb + t * v.st + 8 * i;
-  float lo[8], hi[8];
+  Q4Raw8<T> next_lo, next_hi;
   auto load = [&](int row) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) lo[j] = hi[j] = 0.f;
     if (row >= total) return;
     const T* p = row < H ? q_at + row * q.sh : (row < H + G ? k_at + (row - H) * k.sh : v_at + (row - H - G) * v.sh);
-    q4_load8<T>(lo, p, vec != 0);
-    q4_load8<T>(hi, p + half, vec != 0);
+    next_lo.load(p, vec != 0);
+    next_hi.load(p + half, vec != 0);
   };
   load(r);  // on its way while the angles are computed
   if (threadIdx.x < half && static_cast<int>(blockIdx.y) * per < H + G) {
@@ -136,6 +134,10 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
   for (int r0 = blockIdx.y * per; r0 < total; r0 += gridDim.y * per, r += gridDim.y * per) {
     const bool live = r < total, is_q = r < H, is_k = !is_q && r < H + G;
     const int head = is_q ? r : (is_k ? r - H : r - H - G);
+    float lo[8], hi[8];
+    next_lo.get(lo);
+    next_hi.get(hi);
+    load(r + gridDim.y * per);  // on its way while this row is worked on
     if (is_q || is_k) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -160,11 +162,8 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
       store8<T>(o, lo, vec != 0);
       store8<T>(o + half, hi, vec != 0);
     }
-    const bool put = live && !is_q && page >= 0, more = r0 + static_cast<int>(gridDim.y) * per < total;
-    if (!__any_sync(0xffffffffu, put)) {  // a warp of queries
-      if (more) load(r + gridDim.y * per);
-      continue;
-    }
+    const bool put = live && !is_q && page >= 0;
+    if (!__any_sync(0xffffffffu, put)) continue;  // a warp of queries
     // groups of 32 features: four threads of one half (D = 64, 128), or both halves of two threads (D = 32)
     auto group_max = [&](auto& ml, auto& mh, auto larger) {
       if (D == 32) ml = mh = larger(ml, mh);
@@ -241,7 +240,6 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
         scales[(i / 4 + D / 64) * cache.P] = static_cast<uint16_t>(sh);
       }
     }
-    if (more) load(r + gridDim.y * per);
   }
 }
 

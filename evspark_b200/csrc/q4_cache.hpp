@@ -1,6 +1,8 @@
 // Device views of the paged 4-bit KV cache, shared by q4_cache.cu and q4_attention.cu.
 #pragma once
 
+#include <cstring>
+
 #include "common.cuh"
 
 struct Q4CacheDev {
@@ -33,25 +35,40 @@ inline bool q4_vec(const Q4Tensor& x, size_t el) {
   return reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.sb * el) % 16 == 0 && (x.st * el) % 16 == 0 &&
          (x.sh * el) % 16 == 0;
 }
+// eight values as they lie in memory
+template <typename T>
+struct Q4Raw8 {
+  uint4 w[sizeof(T) / 2] = {};
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      T e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = p[j];
+      memcpy(w, e, sizeof(w));
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t x = (&w[0].x)[j];
+        v[2 * j] = __uint_as_float(x << 16);
+        v[2 * j + 1] = __uint_as_float(x & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float((&w[j / 4].x)[j % 4]);
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void q4_load8(float (&v)[8], const T* p, bool vec) {
-  if (!vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(p[j]);
-    return;
-  }
-  if constexpr (sizeof(T) == 2) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = (&r.x)[j];
-      v[2 * j] = __uint_as_float(w << 16);
-      v[2 * j + 1] = __uint_as_float(w & 0xFFFF0000u);
-    }
-  } else {
-    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-    *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
-  }
+  Q4Raw8<T> r;
+  r.load(p, vec);
+  r.get(v);
 }
 
 // row b's length and its new tokens; false when they lie outside the page table's positions or T
