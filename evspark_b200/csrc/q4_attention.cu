@@ -6,7 +6,8 @@
 // folded in order, and a second kernel folds the CTAs' partial results in order.  The unit's length
 // depends on the row's own position alone (32 keys below 1,024, 64 below 4,096, 256 below 131,072, else
 // 1,024), so a token's result does not depend on what else is in the call: verify blocks and single
-// steps agree bit for bit.  Short units give few keys to many CTAs; from 131,072 keys on there are
+// steps agree bit for bit.  (Calls of more than 64 rows a kv head leave positions from 4,096 on to
+// q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give few keys to many CTAs; from 131,072 keys on there are
 // enough of them, and longer ones spare partial results (440 us instead of 479 at 262,144 keys).
 //
 // Keys and values are decoded in the registers that the products read them from, with no rounding
@@ -20,7 +21,7 @@
 
 #include "internal.hpp"
 #include "q4.cuh"
-#include "q4_cache.hpp"
+#include "q4_attention.hpp"
 
 namespace {
 
@@ -30,29 +31,6 @@ constexpr int QA_ROWS = 16;
 constexpr int QA_CLUSTER = 8;  // slots that one cluster folds: contexts of up to 2,048 keys
 constexpr int NS = 2;           // 16-key chunks per online-softmax step of a warp
 constexpr int QA_STEP = 16 * NS;
-// A row's sums are taken relative to 2^m; m moves up only when a score passes it by more than this (in
-// powers of two), as moving it costs a product per output. Sums in fp32 and probabilities in bf16 keep
-// their relative accuracy below 2^8.
-constexpr float QA_SLACK = 8.f;
-
-// length class of a position, and keys per CTA of a class
-__host__ __device__ constexpr int qa_class(int64_t pos) {
-  return pos < 1024 ? 0 : (pos < 4096 ? 1 : (pos < 131072 ? 2 : 3));
-}
-__host__ __device__ constexpr int64_t qa_class_end(int cl) {
-  return cl == 0 ? 1024 : (cl == 1 ? 4096 : (cl == 2 ? 131072 : (1ll << 40)));
-}
-__host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 4096)); }
-// partial results of one row for lengths up to bound
-inline int qa_slots(int64_t bound) {
-  int n = 1;
-  for (int cl = 0; cl < 4; ++cl) {
-    const int64_t end = std::min(bound, qa_class_end(cl));
-    n = std::max<int64_t>(n, (end + qa_cta_keys(cl) - 1) / qa_cta_keys(cl));
-    if (bound <= qa_class_end(cl)) break;
-  }
-  return n;
-}
 
 template <int NW>
 __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
@@ -65,17 +43,6 @@ __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
   } else {
     w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
   }
-}
-
-// whether one of the bf16 scales of a pair is NaN (scales are at most 2^120: only a NaN's exponent
-// carries into the sign bit)
-__device__ __forceinline__ uint32_t scales_nan(uint32_t s2) { return (s2 + 0x00800080u) & 0x80008000u; }
-
-// 2^x to two units in the last place, 0 below 2^-126
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 constexpr int qa_parts_q(size_t elem) { return elem == 2 ? 1 : 3; }  // bf16 parts of a query value
@@ -107,11 +74,11 @@ __host__ __device__ constexpr int qa_q_floats() {
 }
 
 // One CTA's keys for one tile of 16 rows.  FUSED: each row's result stays in shared memory (fin), else it
-// goes to the CTA's slot of the workspace.
+// goes to the CTA's slot of the workspace.  Classes above top are another kernel's.
 template <typename T, int DH, bool FUSED>
 __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache, const Q4RowsDev& rows, const Q4Tensor& q,
                                           int grp, int t0, int tc, int tiles, float scale_log2, int nslots, bool q_vec,
-                                          float* __restrict__ part_o, float2* __restrict__ part_s) {
+                                          int top, float* __restrict__ part_o, float2* __restrict__ part_s) {
   constexpr int NQ = qa_parts_q(sizeof(T)), NP = qa_parts_p(sizeof(T));
   constexpr int KW = DH / 32;  // code words per thread and key (K)
   constexpr int VN = DH / 8;   // 8-feature tiles of the output
@@ -126,8 +93,8 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
   const int last = min(min(t0 + (tile * QA_ROWS + QA_ROWS - 1) / grp, t0 + tc - 1), count - 1);
   if (first > last) return;
   const int pmin = len + first, pmax = len + last;
-  const int cl0 = qa_class(pmin), cl1 = qa_class(pmax);
-  if (static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl0) > pmax) return;
+  const int cl0 = qa_class(pmin), cl1 = min(qa_class(pmax), top);
+  if (cl1 < cl0 || static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl0) > pmax) return;
 
   // Queries as product operands: step 2 w covers the feature pairs (0,4) (1,5) of the word 8 w ..,
   // step 2 w + 1 the pairs (2,6) (3,7), as q4_word decodes the keys; qs[part][step][lane].
@@ -335,7 +302,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
         const float grow = (mx[i] - m[i]) * scale_log2;  // NaN while nothing is visible
         if (grow > QA_SLACK) {
           moved = true;
-          a[i] = ex2(-grow);
+          a[i] = qa_ex2(-grow);
           m[i] = mx[i];
         }
       }
@@ -361,8 +328,8 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float p0 = ex2(fmaf(s[sub][u][2 * i], scale_log2, mu[i]));
-            const float p1 = ex2(fmaf(s[sub][u][2 * i + 1], scale_log2, mu[i]));
+            const float p0 = qa_ex2(fmaf(s[sub][u][2 * i], scale_log2, mu[i]));
+            const float p1 = qa_ex2(fmaf(s[sub][u][2 * i + 1], scale_log2, mu[i]));
             l[i] += p0 + p1;
             float r0 = p0, r1 = p1;
 #pragma unroll
@@ -384,7 +351,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
           if (k4 + 2 >= kend) vs[1] &= 0xFFFF0000u;
           if (k4 + 3 >= kend) vs[1] &= 0x0000FFFFu;
         }
-        const uint32_t nan0 = scales_nan(vs[0]), nan1 = scales_nan(vs[1]);
+        const uint32_t nan0 = qa_scales_nan(vs[0]), nan1 = qa_scales_nan(vs[1]);
         if (__any_sync(0xffffffffu, (nan0 | nan1) != 0u)) {
           // a group held as NaN must not reach rows that do not see its key (0 NaN is NaN): take it
           // out of the product and set the outputs of the rows that see it
@@ -460,7 +427,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
       float sum = 0.f, f[QA_WARPS];
 #pragma unroll
       for (int w = 0; w < QA_WARPS; ++w) {
-        f[w] = mw[w] == -CUDART_INF_F ? 0.f : ex2(mw[w] - big);
+        f[w] = mw[w] == -CUDART_INF_F ? 0.f : qa_ex2(mw[w] - big);
         sum = fmaf(res[(w * QA_ROWS + r) * LD + DH + 1], f[w], sum);
       }
       float* dst_o;
@@ -503,11 +470,11 @@ __device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDe
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
     q4_attn_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, int grp, int t0, int tc, int tiles, float scale_log2,
-                   int nslots, int q_vec, float* __restrict__ part_o, float2* __restrict__ part_s) {
+                   int nslots, int q_vec, int top, float* __restrict__ part_o, float2* __restrict__ part_s) {
   pdl_trigger();
   extern __shared__ __align__(16) float qa_sm[];  // the queries, then [warp][16][DH + 2] results
   pdl_wait();
-  attn_tile<T, DH, false>(qa_sm, cache, rows, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec != 0, part_o, part_s);
+  attn_tile<T, DH, false>(qa_sm, cache, rows, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec != 0, top, part_o, part_s);
 }
 
 // Short contexts: the CTAs of a tile are one cluster and fold their results through its shared memory,
@@ -520,8 +487,8 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
   extern __shared__ __align__(16) float qa_sm[];  // the queries, [warp][16][DH + 2] results, [16][DH + 2] folded
   pdl_wait();
   const int nslots = gridDim.x;
-  attn_tile<T, DH, true>(qa_sm, cache, rows, q, grp, 0, rows.T, tiles, scale_log2, nslots, q_vec != 0, nullptr,
-                         nullptr);
+  attn_tile<T, DH, true>(qa_sm, cache, rows, q, grp, 0, rows.T, tiles, scale_log2, nslots, q_vec != 0, 3,
+                         nullptr, nullptr);
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
@@ -556,7 +523,7 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
       for (int x = w; x < QA_CLUSTER; x += QA_WARPS)
         if (x < n) {
-          const float f = mx[x] == -CUDART_INF_F ? 0.f : ex2(mx[x] - big);
+          const float f = mx[x] == -CUDART_INF_F ? 0.f : qa_ex2(mx[x] - big);
           ps = fmaf(sm[x], f, ps);
 #pragma unroll
           for (int d = 0; d < DH / 32; ++d) part[d] = fmaf(v[x][d], f, part[d]);
@@ -596,7 +563,7 @@ __global__ void __launch_bounds__(QA_THREADS)
 #pragma unroll 8
   for (int x = warp; x < n; x += QA_WARPS) {
     const float2 st = part_s[prow + x];
-    const float f = st.x == -CUDART_INF_F ? 0.f : ex2(st.x - big);
+    const float f = st.x == -CUDART_INF_F ? 0.f : qa_ex2(st.x - big);
     sum = fmaf(st.y, f, sum);
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) acc[d] = fmaf(part_o[(prow + x) * DH + 32 * d + lane], f, acc[d]);
@@ -654,6 +621,11 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   const int smem = (qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2)) * 4;
   static std::atomic<unsigned long long> done{0};
   EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
+  // From 65 rows a kv head on the tensor-core kernel takes the long positions: it wins from 39 rows on (151 us
+  // instead of 183 at 32,768 keys, 32 kv heads; 26 rows: 257 instead of 242), but blocks of up to 64 tokens
+  // keep the sums of single steps.
+  const bool tcore = sizeof(T) == 2 && DH == 128 && static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS &&
+                     bound > qa_class_end(QA_TC_CLASS - 1);
   // tokens per pass: as many as the workspace holds partial results for
   const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
   const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles
@@ -664,13 +636,16 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
     const int prows = static_cast<int>(padded_rows(static_cast<int64_t>(tc) * grp)), tiles = prows / QA_ROWS;
     float* po = ws;
     float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * prows * nslots * DH);
-    EVS_CUDA_TRY(evs_launch(kern, dim3(nslots, c.G * tiles, r.B), dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc,
-                            tiles, scale_log2, nslots, q_vec, po, ps));
+    EVS_CUDA_TRY(evs_launch(kern, dim3(tcore ? qa_slots(qa_class_end(QA_TC_CLASS - 1)) : nslots, c.G * tiles, r.B),
+                            dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec,
+                            tcore ? QA_TC_CLASS - 1 : 3, po, ps));
+    evs_count_launch(1);
+    if (tcore) EVS_TRY(launch_q4_attn_tc(c, r, q, grp, t0, tc, prows, scale_log2, nslots, q_vec, po, ps, st, true));
     // the combine may start while the last tiles run (it waits for them before it reads)
     EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3(tc * grp, c.G, r.B), dim3(QA_THREADS), 0, st, true, c, r,
                             out, grp, t0, prows, nslots,
                             static_cast<const float*>(po), static_cast<const float2*>(ps)));
-    evs_count_launch(2);
+    evs_count_launch(1);
   }
   return EVS_OK;
 }

@@ -402,3 +402,101 @@ def test_large_pool_offsets(q4):
     a, b = (q4.q4_kv_read(cache, t, i32([0]), 130) for t in (far, near))
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     cache.check()
+
+
+# positions from 4,096 on, more than 64 rows a kv head, bf16 queries, heads of 128: the tcgen05 kernel
+LONG = [  # starts, T, counts, H, G, page
+    ([4096], 65, None, 1, 1, 64),
+    ([4090], 13, None, 12, 2, 16),
+    ([5000, 100, 4095, 7000, 0], 70, [70, 4, 2, 0, 1], 4, 4, 48),
+    ([6143, 4223, 4200], 9, [9, 1, 8], 8, 1, 128),
+    ([8191, 5119], 21, [21, 20], 28, 2, 32),
+    ([4500], 130, None, 2, 1, 64),
+    ([131070], 33, None, 2, 1, 4096),
+]
+
+
+@pytest.mark.parametrize("starts,T,counts,H,G,page", LONG)
+def test_attention_long(q4, starts, T, counts, H, G, page):
+    test_attention(q4, starts, T, counts, H, G, 128, page, BF)
+
+
+@pytest.mark.parametrize("start,T,H,G", [(4088, 13, 2, 2), (7000, 13, 8, 2), (4090, 64, 1, 1)])
+def test_attention_long_blocks_equal_steps(q4, start, T, H, G):
+    test_attention_bits_depend_on_the_token_alone(q4, start, T, H, G, 128, BF)
+
+
+@pytest.mark.parametrize("start,T,H,G", [(4088, 40, 4, 2), (7000, 13, 16, 2), (131066, 12, 8, 1)])
+def test_attention_long_bits_depend_on_the_token_alone(q4, start, T, H, G):
+    """Other rows, other blocks, a padded batch, another page size, bound and strides give the same bits."""
+    D, end = 128, start + T
+    cache, table = make_rows(q4, [end, end, 4100], 64, G, D)
+    k, v = randn(3, end, G, D, seed=1, dtype=BF), randn(3, end, G, D, seed=2, dtype=BF)
+    k[1], v[1] = k[0], v[0]
+    q4.q4_kv_append(cache, table, i32([0, 0, 0]), k, v, counts=i32([end, end, 4100]))
+    q = randn(3, T, H, D, seed=3, dtype=BF) * 2
+    q[1] = q[0]
+    block = q4.q4_attention(q, cache, table, i32([start, start, 4090]), counts=i32([T, T, 5]))
+    assert torch.equal(block[0], block[1])
+    alone = q4.q4_attention(q[:1], cache, table[:1], i32([start]), max_length=end)
+    assert torch.equal(alone[0], block[0])
+    # the same token at another place of a block, behind more padding
+    rows = 65 * G // H + 1  # more than 64 rows a kv head
+    for first in (1, T // 2):
+        part = torch.zeros(1, max(rows, T + 7), H, D, dtype=BF, device=DEV)
+        part[0, :T - first] = q[0, first:]
+        got = q4.q4_attention(part, cache, table[:1], i32([start + first]), counts=i32([T - first]))
+        assert torch.equal(got[0, :T - first], block[0, first:]), first
+    other, ot = make_rows(q4, [end], 16, G, D, seed=5)
+    q4.q4_kv_append(other, ot, i32([0]), k[:1], v[:1])
+    wide = torch.zeros(1, T, H, D + 3, dtype=BF, device=DEV)
+    wide[..., 1:D + 1] = q[0]
+    assert torch.equal(q4.q4_attention(wide[..., 1:D + 1], other, ot, i32([start]))[0], block[0])
+    cache.check()
+
+
+def test_attention_long_unaligned_queries_and_growing_scores(q4):
+    """Queries that cannot be read as words, and keys that grow along the row: the reference of the sums moves."""
+    D, G, H, T, start = 128, 1, 3, 25, 4600
+    cache, table = make_rows(q4, [start + T], 32, G, D)
+    k, v = randn(1, start + T, G, D, seed=1, dtype=BF), randn(1, start + T, G, D, seed=2, dtype=BF)
+    k *= torch.linspace(0.01, 6, start + T, device=DEV)[None, :, None, None].to(BF)
+    q4.q4_kv_append(cache, table, i32([0]), k, v)
+    kk, vv = q4.q4_kv_read(cache, table, i32([0]), start + T)
+    wide = randn(1, T, H, D + 3, seed=3, dtype=BF)
+    q = wide[..., 1:D + 1]
+    out = q4.q4_attention(q, cache, table, i32([start]))
+    want, av, mag = R.attend(q[0], kk[0].double(), vv[0].double(), start, D ** -0.5)
+    assert bool(((out[0].double() - want).abs() <= R.attend_bound(want, av, mag, start + T, D, BF)).all())
+    assert torch.equal(out, q4.q4_attention(q.contiguous(), cache, table, i32([start])))
+
+
+def test_attention_long_nan_groups_and_bad_pages(q4):
+    D, G, H, T, start = 128, 2, 24, 7, 4400
+    cache, table = make_rows(q4, [start + T, start + T], 16, G, D)
+    k, v = randn(2, start + T, G, D, seed=1, dtype=BF), randn(2, start + T, G, D, seed=2, dtype=BF)
+    q4.q4_kv_append(cache, table, i32([0, 0]), k, v)
+    q = randn(2, T, H, D, seed=3, dtype=BF)
+    clean = q4.q4_attention(q, cache, table, i32([start, start]))
+    cache.check()
+    vb, kb = v.clone(), k.clone()
+    vb[0, start + 2, 0, 70] = math.nan  # the token at start + 2, third group of features of kv head 0
+    kb[0, start + 5, 1, 1] = math.inf  # ... at start + 5, kv head 1
+    q4.q4_kv_append(cache, table, i32([0, 0]), kb, vb)
+    got = q4.q4_attention(q, cache, table, i32([start, start]))
+    assert torch.equal(got[1], clean[1]) and torch.equal(got[0, :2], clean[0, :2])
+    assert bool(got[0, 2:, :12, 64:96].isnan().all())
+    keep = [i for i in range(D) if not 64 <= i < 96]
+    assert torch.equal(got[0, 2:, :12][..., keep], clean[0, 2:, :12][..., keep])
+    assert torch.equal(got[0, :5, 12:], clean[0, :5, 12:]) and bool(got[0, 5:, 12:].isnan().all())
+    q4.q4_kv_append(cache, table, i32([0, 0]), k, v)
+    bad = table.clone()
+    bad[0, 200] = cache.num_pages
+    got = q4.q4_attention(q, cache, bad, i32([start, start]))
+    assert bool(got[0].isnan().all()) and torch.equal(got[1], clean[1])
+    with pytest.raises(RuntimeError):
+        cache.check()
+    got = q4.q4_attention(q, cache, table, i32([start, -3]))
+    assert torch.equal(got[0], clean[0]) and bool(got[1].isnan().all())
+    with pytest.raises(RuntimeError):
+        cache.check()
