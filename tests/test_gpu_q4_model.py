@@ -175,6 +175,17 @@ def test_bf16_speculative_equals_native(cuda):
         assert es.generate(prompt, n_tokens=32, seed=5).ids.shape == (32,)
 
 
+def test_bf16_speculative_equals_native_behind_a_long_prompt(cuda):
+    """A prompt whose long chunks take the tensor-core attention: blocks and steps behind it still agree."""
+    from evspark_b200.api import EvSpark
+
+    prompt = "".join(np.random.default_rng(4).choice(list("ACGT"), size=4500))
+    with EvSpark.load(ckpt=None, model_name="evo2_7b_slice", kv_format="q4", max_chunk=1024) as es:
+        spec = es.generate(prompt, n_tokens=24, greedy=True)
+        native = es.generate_native(prompt, n_tokens=24, greedy=True)
+        assert spec.ids.tolist() == native.ids.tolist()
+
+
 def test_streams_equal_single_streams(tiny):
     from evspark_b200.specdec.block import prefill
 
