@@ -760,12 +760,17 @@ int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 attention: q must be fp32 or bf16");
   EVS_CHECK_ARG(n_heads >= cache->kv_heads && n_heads % cache->kv_heads == 0,
                 "q4 attention: n_heads must be a multiple of kv_heads");
-  EVS_CHECK_ARG(scale > 0.f && std::isfinite(scale), "q4 attention: scale must be positive");
+  EVS_CHECK_ARG(scale > 0.f && scale <= 1e38f, "q4 attention: scale must be positive and at most 1e38");
   EVS_CHECK_ARG(max_length >= 0, "q4 attention: max_length must not be negative");
   EVS_CHECK_ARG(cache->kv_heads <= 65535 && rows->batch <= 65535, "q4 attention: too many heads or rows");
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "q4 attention: the workspace must be 16-byte aligned");
   const Q4Tensor tq{const_cast<void*>(q), q_strides[0], q_strides[1], q_strides[2]};
   const Q4Tensor to{out, out_strides[0], out_strides[1], out_strides[2]};
+  const int B = rows->batch, T = rows->tokens, D = cache->head_dim;
+  const bool in_place = q == out && tq.sb == to.sb && tq.st == to.st && tq.sh == to.sh;
+  EVS_CHECK_ARG(q4_distinct(to, B, T, n_heads, D), "q4 attention: elements of out overlap");
+  EVS_CHECK_ARG(in_place || !q4_share(to, n_heads, tq, n_heads, B, T, D, dtype == EVS_DTYPE_BF16 ? 2 : 4),
+                "q4 attention: out overlaps q");
   return launch_q4_attention(q4_cache_dev(cache), q4_rows_dev(rows), tq, to, n_heads, scale,
                              bound_of(cache, rows, max_length), workspace, workspace_bytes, dtype, st, false);
 }

@@ -300,6 +300,38 @@ __global__ void __launch_bounds__(APP_THREADS)
 
 }  // namespace
 
+bool q4_distinct(const Q4Tensor& x, int B, int T, int heads, int D) {
+  struct {
+    int64_t stride, n;
+  } dim[3] = {{x.sb, B}, {x.st, T}, {x.sh, heads}};
+  std::sort(dim, dim + 3, [](const auto& a, const auto& b) { return a.stride < b.stride; });
+  int64_t least = D;
+  for (const auto& d : dim) {
+    if (d.n <= 1) continue;
+    if (d.stride < least) return false;
+    least = d.stride * d.n;
+  }
+  return true;
+}
+
+bool q4_share(const Q4Tensor& x, int x_heads, const Q4Tensor& y, int y_heads, int B, int T, int D, size_t el) {
+  const int64_t e = static_cast<int64_t>(el), px = reinterpret_cast<intptr_t>(x.p), py = reinterpret_cast<intptr_t>(y.p);
+  auto reach = [&](const Q4Tensor& t, int heads, int64_t p, int64_t* lo, int64_t* hi) {
+    *lo = p, *hi = p + D * e;
+    const int64_t last[3] = {(B - 1) * t.sb * e, (T - 1) * t.st * e, (heads - 1) * t.sh * e};
+    for (int64_t d : last) (d < 0 ? *lo : *hi) += d;
+  };
+  int64_t x0, x1, y0, y1;
+  reach(x, x_heads, px, &x0, &x1);
+  reach(y, y_heads, py, &y0, &y1);
+  if (x1 <= y0 || y1 <= x0) return false;
+  if (x.st != y.st || x.st <= 0 || (B > 1 && (x.sb != y.sb || x.sb % x.st != 0)) || (py - px) % e != 0 || x.sh < 0 ||
+      y.sh < 0)
+    return true;
+  const int64_t column = ((py - px) / e % x.st + x.st) % x.st;  // of y's rows, from x's on
+  return column < (x_heads - 1) * x.sh + D || column + (y_heads - 1) * y.sh + D > x.st;
+}
+
 int q4_check_cache(const evs_q4_cache* c) {
   EVS_CHECK_ARG(c != nullptr && c->pool != nullptr, "null argument");
   EVS_CHECK_ARG(c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128, "q4 cache: head_dim must be 32, 64 or 128");
@@ -394,6 +426,15 @@ int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG(rope_base > 0.0 && std::isfinite(rope_base), "q4 append: rope_base must be positive");
   const Q4Tensor tk = tensor_of(k, k_strides), tv = tensor_of(v, v_strides);
   const Q4Tensor tq = q != nullptr ? tensor_of(q, q_strides) : tk, to = q != nullptr ? tensor_of(q_out, q_out_strides) : tk;
+  if (q != nullptr) {
+    const int B = rows->batch, T = rows->tokens, G = cache->kv_heads, D = cache->head_dim;
+    const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
+    const bool in_place = q == q_out && tq.sb == to.sb && tq.st == to.st && tq.sh == to.sh;
+    EVS_CHECK_ARG(q4_distinct(to, B, T, n_heads, D), "q4 append: elements of q_out overlap");
+    EVS_CHECK_ARG((in_place || !q4_share(to, n_heads, tq, n_heads, B, T, D, el)) &&
+                      !q4_share(to, n_heads, tk, G, B, T, D, el) && !q4_share(to, n_heads, tv, G, B, T, D, el),
+                  "q4 append: q_out overlaps another tensor of the call");
+  }
   return launch_q4_append(q4_cache_dev(cache), q4_rows_dev(rows), tq, tk, tv, to, q != nullptr ? n_heads : 0, dtype,
                           rope_base, st, false);
 }
@@ -404,8 +445,12 @@ int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, 
   EVS_TRY(q4_check_rows(cache, rows));
   EVS_CHECK_ARG(k && v && k_strides && v_strides, "null argument");
   EVS_CHECK_ARG(dtype == EVS_DTYPE_BF16 || dtype == EVS_DTYPE_FP32, "q4 read: k and v must be fp32 or bf16");
-  return launch_q4_read(q4_cache_dev(cache), q4_rows_dev(rows), tensor_of(k, k_strides), tensor_of(v, v_strides), dtype,
-                        st);
+  const Q4Tensor tk = tensor_of(k, k_strides), tv = tensor_of(v, v_strides);
+  const int B = rows->batch, T = rows->tokens, G = cache->kv_heads, D = cache->head_dim;
+  EVS_CHECK_ARG(q4_distinct(tk, B, T, G, D) && q4_distinct(tv, B, T, G, D) &&
+                    !q4_share(tk, G, tv, G, B, T, D, dtype == EVS_DTYPE_BF16 ? 2 : 4),
+                "q4 read: elements of k and v overlap");
+  return launch_q4_read(q4_cache_dev(cache), q4_rows_dev(rows), tk, tv, dtype, st);
 }
 
 }  // extern "C"

@@ -85,6 +85,11 @@ __device__ __forceinline__ int64_t q4_page(const Q4CacheDev& c, const Q4RowsDev&
   return id >= 0 && id < c.pages ? id : -1;
 }
 
+// Outputs [B, T, heads, D] (D contiguous): whether their elements are distinct, and whether two tensors may share
+// one: their spans in memory meet, and they are not separate columns of rows of one stride (as q, k and v of a
+// fused projection are).
+bool q4_distinct(const Q4Tensor& x, int B, int T, int heads, int D);
+bool q4_share(const Q4Tensor& x, int x_heads, const Q4Tensor& y, int y_heads, int B, int T, int D, size_t el);
 int q4_check_cache(const evs_q4_cache* c);
 int q4_check_rows(const evs_q4_cache* c, const evs_q4_rows* r);
 Q4CacheDev q4_cache_dev(const evs_q4_cache* c);

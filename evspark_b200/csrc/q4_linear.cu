@@ -443,6 +443,8 @@ int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* co
   const size_t xa = x_dtype == EVS_DTYPE_BF16 ? 2 : 4, oa = out_dtype == EVS_DTYPE_BF16 ? 2 : 4;
   EVS_CHECK_ARG(reinterpret_cast<uintptr_t>(x) % xa == 0 && reinterpret_cast<uintptr_t>(out) % oa == 0,
                 "q4 linear: misaligned pointer");
+  const char *x0 = static_cast<const char*>(x), *o0 = static_cast<const char*>(out);
+  EVS_CHECK_ARG(x0 + ((M - 1) * ldx + K) * xa <= o0 || o0 + ((M - 1) * ldo + N) * oa <= x0, "q4 linear: out overlaps x");
   return launch_q4_linear(x, x_dtype, ldx, M, codes, scales, N, K, group, out, out_dtype, ldo, st, false);
 }
 

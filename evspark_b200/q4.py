@@ -351,8 +351,11 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
     bound of lengths + counts, keeps the launch small; without it the page table's size bounds it.
     Returns [B, T, heads, D] in q's dtype, or fills ``out`` (padding behind counts[b] is left unwritten).
 
+    ``out`` may be q.
+
     A token's result depends only on its position, its q and the keys it sees, bit for bit: not on the
-    batch, the other tokens of the call, max_length or the page size."""
+    batch, the other tokens of the call, max_length or the page size.  One size matters: bf16 calls of more
+    than 64 rows (T * heads / kv_heads, D = 128) sum in another order from position 4,096 on."""
     if q.dim() != 4:
         raise ValueError(f"q4_attention: q must be [B, T, heads, D], got {tuple(q.shape)}")
     B, T, H, _ = q.shape
@@ -363,8 +366,8 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
     qs = _heads(q, shape, q.dtype, index, "q4_attention: q")
     if scale is None:
         scale = cache.head_dim ** -0.5
-    elif not 0.0 < scale < float("inf"):
-        raise ValueError(f"q4_attention: scale must be positive and finite, got {scale}")
+    elif not 0.0 < scale <= 1e38:
+        raise ValueError(f"q4_attention: scale must be positive and at most 1e38, got {scale}")
     if max_length is not None and not 1 <= max_length < 2 ** 31:
         raise ValueError(f"q4_attention: max_length must be positive, got {max_length}")
     rows, positions = _rows(cache, page_table, lengths, counts, B, T, "q4_attention")
@@ -374,7 +377,7 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
     if B == 0 or T == 0:
         return out
     ml = 0 if max_length is None else max_length
-    sizes = (B, T, H, ml or positions)
+    sizes = (B, T, H, min(ml, positions) if ml else positions)
     need = cache._workspace.get(sizes)
     if need is None:
         need = N.lib().evs_q4_attention_workspace(cache._ref, rows, H, ml)

@@ -237,7 +237,8 @@ EVS_API int evs_q4_quantize(const void* w, int dtype, int64_t ldw, int N, int K,
 EVS_API int evs_q4_dequantize(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
                               int64_t ldo, cudaStream_t stream);
 /* out[m][n] = sum_k x[m][k] w[n][k], sums in fp32; x [M, K] and out [M, N] fp32 or bf16, row strides
- * ldx and ldo in elements.  A row of out does not depend on M or on the other rows of x. */
+ * ldx and ldo in elements; out must not overlap x.  A row of out does not depend on M or on the other
+ * rows of x. */
 EVS_API int evs_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N,
                           int K, int group, void* out, int out_dtype, int64_t ldo, cudaStream_t stream);
 
@@ -265,9 +266,9 @@ typedef struct evs_q4_rows {
   int32_t max_pages, batch, tokens;
 } evs_q4_rows;
 /* Rotates k (rotate-half, angle position * rope_base^(-2 j / D)) and stores k and v; with q != NULL
- * also q_out = rotated q.  Tensors [batch, tokens, heads, D] of one dtype (fp32 or bf16), strides in
- * elements for the first three dimensions, D contiguous.  Two rows that append to the same slot of
- * the same page in one call race. */
+ * also q_out = rotated q (q_out may be q itself, and overlaps no other tensor).  Tensors [batch, tokens,
+ * heads, D] of one dtype (fp32 or bf16), strides in elements for the first three dimensions, D
+ * contiguous.  Two rows that append to the same slot of the same page in one call race. */
 EVS_API int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const void* k, const int64_t* k_strides,
                              const void* v, const int64_t* v_strides, const void* q, const int64_t* q_strides,
                              void* q_out, const int64_t* q_out_strides, int n_heads, int dtype, double rope_base,
@@ -278,9 +279,9 @@ EVS_API int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, v
 /* Causal attention of the new tokens over the cache (they are appended already): token t of row b
  * sees positions 0 .. lengths[b] + t.  q and out [batch, tokens, n_heads, D] (fp32 or bf16, out of
  * q's dtype), already rotated; n_heads a multiple of kv_heads (query head h reads kv head
- * h / (n_heads / kv_heads)).  max_length >= max(lengths + counts) bounds the launch (0: the whole
- * table).  scale must be positive.  workspace: device scratch of at least evs_q4_attention_workspace
- * bytes (0 for short contexts, -1 for arguments that are refused), one per call in flight.  A token's
+ * h / (n_heads / kv_heads)); out may be q itself but must not overlap it otherwise.  max_length >=
+ * max(lengths + counts) bounds the launch (0: the whole table).  scale must be positive, at most 1e38.
+ * workspace: device scratch of at least evs_q4_attention_workspace bytes (0 for short contexts, -1 for arguments that are refused), one per call in flight.  A token's
  * result depends on its position, its q and the keys it sees alone: not on the batch, the other tokens,
  * max_length, the page size or the workspace. One size matters: from position 4,096 on, calls of more
  * than 64 rows (tokens * n_heads / kv_heads; bf16, D = 128) sum in another order than smaller ones. */

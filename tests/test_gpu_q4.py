@@ -500,3 +500,55 @@ def test_attention_long_nan_groups_and_bad_pages(q4):
     assert torch.equal(got[0], clean[0]) and bool(got[1].isnan().all())
     with pytest.raises(RuntimeError):
         cache.check()
+
+
+def test_outputs_that_overlap_are_refused(q4):
+    D, G, H, T, B = 64, 2, 4, 3, 2
+    cache, table = make_rows(q4, [40, 40], 16, G, D)
+    buf = randn(B, T, (H + 2 * G + 1) * D, seed=1, dtype=BF)
+    q, k, v = (buf[..., a * D:b * D].unflatten(-1, (-1, D)) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
+    at = i32([5, 9])
+    pool = cache.pool.clone()
+    for bad in (buf[..., D:(H + 1) * D], buf[..., (H + G - 2) * D:(2 * H + G - 2) * D],
+                buf[0, 0, :H * D].clone().expand(B, T, H * D)):
+        with pytest.raises(ValueError, match="overlap"):
+            q4.q4_kv_append(cache, table, at, k, v, q=q, q_out=bad.unflatten(-1, (-1, D)))
+    assert torch.equal(pool, cache.pool)
+    # apart from each other: a column of the same buffer that no input holds, or q itself
+    want = q4.q4_kv_append(cache, table, at, k, v, q=q)
+    assert torch.equal(q4.q4_kv_append(cache, table, at, k, v, q=q, q_out=q), want) and torch.equal(q, want)
+    # attention in place equals the one into another tensor, on both launch paths
+    for room in (0, 300):
+        wide = torch.cat([table, torch.full((B, room), -1, dtype=torch.int32, device=DEV)], 1)
+        q4.q4_kv_append(cache, wide, i32([0, 0]), *(randn(B, 12, G, D, seed=s, dtype=BF) for s in (2, 3)))
+        ref = q4.q4_attention(want, cache, wide, at)
+        mine = want.clone()
+        assert torch.equal(q4.q4_attention(mine, cache, wide, at, out=mine), ref)
+    flat = randn(B * T * H * D + 64, seed=4, dtype=BF)
+    with pytest.raises(ValueError, match="overlap"):
+        q4.q4_attention(flat[:-64].view(B, T, H, D), cache, table, at, out=flat[64:].view(B, T, H, D))
+    with pytest.raises(ValueError, match="overlap"):
+        q4.q4_attention(want, cache, table, at, out=want[:, :1].clone().expand(B, T, H, D))
+    kk = torch.empty(B, T, G, D, dtype=BF, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        q4.q4_kv_read(cache, table, at, T, out=(kk, kk))
+    w = q4.quantize_weight(randn(128, 128, seed=5), 64)
+    x = randn(4, 128, seed=6)
+    with pytest.raises(ValueError, match="overlap"):
+        q4.q4_linear(x, w, out=x)
+    with pytest.raises(ValueError, match="scale"):
+        q4.q4_attention(want, cache, table, at, scale=2e38)
+
+
+def test_workspace_follows_the_table_not_the_bound_alone(q4):
+    """The same max_length with a short and then a long page table."""
+    D, G, end = 32, 1, 3000
+    cache, table = make_rows(q4, [end], 16, G, D)
+    k, v = randn(1, end, G, D, seed=1), randn(1, end, G, D, seed=2)
+    q4.q4_kv_append(cache, table, i32([0]), k, v)
+    q = randn(1, 2, G, D, seed=3)
+    want = q4.q4_attention(q, cache, table, i32([end - 2]))
+    fresh = q4.Q4Cache.from_pool(cache.pool, head_dim=D, page_size=16)
+    q4.q4_attention(q, fresh, table[:, :10].contiguous(), i32([100]), max_length=end)
+    assert torch.equal(q4.q4_attention(q, fresh, table, i32([end - 2]), max_length=end), want)
+    fresh.check()
