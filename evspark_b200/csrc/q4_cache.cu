@@ -300,16 +300,34 @@ __global__ void __launch_bounds__(APP_THREADS)
 
 }  // namespace
 
+namespace {
+struct Dim {
+  int64_t stride, x, y;  // sizes in the two tensors
+};
+// whether off = sum of t_k stride_k + r with -(y_k - 1) <= t_k <= x_k - 1 and |r| < D: an element of the first
+// tensor that is one of the second, off elements behind it.  dim: largest strides first.
+bool meet(int64_t off, const Dim* dim, int n, int D) {
+  if (n == 0) return off > -D && off < D;
+  int64_t low = -(D - 1), high = D - 1;  // of the dimensions behind this one
+  for (int i = 1; i < n; ++i) low -= (dim[i].y - 1) * dim[i].stride, high += (dim[i].x - 1) * dim[i].stride;
+  auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0 ? 1 : 0); };
+  const int64_t first = std::max(-(dim[0].y - 1), -floor_div(high - off, dim[0].stride));
+  const int64_t last = std::min(dim[0].x - 1, floor_div(off - low, dim[0].stride));
+  if (last - first >= 8) return true;  // interleaved beyond what is worth telling apart
+  for (int64_t t = first; t <= last; ++t)
+    if (meet(off - t * dim[0].stride, dim + 1, n - 1, D)) return true;
+  return false;
+}
+}  // namespace
+
 bool q4_distinct(const Q4Tensor& x, int B, int T, int heads, int D) {
-  struct {
-    int64_t stride, n;
-  } dim[3] = {{x.sb, B}, {x.st, T}, {x.sh, heads}};
-  std::sort(dim, dim + 3, [](const auto& a, const auto& b) { return a.stride < b.stride; });
+  Dim dim[3] = {{x.sb, B, 1}, {x.st, T, 1}, {x.sh, heads, 1}};
+  std::sort(dim, dim + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
   int64_t least = D;
-  for (const auto& d : dim) {
-    if (d.n <= 1) continue;
+  for (const Dim& d : dim) {
+    if (d.x <= 1) continue;
     if (d.stride < least) return false;
-    least = d.stride * d.n;
+    least = d.stride * d.x;
   }
   return true;
 }
@@ -325,11 +343,19 @@ bool q4_share(const Q4Tensor& x, int x_heads, const Q4Tensor& y, int y_heads, in
   reach(x, x_heads, px, &x0, &x1);
   reach(y, y_heads, py, &y0, &y1);
   if (x1 <= y0 || y1 <= x0) return false;
-  if (x.st != y.st || x.st <= 0 || (B > 1 && (x.sb != y.sb || x.sb % x.st != 0)) || (py - px) % e != 0 || x.sh < 0 ||
-      y.sh < 0)
-    return true;
-  const int64_t column = ((py - px) / e % x.st + x.st) % x.st;  // of y's rows, from x's on
-  return column < (x_heads - 1) * x.sh + D || column + (y_heads - 1) * y.sh + D > x.st;
+  // spans that meet: views of one buffer are told apart where their strides are the same
+  const int64_t all[3][4] = {{x.sb, y.sb, B, B}, {x.st, y.st, T, T}, {x.sh, y.sh, x_heads, y_heads}};
+  Dim dim[3];
+  int n = 0;
+  for (const auto& d : all) {
+    if (d[2] <= 1 && d[3] <= 1) continue;
+    if (d[2] > 1 && d[3] > 1 && d[0] != d[1]) return true;
+    dim[n++] = {d[2] > 1 ? d[0] : d[1], d[2], d[3]};
+    if (dim[n - 1].stride <= 0) return true;
+  }
+  if ((py - px) % e != 0) return true;
+  std::sort(dim, dim + n, [](const Dim& a, const Dim& b) { return a.stride > b.stride; });
+  return meet((py - px) / e, dim, n, D);
 }
 
 int q4_check_cache(const evs_q4_cache* c) {

@@ -85,9 +85,8 @@ __device__ __forceinline__ int64_t q4_page(const Q4CacheDev& c, const Q4RowsDev&
   return id >= 0 && id < c.pages ? id : -1;
 }
 
-// Outputs [B, T, heads, D] (D contiguous): whether their elements are distinct, and whether two tensors may share
-// one: their spans in memory meet, and they are not separate columns of rows of one stride (as q, k and v of a
-// fused projection are).
+// [B, T, heads, D] tensors (D contiguous): whether an output's elements are distinct, and whether two tensors may
+// share one (views of one buffer with the same strides, as q, k and v of a fused projection are, are told apart).
 bool q4_distinct(const Q4Tensor& x, int B, int T, int heads, int D);
 bool q4_share(const Q4Tensor& x, int x_heads, const Q4Tensor& y, int y_heads, int B, int T, int D, size_t el);
 int q4_check_cache(const evs_q4_cache* c);

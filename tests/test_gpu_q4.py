@@ -517,6 +517,12 @@ def test_outputs_that_overlap_are_refused(q4):
     # apart from each other: a column of the same buffer that no input holds, or q itself
     want = q4.q4_kv_append(cache, table, at, k, v, q=q)
     assert torch.equal(q4.q4_kv_append(cache, table, at, k, v, q=q, q_out=q), want) and torch.equal(q, want)
+    heads_first = torch.cat([t.transpose(1, 2) for t in (randn(B, T, H, D, seed=8, dtype=BF), k, v)], 1)
+    qt, kt, vt = (heads_first[:, a:b].transpose(1, 2) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
+    rotated = q4.q4_kv_append(cache, table, at, kt, vt, q=qt)
+    assert torch.equal(q4.q4_kv_append(cache, table, at, kt, vt, q=qt, q_out=qt), rotated)
+    with pytest.raises(ValueError, match="overlap"):
+        q4.q4_kv_append(cache, table, at, kt, vt, q=qt, q_out=heads_first[:, 1:H + 1].transpose(1, 2))
     # attention in place equals the one into another tensor, on both launch paths
     for room in (0, 300):
         wide = torch.cat([table, torch.full((B, room), -1, dtype=torch.int32, device=DEV)], 1)
