@@ -92,7 +92,7 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
 // Weight rows are the product's 16-row operand and tokens its 8-column one: a warp takes 32 rows x 128
 // features a step against every token of the tile, so the codes are decoded once, in the registers that
 // the product reads.  What bounds it is the decode's instructions and their latency: 420 warp
-// instructions per 4,096 codes (384 of them shifts, masks and fma of the decode), 0.44 issued a clock and
+// instructions per 4,096 codes (192 of them shifts, masks and fma of the decode), 0.44 issued a clock and
 // scheduler.  13 x 22016 x 4096, group 64: 20.4 us, 2.3 TB/s of codes and scales (floor 7.5 us at 6.5 TB/s);
 // 13 x 8192 x 22528: 34.8 us; 1 x 4096 x 4096: 6.1 us.
 // grid (K splits = cluster, row tiles, token tiles).  Registers hold the next two K blocks' codes

@@ -329,7 +329,7 @@ def q4_kv_read(cache: Q4Cache, page_table: torch.Tensor, starts: torch.Tensor, t
     if out is None:
         if dtype not in _DT:
             raise ValueError(f"q4_kv_read: dtype must be bf16 or fp32, got {dtype}")
-        out = tuple(torch.empty(shape, dtype=dtype, device=cache.pool.device) for _ in range(2))
+        out = tuple(cache.pool.new_empty(shape, dtype=dtype) for _ in range(2))
     k, v = out
     dt = _dtype(k, "q4_kv_read: k")
     ks = _heads(k, shape, k.dtype, index, "q4_kv_read: k")
@@ -386,7 +386,7 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
         cache._workspace[sizes] = need
     ws, wp = None, None
     if need > 0:
-        ws = torch.empty(need, dtype=torch.uint8, device=cache.pool.device)
+        ws = cache.pool.new_empty((need,))
         wp = ws.data_ptr()
     else:
         need = 0
