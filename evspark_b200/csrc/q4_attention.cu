@@ -454,13 +454,16 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
 // whether row b's token t is a token, and its position; a row that cannot be read (bad lengths, or beyond
 // the launch's slots) is set to NaN
 template <typename T, int DH>
-__device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDev& rows, int b, int t, int nslots, T* dst,
-                                         int* n) {
+__device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDev& rows, int b, int t, int nslots, bool tcore,
+                                         T* dst, int* n) {
   const int lane = threadIdx.x & 31;
   int len, count;
   const bool ok = q4_row(rows, b, &len, &count, cache.P);
   if (t >= (ok ? count : min(max(count, 0), rows.T))) return false;
-  if (ok) *n = static_cast<int>((static_cast<int64_t>(len) + t) / qa_cta_keys(qa_class(static_cast<int64_t>(len) + t))) + 1;
+  if (ok) {
+    const int pos = len + t;
+    *n = pos / (tcore && pos >= QA_TC_BEGIN ? qa_tc_keys(qa_tc_class(pos)) : qa_cta_keys(qa_class(pos))) + 1;
+  }
   if (ok && *n <= nslots) return true;
   for (int d = lane; d < DH; d += 32) dst[d] = from_f32<T>(CUDART_NAN_F);
   if (ok && lane == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_ATTN, b);
@@ -498,7 +501,7 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
     if (R >= rows.T * grp) break;
     T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
     int n;
-    if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) continue;
+    if (!fold_row<T, DH>(cache, rows, b, t, nslots, false, dst, &n)) continue;
     const uint32_t at = smem_u32(fin + r * (DH + 2));
     float v[QA_CLUSTER][DH / 32], mx[QA_CLUSTER], sm[QA_CLUSTER], big = -CUDART_INF_F;
 #pragma unroll
@@ -544,7 +547,7 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS)
     q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int prows, int nslots,
-                      const float* __restrict__ part_o, const float2* __restrict__ part_s) {
+                      int tcore, const float* __restrict__ part_o, const float2* __restrict__ part_s) {
   __shared__ float fold[QA_WARPS][DH + 1];
   pdl_trigger();
   pdl_wait();
@@ -552,7 +555,7 @@ __global__ void __launch_bounds__(QA_THREADS)
   const int t = t0 + R / grp;
   T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
   int n;
-  if (!fold_row<T, DH>(cache, rows, b, t, nslots, dst, &n)) return;  // the same for the whole CTA
+  if (!fold_row<T, DH>(cache, rows, b, t, nslots, tcore != 0, dst, &n)) return;  // the same for the whole CTA
   const size_t prow = ((static_cast<size_t>(b) * cache.G + kvh) * static_cast<size_t>(prows) + R) * nslots;
   float big = -CUDART_INF_F;
   for (int x = lane; x < n; x += 32) big = fmaxf(big, part_s[prow + x].x);
@@ -590,10 +593,11 @@ inline bool fused_fits(int nslots, int64_t T, int grp, int G) {
 template <typename T, int DH>
 int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& out, int H, float scale,
                 int64_t bound, float* ws, int64_t ws_floats, cudaStream_t st, bool pdl) {
-  const int grp = H / c.G, nslots = qa_slots(bound);
+  const int grp = H / c.G;
   const float scale_log2 = scale * 1.4426950408889634f;
   const int q_vec = q4_vec(q, sizeof(T));
-  if (fused_fits(nslots, r.T, grp, c.G)) {
+  if (fused_fits(qa_slots(bound), r.T, grp, c.G)) {
+    const int nslots = qa_slots(bound);
     auto* kern = q4_attn_fused_kernel<T, DH>;
     const int smem = (qa_q_floats<T, DH>() + (QA_WARPS + 1) * QA_ROWS * (DH + 2)) * 4;
     static std::atomic<unsigned long long> done{0};
@@ -625,7 +629,8 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   // instead of 183 at 32,768 keys, 32 kv heads; 26 rows: 257 instead of 242), but blocks of up to 64 tokens
   // keep the sums of single steps.
   const bool tcore = sizeof(T) == 2 && DH == 128 && static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS &&
-                     bound > qa_class_end(QA_TC_CLASS - 1);
+                     bound > QA_TC_BEGIN;
+  const int nslots = tcore ? qa_tc_slots(bound) : qa_slots(bound);
   // tokens per pass: as many as the workspace holds partial results for
   const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
   const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles
@@ -636,14 +641,14 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
     const int prows = static_cast<int>(padded_rows(static_cast<int64_t>(tc) * grp)), tiles = prows / QA_ROWS;
     float* po = ws;
     float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * prows * nslots * DH);
-    EVS_CUDA_TRY(evs_launch(kern, dim3(tcore ? qa_slots(qa_class_end(QA_TC_CLASS - 1)) : nslots, c.G * tiles, r.B),
+    EVS_CUDA_TRY(evs_launch(kern, dim3(tcore ? qa_slots(QA_TC_BEGIN) : nslots, c.G * tiles, r.B),
                             dim3(QA_THREADS), smem, st, pdl, c, r, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec,
-                            tcore ? QA_TC_CLASS - 1 : 3, po, ps));
+                            tcore ? qa_class(QA_TC_BEGIN - 1) : 3, po, ps));
     evs_count_launch(1);
     if (tcore) EVS_TRY(launch_q4_attn_tc(c, r, q, grp, t0, tc, prows, scale_log2, nslots, q_vec, po, ps, st, true));
     // the combine may start while the last tiles run (it waits for them before it reads)
     EVS_CUDA_TRY(evs_launch(q4_combine_kernel<T, DH>, dim3(tc * grp, c.G, r.B), dim3(QA_THREADS), 0, st, true, c, r,
-                            out, grp, t0, prows, nslots,
+                            out, grp, t0, prows, nslots, tcore ? 1 : 0,
                             static_cast<const float*>(po), static_cast<const float2*>(ps)));
     evs_count_launch(1);
   }

@@ -13,10 +13,19 @@ __host__ __device__ constexpr int64_t qa_class_end(int cl) {
   return cl == 0 ? 1024 : (cl == 1 ? 4096 : (cl == 2 ? 131072 : (1ll << 40)));
 }
 __host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 4096)); }
-// The classes from QA_TC_CLASS on are the tensor-core kernel's where the call has more than QA_FEW_ROWS rows
-// (tokens times query heads) a kv head.
-constexpr int QA_TC_CLASS = 2;
+// Positions from QA_TC_BEGIN on are the tensor-core kernel's where the call has more than QA_FEW_ROWS rows (tokens
+// times query heads) a kv head.  It has classes of its own, with a slot of keys per CTA: with 2,048 keys instead
+// of 1,024, 16 rows of 13 tokens at up to 16,384 keys take 220 us instead of 196, but 1,024 tokens behind 32,768
+// keys (64 / 8 heads) 2,076 instead of 2,640.
 constexpr int QA_FEW_ROWS = 64;
+constexpr int QA_TC_BEGIN = 4096;
+constexpr int QA_TC_CLASSES = 3;
+__host__ __device__ constexpr int qa_tc_class(int64_t pos) { return pos < 16384 ? 0 : (pos < 65536 ? 1 : 2); }
+__host__ __device__ constexpr int qa_tc_class_begin(int cl) { return cl == 0 ? QA_TC_BEGIN : (cl == 1 ? 16384 : 65536); }
+__host__ __device__ constexpr int64_t qa_tc_class_end(int cl) {
+  return cl == 0 ? 16384 : (cl == 1 ? 65536 : (1ll << 40));
+}
+__host__ __device__ constexpr int qa_tc_keys(int cl) { return cl == 0 ? 1024 : (cl == 1 ? 2048 : 4096); }
 // partial results of one row for lengths up to bound
 inline int qa_slots(int64_t bound) {
   int n = 1;
@@ -25,6 +34,13 @@ inline int qa_slots(int64_t bound) {
     n = std::max<int64_t>(n, (end + qa_cta_keys(cl) - 1) / qa_cta_keys(cl));
     if (bound <= qa_class_end(cl)) break;
   }
+  return n;
+}
+
+inline int qa_tc_slots(int64_t bound) {
+  int n = qa_slots(std::min<int64_t>(bound, QA_TC_BEGIN));
+  for (int cl = 0; cl < QA_TC_CLASSES && bound > qa_tc_class_begin(cl); ++cl)
+    n = std::max<int64_t>(n, (std::min(bound, qa_tc_class_end(cl)) + qa_tc_keys(cl) - 1) / qa_tc_keys(cl));
   return n;
 }
 
@@ -44,7 +60,7 @@ __device__ __forceinline__ float qa_ex2(float x) {
 // carries into the sign bit)
 __device__ __forceinline__ uint32_t qa_scales_nan(uint32_t s2) { return (s2 + 0x00800080u) & 0x80008000u; }
 
-// The classes from QA_TC_CLASS on, bf16 queries, head_dim 128: partial results of tc tokens from t0 on, prows
+// The positions from QA_TC_BEGIN on, bf16 queries, head_dim 128: partial results of tc tokens from t0 on, prows
 // rows a head in the workspace.
 int launch_q4_attn_tc(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, int grp, int t0, int tc, int prows,
                       float scale_log2, int nslots, int q_vec, float* part_o, float2* part_s, cudaStream_t st, bool pdl);

@@ -4,16 +4,18 @@
 //
 // One CTA takes up to 128 query rows (a row is one token of one query head of the kv head) over its slot of
 // keys, 64 keys a step: S = Q K^T (128 x 64 x 128) and O += P V (128 x 128 x 64).  Four warps decode keys and
-// values into shared memory once for all rows; one warp issues the products; four warps run the online
-// softmax, one row a thread, with S, then P in S's place, and O in tensor memory.  Two stages of everything,
-// so that a step's scores are there while the one before is still worked on; two CTAs an SM.
+// values into shared memory once for all rows; one warp issues whatever product is ready first; four warps run
+// the online softmax, one row a thread, with S, then P in S's place, and O in tensor memory.  Two stages of
+// everything, so that a step's scores are there while the one before is still worked on; two CTAs an SM.
 //
 // Measured beside the 16-row mma.sync kernel, which decodes the keys once per 16 rows: 16 rows of 13 tokens,
-// 64 / 8 heads, up to 16,384 keys 200 us instead of 304; 1,024 tokens, 32 heads, behind 16,384 keys 825
-// instead of 1,924; but 13 tokens of 32 heads at 65,536 keys 242 instead of 131: a step takes the same time
-// for 1 row as for 128.  What bounds it: about 1,700 clocks an SM for a 64-key step, shared memory (decoded
-// operands stored once and read twice, the queries once a step: 770 clocks) and the decoding warps' latency.
-// Four stages at one CTA an SM, with 8 or 16 decoding warps, take as long (212 us).
+// 64 / 8 heads, up to 16,384 keys 191 us instead of 304; 1,024 tokens, 32 heads, behind 16,384 keys 656
+// instead of 1,886; but 13 tokens of 32 heads at 65,536 keys 242 instead of 131: a step takes nearly the same
+// time for 1 row as for 128.  What bounds it: a step's 64 keys take about 1,700 clocks an SM, of which shared
+// memory (decoded operands stored once and read twice, the queries once a step) is busy for 770; a CTA's
+// decoding warps work 2,200 clocks on a step, its softmax warps 1,400, both at a third of the issue slots.
+// Tried and no faster: one CTA an SM with four stages and 8 or 16 decoding warps; the queries in tensor memory
+// with one stage of scores; a barrier each for decoded keys and values.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
                       float scale_log2, int nslots, int q_vec, float* __restrict__ part_o,
                       float2* __restrict__ part_s) {
   extern __shared__ uint8_t tc_raw[];
-  __shared__ int nan_from[2][4];  // per class and 32-feature group: the first key whose values are NaN
+  __shared__ int nan_from[QA_TC_CLASSES][4];  // per class and 32-feature group: the first key whose values are NaN
   pdl_wait();
   const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
   int len, count;
@@ -161,8 +163,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
   const int last = min(min(t0 + (tile * TC_ROWS + TC_ROWS - 1) / grp, t0 + tc - 1), count - 1);
   if (first > last) return;
   const int pmin = len + first, pmax = len + last;
-  const int cl0 = max(qa_class(pmin), QA_TC_CLASS), cl1 = qa_class(pmax);
-  if (cl1 < cl0 || static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl0) > pmax) return;
+  const int cl0 = qa_tc_class(pmin), cl1 = qa_tc_class(pmax);
+  if (pmax < QA_TC_BEGIN || static_cast<int64_t>(blockIdx.x) * qa_tc_keys(cl0) > pmax) return;
 
   uint8_t* smem = tc_raw + ((1024 - (smem_u32(tc_raw) & 1023)) & 1023);
   uint8_t *qs = smem, *ks = smem + Q_BYTES, *vs = ks + STAGES * KV_BYTES;
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
     fence_barrier_init();
     *gave_up = 0;
   }
-  if (threadIdx.x < 8) nan_from[threadIdx.x >> 2][threadIdx.x & 3] = INT32_MAX;
+  if (threadIdx.x < 4 * QA_TC_CLASSES) nan_from[threadIdx.x >> 2][threadIdx.x & 3] = INT32_MAX;
   if (warp == SOFT_WARPS + DEC_WARPS) {
     tmem_alloc(tmem_slot, TMEM_COLS);
     tmem_relinquish();
@@ -222,18 +224,18 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
   bool ok = true;
   int it = 0;  // steps so far
   for (int cl = cl0; cl <= cl1; ++cl) {
-    const int kall = static_cast<int>(min(static_cast<int64_t>(pmax), qa_class_end(cl) - 1)) + 1;
-    if (static_cast<int64_t>(blockIdx.x) * qa_cta_keys(cl) >= kall) continue;
-    const int kbeg = blockIdx.x * qa_cta_keys(cl), kend = min(kall, kbeg + qa_cta_keys(cl));
+    const int kall = static_cast<int>(min(static_cast<int64_t>(pmax), qa_tc_class_end(cl) - 1)) + 1;
+    if (static_cast<int64_t>(blockIdx.x) * qa_tc_keys(cl) >= kall) continue;
+    const int kbeg = blockIdx.x * qa_tc_keys(cl), kend = min(kall, kbeg + qa_tc_keys(cl));
     const int steps = (kend - kbeg + TC_KEYS - 1) / TC_KEYS;
 
     if (warp < SOFT_WARPS) {
       const int R = tile * TC_ROWS + threadIdx.x, t = t0 + R / grp;
-      const bool mine = R < tc * grp && t < count && qa_class(len + t) == cl;
+      const bool mine = R < tc * grp && t < count && len + t >= QA_TC_BEGIN && qa_tc_class(len + t) == cl;
       const int lim = mine ? len + t : INT32_MAX - 1;
       const bool any = __any_sync(0xffffffffu, mine);
       // keys that every row of the class sees need no mask
-      const int clear = max(pmin, static_cast<int>(qa_class_end(cl - 1))) + 1;
+      const int clear = max(pmin, qa_tc_class_begin(cl)) + 1;
       const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < steps && ok; ++i) {
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
           tmem_ld_32x32b_x16(tmem_o + lanes + c0, o);
           tmem_ld_wait();
           if (mine) {
-            const bool bad = !ok || nan_from[cl - QA_TC_CLASS][c0 / 32] <= lim;
+            const bool bad = !ok || nan_from[cl][c0 / 32] <= lim;
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
               *reinterpret_cast<float4*>(part_o + prow * DH + c0 + j) =
@@ -285,21 +287,26 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
       const int32_t* table = rows.table + b * rows.table_stride;
       const uint8_t* head_base = cache.block(0, kvh);
       const size_t page_bytes = static_cast<size_t>(cache.G) * cache.block_bytes;
-      // lane i < 4: page (or -1) and slot of the 16 keys from 16 i on
-      int page = -1, slot = 0;
+      // lane i: page id and slot of chunk i (16 keys) of a run of 512 keys; the next run's are on their way while
+      // one is used
+      int page = -1, slot = 0, page_next = -1, slot_next = 0;
       bool bad = false;
       auto load_pages = [&](int key) {
         const int kk = key + 16 * lane;
-        page = -1;
-        if (lane < TC_KEYS / 16 && kk < kend) {
+        page_next = -1;
+        if (kk < kend) {
           const int n = kk / P;
-          slot = kk - n * P;
-          page = __ldg(table + n);
-          if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(cache.pages)) {
-            page = -1;
-            bad = true;
-          }
+          slot_next = kk - n * P;
+          page_next = __ldg(table + n);
         }
+      };
+      // chunk sub of step i: whether its page is one of the pool, and its slot
+      auto chunk_of = [&](int i, int sub, int* sl) {
+        const int at = (4 * i + sub) & 31, id = __shfl_sync(0xffffffffu, page, at);
+        *sl = __shfl_sync(0xffffffffu, slot, at);
+        const bool in = kbeg + i * TC_KEYS + 16 * sub < kend, ok = in && static_cast<uint32_t>(id) < static_cast<uint32_t>(cache.pages);
+        bad |= in && !ok;
+        return ok ? id : -1;
       };
       // keys: a thread takes 32 features c of key 32 p + 8 dw + lane % 8 (p: two passes); values: eight
       // features f8 of the eight keys from k8 on
@@ -310,11 +317,16 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
         uint32_t vw[8];
         uint4 vsc;
       } raw[2];
-      auto load_k = [&](Raw& x) {
+      auto load = [&](Raw& x, int i) {
+        if ((i & 7) == 0) {
+          page = page_next, slot = slot_next;
+          load_pages(kbeg + (i + 8) * TC_KEYS);
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int id = __shfl_sync(0xffffffffu, page, 2 * p + (dw >> 1));
-          const int sl = __shfl_sync(0xffffffffu, slot, 2 * p + (dw >> 1)) + (dw & 1) * 8 + (lane & 7);
+          int sl;
+          const int id = chunk_of(i, 2 * p + (dw >> 1), &sl);
+          sl += (dw & 1) * 8 + (lane & 7);
           x.kw[p] = make_uint4(0u, 0u, 0u, 0u);
           x.ksc[p] = 0x7FC0u;  // keys without a page: a NaN score for whoever sees them
           if (id >= 0) {
@@ -323,10 +335,9 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
             x.ksc[p] = __ldg(reinterpret_cast<const uint16_t*>(blk + P * DH) + c * P + sl);
           }
         }
-      };
-      auto load_v = [&](Raw& x) {
-        const int id = __shfl_sync(0xffffffffu, page, k8 >> 4);
-        const int sl = __shfl_sync(0xffffffffu, slot, k8 >> 4) + (k8 & 8);
+        int sl;
+        const int id = chunk_of(i, k8 >> 4, &sl);
+        sl += k8 & 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) x.vw[j] = 0u;
         x.vsc = make_uint4(0u, 0u, 0u, 0u);
@@ -368,7 +379,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
           for (int e = 0; e < 8; ++e) {
             uint32_t& w = (&x.vsc.x)[e >> 1];
             if (((e & 1 ? w >> 16 : w) & 0x7F80u) == 0x7F80u) {
-              atomicMin(&nan_from[cl - QA_TC_CLASS][f8 >> 2], key + k8 + e);
+              atomicMin(&nan_from[cl][f8 >> 2], key + k8 + e);
               w &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
             }
           }
@@ -393,17 +404,11 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
         fence_async_smem();  // also waits for loads on their way: one a step
         __syncwarp();
         if (lane == 0) mbar_arrive(kv_full + n % STAGES);
-        load_k(x);  // STAGES steps ahead
-        load_v(x);
-        load_pages(key + 3 * TC_KEYS);
+        load(x, i + 2);
       };
       load_pages(kbeg);
-      load_k(raw[0]);
-      load_v(raw[0]);
-      load_pages(kbeg + TC_KEYS);
-      load_k(raw[1]);
-      load_v(raw[1]);
-      load_pages(kbeg + 2 * TC_KEYS);
+      load(raw[0], 0);
+      load(raw[1], 1);
       for (int i = 0; i < steps && ok; i += 2) {
         decode(raw[0], i);
         if (ok && i + 1 < steps) decode(raw[1], i + 1);
@@ -417,33 +422,44 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
       const uint32_t k0 = static_cast<uint32_t>(umma_desc_sw128(smem_u32(ks)));
       const uint32_t v0 = static_cast<uint32_t>(umma_desc_sw128(smem_u32(vs)));
       constexpr uint32_t S_DESC = umma_idesc_bf16(TC_ROWS, TC_KEYS), O_DESC = umma_idesc_bf16(TC_ROWS, DH);
-      auto scores = [&](int n) {
-        // (decoded after the product of the P in S's place was done)
-        if (!wait(kv_full, n)) return false;
-        tc_fence_after();
-        const uint32_t st = n % STAGES, d = tmem + st * TC_KEYS, k = k0 + st * (KV_BYTES >> 4);
-#pragma unroll
-        for (int j = 0; j < DH / 16; ++j) {
-          const uint32_t qa = q0 + (((j >> 2) * (TC_ROWS * 128) + (j & 3) * 32) >> 4);
-          const uint32_t kb = k + (((j >> 2) * (TC_KEYS * 128) + (j & 3) * 32) >> 4);
-          if (j == 0)
-            mma_ss<false>(on, d, qa, kb, high, S_DESC);
-          else
-            mma_ss<true>(on, d, qa, kb, high, S_DESC);
-        }
-        mma_commit(on, smem_u32(s_full) + 8 * st);
-        return true;
+      // whatever is ready first: a step's scores (its keys are decoded, so the P in S's place is multiplied, too)
+      // or the outputs of the one before
+      auto ready = [&](uint64_t* bars, int n) {
+        return __all_sync(0xffffffffu, mbar_try_wait(bars + n % STAGES, n / STAGES & 1)) != 0;
       };
-      ok = ok && scores(it);
-      for (int i = 0; i < steps && ok; ++i) {
-        const int n = it + i;
-        ok = (i + 1 >= steps || scores(n + 1)) && wait(p_full, n);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t st = n % STAGES, p = tmem + st * TC_KEYS, v = v0 + st * (KV_BYTES >> 4);
+      uint64_t idle_since = 0;
+      for (int qk = 0, pv = 0, idle = 0; pv < steps;) {
+        if (qk < steps && qk < pv + STAGES && ready(kv_full, it + qk)) {
+          tc_fence_after();
+          const uint32_t st = (it + qk) % STAGES, d = tmem + st * TC_KEYS, k = k0 + st * (KV_BYTES >> 4);
 #pragma unroll
-        for (int j = 0; j < TC_KEYS / 16; ++j) mma_ts(on, tmem_o, p + 8 * j, v + 2 * j, high, O_DESC, i != 0 || j != 0);
-        mma_commit(on, smem_u32(pv_done) + 8 * st);
+          for (int j = 0; j < DH / 16; ++j) {
+            const uint32_t qa = q0 + (((j >> 2) * (TC_ROWS * 128) + (j & 3) * 32) >> 4);
+            const uint32_t kb = k + (((j >> 2) * (TC_KEYS * 128) + (j & 3) * 32) >> 4);
+            if (j == 0)
+              mma_ss<false>(on, d, qa, kb, high, S_DESC);
+            else
+              mma_ss<true>(on, d, qa, kb, high, S_DESC);
+          }
+          mma_commit(on, smem_u32(s_full) + 8 * st);
+          ++qk, idle = 0;
+        } else if (pv < qk && ready(p_full, it + pv)) {
+          tc_fence_after();
+          const uint32_t st = (it + pv) % STAGES, p = tmem + st * TC_KEYS, v = v0 + st * (KV_BYTES >> 4);
+#pragma unroll
+          for (int j = 0; j < TC_KEYS / 16; ++j) mma_ts(on, tmem_o, p + 8 * j, v + 2 * j, high, O_DESC, pv != 0 || j != 0);
+          mma_commit(on, smem_u32(pv_done) + 8 * st);
+          ++pv, idle = 0;
+        } else if ((++idle & 255) == 0) {
+          const uint64_t now = __shfl_sync(0xffffffffu, globaltimer_ns(), 0);
+          if (idle == 256) idle_since = now;
+          if (*gave_up != 0 || now - idle_since > EVS_WAIT_LIMIT_NS) {
+            evs_record_error(cache.err, EVS_ETIMEOUT, EVS_K_Q4_ATTN, b);
+            *gave_up = 1;
+            break;
+          }
+        }
+        __syncwarp();
       }
       it += steps;
     }
