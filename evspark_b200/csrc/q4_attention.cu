@@ -634,8 +634,12 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   // tokens per pass: as many as the workspace holds partial results for
   const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
   const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles
-  const int tokens = static_cast<int>(std::min<int64_t>(r.T, fit * QA_ROWS / grp));
+  int tokens = static_cast<int>(std::min<int64_t>(r.T, fit * QA_ROWS / grp));
   EVS_CHECK_RANGE(tokens >= 1, "q4 attention: the workspace is too small");
+  if (tokens < r.T && grp <= 128) {  // passes of the same length, in whole tiles of the tensor-core kernel
+    const int passes = (r.T + tokens - 1) / tokens, tile = 128 / grp, even = (r.T + passes - 1) / passes;
+    tokens = std::min(tokens, (even + tile - 1) / tile * tile);
+  }
   for (int t0 = 0; t0 < r.T; t0 += tokens) {
     const int tc = std::min(tokens, r.T - t0);
     const int prows = static_cast<int>(padded_rows(static_cast<int64_t>(tc) * grp)), tiles = prows / QA_ROWS;

@@ -9,7 +9,7 @@
 // everything, so that a step's scores are there while the one before is still worked on; two CTAs an SM.
 //
 // Measured beside the 16-row mma.sync kernel, which decodes the keys once per 16 rows: 16 rows of 13 tokens,
-// 64 / 8 heads, up to 16,384 keys 191 us instead of 304; 1,024 tokens, 32 heads, behind 16,384 keys 656
+// 64 / 8 heads, up to 16,384 keys 191 us instead of 304; 1,024 tokens, 32 heads, behind 16,384 keys 616
 // instead of 1,886; but 13 tokens of 32 heads at 65,536 keys 242 instead of 131: a step takes nearly the same
 // time for 1 row as for 128.  What bounds it: a step's 64 keys take about 1,700 clocks an SM, of which shared
 // memory (decoded operands stored once and read twice, the queries once a step) is busy for 770; a CTA's

@@ -558,3 +558,33 @@ def test_workspace_follows_the_table_not_the_bound_alone(q4):
     q4.q4_attention(q, fresh, table[:, :10].contiguous(), i32([100]), max_length=end)
     assert torch.equal(q4.q4_attention(q, fresh, table, i32([end - 2]), max_length=end), want)
     fresh.check()
+
+
+@pytest.mark.parametrize("D,H,G,T,start,dtype", [(32, 4, 2, 40, 2500, F32), (128, 3, 1, 50, 2300, BF), (128, 2, 1, 130, 4000, BF),
+                                                 (128, 6, 1, 50, 6000, BF)])
+def test_small_workspace_takes_several_passes(q4, D, H, G, T, start, dtype):
+    """The C entry with less scratch than it asks for: the same bits in more passes, and a refusal below a token."""
+    import ctypes as C
+
+    from evspark_b200 import _native as N
+
+    end = start + T
+    cache, table = make_rows(q4, [end, 7], 32, G, D)
+    fill_cache(q4, cache, table, [0, 0], [end, 7], G, D, dtype=dtype)
+    lengths, counts = i32([start, 2]), i32([T, 5])
+    q = randn(2, T, H, D, seed=7, dtype=dtype)
+    want = q4.q4_attention(q, cache, table, lengths, counts=counts)
+    rows = N.Q4RowsDesc(table.data_ptr(), lengths.data_ptr(), counts.data_ptr(), table.stride(0), table.shape[1], 2, T)
+    need = N.lib().evs_q4_attention_workspace(cache._ref, C.addressof(rows), H, 0)
+    per_row = need // (-(-T * H // G // 16) * 16)
+    strides = (C.c_int64 * 3)(*q.stride()[:3])
+    for scratch in (16 * per_row, 48 * per_row, need):
+        out = torch.zeros_like(q)
+        ws = torch.empty(scratch, dtype=torch.uint8, device=DEV)
+        q4._call(0, "evs_q4_attention", cache._ref, C.addressof(rows), q.data_ptr(), strides, H, D ** -0.5, 0,
+                 out.data_ptr(), strides, q4._DT[dtype], ws.data_ptr(), scratch)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1, :5], want[1, :5]) and not bool(out[1, 5:].any())
+    with pytest.raises(ValueError, match="workspace"):
+        q4._call(0, "evs_q4_attention", cache._ref, C.addressof(rows), q.data_ptr(), strides, H, D ** -0.5, 0,
+                 out.data_ptr(), strides, q4._DT[dtype], ws.data_ptr(), 8 * per_row // 16)
+    cache.check()
