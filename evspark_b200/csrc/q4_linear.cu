@@ -13,7 +13,14 @@ namespace {
 
 constexpr int LIN_WARPS = 8;
 constexpr int LIN_THREADS = 32 * LIN_WARPS;
+// CTAs an SM: two wherever registers and shared memory allow it, so that the grid is resident at once
+template <typename TX, int NT>
+constexpr int lin_per_sm() {
+  return NT * (sizeof(TX) == 2 ? 1 : 3) <= 6 ? 2 : 1;
+}
 constexpr int LIN_CLUSTER = 8;    // CTAs of one output tile at most (splits of K)
+// rows of a tile that one CTA of the cluster adds up
+__host__ __device__ constexpr int lin_own_rows(int rows, int splits) { return ((rows + splits - 1) / splits + 7) / 8 * 8; }
 
 // x staged in shared memory in the order in which the products read it: per (K block, 8-token
 // tile, part) four words of 16 bytes per lane; lane (n, c) word w holds features 32 c + 8 w .. + 7 of
@@ -93,12 +100,12 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
 // features a step against every token of the tile, so the codes are decoded once, in the registers that
 // the product reads.  What bounds it is the decode's instructions and their latency: 420 warp
 // instructions per 4,096 codes (192 of them shifts, masks and fma of the decode), 0.44 issued a clock and
-// scheduler.  13 x 22016 x 4096, group 64: 20.4 us, 2.3 TB/s of codes and scales (floor 7.5 us at 6.5 TB/s);
-// 13 x 8192 x 22528: 34.8 us; 1 x 4096 x 4096: 6.1 us.
+// scheduler.  13 x 22016 x 4096, group 64: 20.0 us, 2.4 TB/s of codes and scales (floor 7.5 us at 6.5 TB/s);
+// 13 x 8192 x 22528: 34.1 us; 1 x 4096 x 4096: 6.4 us; 32 x 4096 x 4096: 12.4 us.
 // grid (K splits = cluster, row tiles, token tiles).  Registers hold the next two K blocks' codes
 // while one is multiplied; the first ones are on their way before x is staged.
 template <typename TX, typename TO, int NT, int KW>
-__global__ void __launch_bounds__(LIN_THREADS, NT <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(LIN_THREADS, lin_per_sm<TX, NT>())
     q4_linear_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint8_t* __restrict__ codes,
                      const uint16_t* __restrict__ scales, int N, int K, int group_shift, TO* __restrict__ out,
                      int64_t ldo, int chunk_kb, int vec, uint32_t red_offset) {
@@ -214,48 +221,63 @@ __global__ void __launch_bounds__(LIN_THREADS, NT <= 2 ? 2 : 1)
     }
   }
   // Sums over the K warps and the cluster's splits, in that order.  Rank r owns RC rows of the output
-  // tile; every CTA pushes its sums into the owner's [split][K warp][token][row] slots, which alias
-  // nothing that a slower CTA still reads, so one cluster barrier is enough.
+  // tile; every CTA pushes its sums into the owner's [split][K warp][row][token] slots, which alias
+  // nothing that a slower CTA still reads, so one cluster barrier is enough.  A thread's tokens of a row
+  // lie side by side there (place c 2 NT + 2 j + e holds token 8 j + 2 c + e), so that remote stores are
+  // wide: 13 x 4096 x 4096 takes 7.3 us, 8.1 with stores of 4 bytes.
   constexpr int TOK = 8 * NT;
-  const int RC = (LIN_ROWS + S - 1) / S;
+  const int RC = lin_own_rows(LIN_ROWS, S);
   const uint32_t red = smem_u32(lin_sm) + red_offset;
   cluster_wait();  // every CTA of the cluster has started
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = 32 * wr + 16 * i + 8 * h + g, owner = r / RC;
+      const int r = 32 * wr + 16 * i + 8 * h, owner = r / RC;  // RC is a multiple of 8
       uint32_t a;
       asm("mapa.shared::cluster.u32 %0, %1, %2;"
           : "=r"(a)
-          : "r"(red + 4 * (((rank * KW + wk) * TOK + 2 * c) * RC + r - owner * RC)), "r"(owner));
+          : "r"(red + 4 * (((rank * KW + wk) * RC + r - owner * RC + g) * TOK + c * 2 * NT)), "r"(owner));
+      if constexpr (NT == 1) {
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(acc[i][0][2 * h]), "f"(acc[i][0][2 * h + 1])
+                     : "memory");
+      } else {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a + 4 * (8 * j + e) * RC), "f"(acc[i][j][2 * h + e])
+        for (int j = 0; j < NT; j += 2)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a + 8 * j), "f"(acc[i][j][2 * h]),
+                       "f"(acc[i][j][2 * h + 1]), "f"(acc[i][j + 1][2 * h]), "f"(acc[i][j + 1][2 * h + 1])
                        : "memory");
+      }
     }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  const float* mine = reinterpret_cast<const float*>(lin_sm + red_offset);
+  const float4* mine = reinterpret_cast<const float4*>(lin_sm + red_offset);
+  constexpr int UNITS = TOK / 4;  // of a row
   const int tokens = min(TOK, M - m0), first = rank * RC, own_rows = min(RC, min(LIN_ROWS, N - n0) - first);
-  for (int i = threadIdx.x; i < tokens * own_rows; i += LIN_THREADS) {
-    const int tok = i / own_rows, r = i - tok * own_rows;
-    float v[LIN_CLUSTER][KW];
+  for (int i = threadIdx.x; i < own_rows * UNITS; i += LIN_THREADS) {
+    const int r = i / UNITS, u = i % UNITS;
+    float4 v[LIN_CLUSTER][KW];
 #pragma unroll
     for (int p = 0; p < LIN_CLUSTER; ++p)
 #pragma unroll
-      for (int q = 0; q < KW; ++q) v[p][q] = p < S ? mine[((p * KW + q) * TOK + tok) * RC + r] : 0.f;
-    float sum = 0.f;
+      for (int q = 0; q < KW; ++q)
+        v[p][q] = p < S ? mine[((p * KW + q) * RC + r) * UNITS + u] : make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = 0; p < LIN_CLUSTER; ++p)
       if (p < S) {
-        float part = v[p][0];
 #pragma unroll
-        for (int q = 1; q < KW; ++q) part += v[p][q];
-        sum += part;
+        for (int e = 0; e < 4; ++e) {
+          float part = (&v[p][0].x)[e];
+#pragma unroll
+          for (int q = 1; q < KW; ++q) part += (&v[p][q].x)[e];
+          sum[e] += part;
+        }
       }
-    out[static_cast<int64_t>(m0 + tok) * ldo + n0 + first + r] = from_f32<TO>(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = 4 * u + e, tok = at % (2 * NT) / 2 * 8 + at / (2 * NT) * 2 + (at & 1);
+      if (tok < tokens) out[static_cast<int64_t>(m0 + tok) * ldo + n0 + first + r] = from_f32<TO>(sum[e]);
+    }
   }
 }
 
@@ -267,13 +289,14 @@ int launch_linear_kw(const void* x, int64_t ldx, int M, const void* codes, const
   const int block_bytes = NT * NP * 2048;  // staged x of one K block
   const int slice = (KB + S - 1) / S;
   // a multiple of 2 KW blocks: whichever the chunk, a K warp takes the same blocks in the same registers
-  int chunk = std::max(2 * KW, (NT <= 2 ? 81920 : 131072) / block_bytes / (2 * KW) * (2 * KW));
+  const int red_bytes = S * KW * 8 * NT * lin_own_rows(ROWS, S) * 4;
+  const int room = (lin_per_sm<TX, NT>() == 2 ? 96 * 1024 : 200 * 1024) - red_bytes;  // some L1 left for the scales
+  int chunk = std::max(2 * KW, room / block_bytes / (2 * KW) * (2 * KW));
   chunk = std::min(chunk, slice);
-  const int red_offset = chunk * block_bytes;
-  const int smem = red_offset + S * KW * 8 * NT * ((ROWS + S - 1) / S) * 4;
+  const int red_offset = chunk * block_bytes, smem = red_offset + red_bytes;
   auto* kern = q4_linear_kernel<TX, TO, NT, KW>;
   static std::atomic<unsigned long long> done{0};
-  EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), 200 * 1024));
+  EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), 227 * 1024));
   const int vec = (reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(TX)) % 16 == 0) ? 1 : 0;
   const int ztiles = (M + 8 * NT - 1) / (8 * NT);
   EVS_CHECK_ARG(tiles <= 65535 && ztiles <= 65535, "q4 linear: too many rows or tokens");
@@ -317,10 +340,9 @@ int launch_linear_t(const void* x, int64_t ldx, int M, const void* codes, const 
                     void* out, int64_t ldo, cudaStream_t st, bool pdl) {
   if (M <= 8) return launch_linear_nt<TX, TO, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
   if (M <= 16) return launch_linear_nt<TX, TO, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
-  // tokens beyond one tile's read the weight again; three-part fp32 rows leave no room for 64 of them
-  if (M <= 32 || sizeof(TX) == 4)
-    return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
-  return launch_linear_nt<TX, TO, 8>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
+  // tokens beyond one tile's read the weight again: tiles of 64 would leave one CTA an SM (64 tokens x 4096 x
+  // 4096 then take 35 us, and 64 x 8192 x 22528 145)
+  return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl);
 }
 
 // one warp per (row, group): codes and scale of the group's features (K padded with zeros)

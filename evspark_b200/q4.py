@@ -143,7 +143,7 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
 
     bf16 rows multiply the held weight values exactly; fp32 rows are used at full precision.  A row's
     result does not depend on the other rows.  Meant for the few tokens of a decode step or verify
-    block: every 64 rows read the weight once."""
+    block: every 32 rows read the weight once."""
     codes, scales, n, k, group = w._args
     dt = _DT.get(x.dtype)
     if dt is None:
