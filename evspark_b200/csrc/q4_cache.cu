@@ -91,7 +91,7 @@ __device__ __forceinline__ uint32_t codes_fast(const float (&x)[8], float s, flo
 // and rotation in 64 bits (2 of the 64 fma a clock that an SM has per value: not what bounds this), so
 // that a key's codes are those of its exact rotation.  The next head row's loads are in flight while one
 // is worked on (69.5 us instead of 78.1 for eight rows of up to 1,024 tokens, 32 heads of 128, bf16; about
-// 2.3 TB/s): instructions bound it, 0.69 issued a clock and scheduler, 30 per value.  13 tokens: 6.5 us, a
+// 2.3 TB/s): instructions bound it, 0.69 issued a clock and scheduler, 30 per value.  13 tokens: 6.3 us, a
 // chain of latencies.
 template <typename T>
 __global__ void __launch_bounds__(APP_THREADS, 4)
@@ -123,15 +123,15 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
     next_lo.load(p, vec != 0);
     next_hi.load(p + half, vec != 0);
   };
-  load(r);  // on its way while the angles are computed
+  load(r);  // on its way while the angles are computed, as is the page
+  const int64_t page = q4_page(cache, rows, b, pos);
+  const int slot = pos % cache.P;
   if (threadIdx.x < half && static_cast<int>(blockIdx.y) * per < H + G) {
     double s, c;
     sincos(static_cast<double>(pos) * freq.f[threadIdx.x], &s, &c);
     turn[threadIdx.x & 7][threadIdx.x >> 3] = make_double2(c, s);
   }
   __syncthreads();
-  const int64_t page = q4_page(cache, rows, b, pos);
-  const int slot = pos % cache.P;
   if (page < 0 && threadIdx.x == 0 && blockIdx.y == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
   // rows of one pass share the count of passes, so that whole warps meet the shuffles below
   for (int r0 = blockIdx.y * per; r0 < total; r0 += gridDim.y * per, r += gridDim.y * per) {
