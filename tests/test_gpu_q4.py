@@ -588,3 +588,38 @@ def test_small_workspace_takes_several_passes(q4, D, H, G, T, start, dtype):
         q4._call(0, "evs_q4_attention", cache._ref, C.addressof(rows), q.data_ptr(), strides, H, D ** -0.5, 0,
                  out.data_ptr(), strides, q4._DT[dtype], ws.data_ptr(), 8 * per_row // 16)
     cache.check()
+
+
+def test_attention_long_in_graphs_and_on_two_streams_at_once(q4):
+    """The tcgen05 kernel captured, replayed with other lengths and queries, and two calls at the same time."""
+    D, G, H, T, room = 128, 4, 8, 40, 9000
+    cache, table = make_rows(q4, [room, room], 64, G, D)
+    fill_cache(q4, cache, table, [0, 0], [room, room], G, D)
+    q, lengths = randn(2, T, H, D, seed=5, dtype=BF), i32([4090, 8000])
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        q4.q4_attention(q, cache, table, lengths, out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            q4.q4_attention(q, cache, table, lengths, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    for seed, starts in ((6, (8900, 5000)), (7, (100, 4500)), (8, (4096, 0))):
+        q.copy_(randn(2, T, H, D, seed=seed, dtype=BF))
+        lengths.copy_(i32(starts))
+        graph.replay()
+        assert torch.equal(out, q4.q4_attention(q, cache, table, lengths)), starts
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    qs = [randn(2, T, H, D, seed=20 + i, dtype=BF) for i in range(2)]
+    at = [i32([8000, 6000]), i32([5000, 8500])]
+    want = [q4.q4_attention(qs[i], cache, table, at[i]) for i in range(2)]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(q4.q4_attention(qs[i], cache, table, at[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+    cache.check()
