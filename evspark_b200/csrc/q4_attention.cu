@@ -13,7 +13,7 @@
 // Keys and values are decoded in the registers that the products read them from, with no rounding
 // between codes and product.  What bounds it: about 1,000 warp instructions per 32 keys and row tile
 // (384 the decode), 0.54 issued a clock and scheduler at 12 warps an SM.  bf16, 32 heads of 128, 13
-// tokens: 131 us at 65,536 keys (2.3 TB/s of codes and scales; floor 46 us), 412 us at 262,144 (2.9 TB/s).
+// tokens: 128 us at 65,536 keys (2.4 TB/s of codes and scales; floor 46 us), 411 us at 262,144 (2.9 TB/s).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -73,8 +73,8 @@ __host__ __device__ constexpr int qa_q_floats() {
   return qa_parts_q(sizeof(T)) * 2 * (DH / 32) * 32 * 4;
 }
 
-// One CTA's keys for one tile of 16 rows.  FUSED: each row's result stays in shared memory (fin), else it
-// goes to the CTA's slot of the workspace.  Classes above top are another kernel's.
+// One CTA's keys for one tile of 16 rows.  FUSED: each row's result goes into the shared memory of the CTA
+// of the cluster that folds it, else to the CTA's slot of the workspace.  Classes above top are another kernel's.
 template <typename T, int DH, bool FUSED>
 __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache, const Q4RowsDev& rows, const Q4Tensor& q,
                                           int grp, int t0, int tc, int tiles, float scale_log2, int nslots, bool q_vec,
@@ -430,21 +430,32 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
         f[w] = mw[w] == -CUDART_INF_F ? 0.f : qa_ex2(mw[w] - big);
         sum = fmaf(res[(w * QA_ROWS + r) * LD + DH + 1], f[w], sum);
       }
-      float* dst_o;
       if constexpr (FUSED) {
-        dst_o = res + (QA_WARPS * QA_ROWS + r) * LD;
-        if (lane == 0) *reinterpret_cast<float2*>(dst_o + DH) = make_float2(big, sum);
+        // to the CTA that folds the row: [slot][row / nslots] of its shared memory
+        const uint32_t at = smem_u32(res + QA_WARPS * QA_ROWS * LD) +
+                            4 * ((blockIdx.x * ((QA_ROWS + nslots - 1) / nslots) + r / nslots) * LD);
+        uint32_t dst;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(at), "r"(r % nslots));
+        if (lane == 0)
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst + 4 * DH), "f"(big), "f"(sum) : "memory");
+#pragma unroll
+        for (int d = 0; d < DH; d += 32) {
+          float acc = 0.f;
+#pragma unroll
+          for (int w = 0; w < QA_WARPS; ++w) acc = fmaf(res[(w * QA_ROWS + r) * LD + d + lane], f[w], acc);
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4 * (d + lane)), "f"(acc) : "memory");
+        }
       } else {
         const size_t prow =
             ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots + blockIdx.x;
-        dst_o = part_o + prow * DH;
         if (lane == 0) part_s[prow] = make_float2(big, sum);
-      }
-      for (int d = lane; d < DH; d += 32) {
-        float acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < QA_WARPS; ++w) acc = fmaf(res[(w * QA_ROWS + r) * LD + d], f[w], acc);
-        dst_o[d] = acc;
+        for (int d = 0; d < DH; d += 32) {
+          float acc = 0.f;
+#pragma unroll
+          for (int w = 0; w < QA_WARPS; ++w) acc = fmaf(res[(w * QA_ROWS + r) * LD + d + lane], f[w], acc);
+          part_o[prow * DH + d + lane] = acc;
+        }
       }
     }
     __syncthreads();
@@ -480,21 +491,28 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
   attn_tile<T, DH, false>(qa_sm, cache, rows, q, grp, t0, tc, tiles, scale_log2, nslots, q_vec != 0, top, part_o, part_s);
 }
 
+// rows that the CTAs of a cluster of nslots hold for folding: [slot][row / nslots], at most
+constexpr int QA_FOLD_ROWS = QA_ROWS + QA_CLUSTER - 1;
+
 // Short contexts: the CTAs of a tile are one cluster and fold their results through its shared memory,
-// with the combine kernel's arithmetic and without its launch and the workspace.
+// with the combine kernel's arithmetic and without its launch and the workspace.  Row r is folded by CTA
+// r % nslots, into whose shared memory the others push their results: one cluster barrier on the way.
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
     q4_attn_fused_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor q, Q4Tensor out, int grp, int tiles,
                          float scale_log2, int q_vec) {
+  cluster_arrive_relaxed();
   pdl_trigger();
-  extern __shared__ __align__(16) float qa_sm[];  // the queries, [warp][16][DH + 2] results, [16][DH + 2] folded
+  extern __shared__ __align__(16) float qa_sm[];  // the queries, [warp][16][DH + 2] results, the rows to fold
   pdl_wait();
+  cluster_wait();  // every CTA of the cluster has started
   const int nslots = gridDim.x;
   attn_tile<T, DH, true>(qa_sm, cache, rows, q, grp, 0, rows.T, tiles, scale_log2, nslots, q_vec != 0, 3,
                          nullptr, nullptr);
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int kvh = blockIdx.y / tiles, tile = blockIdx.y % tiles, b = blockIdx.z;
+  const int per = (QA_ROWS + nslots - 1) / nslots;
   const float* fin = qa_sm + qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2);
   for (int r = warp * nslots + blockIdx.x; r < QA_ROWS; r += QA_WARPS * nslots) {
     const int R = tile * QA_ROWS + r, t = R / grp;
@@ -502,17 +520,15 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
     T* dst = static_cast<T*>(out.p) + b * out.sb + t * out.st + (kvh * grp + R % grp) * out.sh;
     int n;
     if (!fold_row<T, DH>(cache, rows, b, t, nslots, false, dst, &n)) continue;
-    const uint32_t at = smem_u32(fin + r * (DH + 2));
+    const float* row = fin + r / nslots * (DH + 2);
     float v[QA_CLUSTER][DH / 32], mx[QA_CLUSTER], sm[QA_CLUSTER], big = -CUDART_INF_F;
 #pragma unroll
     for (int x = 0; x < QA_CLUSTER; ++x)
       if (x < n) {
-        uint32_t a;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(x));
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(mx[x]), "=f"(sm[x]) : "r"(a + 4 * DH) : "memory");
+        const float* a = row + x * per * (DH + 2);
+        mx[x] = a[DH], sm[x] = a[DH + 1];
 #pragma unroll
-        for (int d = 0; d < DH / 32; ++d)
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[x][d]) : "r"(a + 4 * (32 * d + lane)) : "memory");
+        for (int d = 0; d < DH / 32; ++d) v[x][d] = a[32 * d + lane];
         big = fmaxf(big, mx[x]);
       }
     float acc[DH / 32], sum = 0.f;
@@ -538,9 +554,6 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) dst[32 * d + lane] = from_f32<T>(acc[d] / sum);
   }
-  // no CTA of the cluster leaves while another still reads its results
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // One CTA per output row: warp w folds the slots w, w + 4, ... in order, then the four sums in order.
@@ -599,7 +612,7 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   if (fused_fits(qa_slots(bound), r.T, grp, c.G)) {
     const int nslots = qa_slots(bound);
     auto* kern = q4_attn_fused_kernel<T, DH>;
-    const int smem = (qa_q_floats<T, DH>() + (QA_WARPS + 1) * QA_ROWS * (DH + 2)) * 4;
+    const int smem = (qa_q_floats<T, DH>() + (QA_WARPS * QA_ROWS + QA_FOLD_ROWS) * (DH + 2)) * 4;
     static std::atomic<unsigned long long> done{0};
     EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
     const int tiles = static_cast<int>(padded_rows(static_cast<int64_t>(r.T) * grp) / QA_ROWS);
