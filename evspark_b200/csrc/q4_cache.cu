@@ -246,55 +246,63 @@ __global__ void __launch_bounds__(APP_THREADS, 4)
   }
 }
 
-// One thread per eight values of K or V: the values that the cache holds at lengths[b] + t.  Four loads
-// of a thread in flight; 31 us for eight rows of up to 1,024 tokens, 32 heads of 128 (2.9 TB/s, bound by
-// the chain length, page, codes of each CTA).
-template <typename T>
+// One thread per eight values of K or V: the values that the cache holds at lengths[b] + t.  A CTA takes TOK
+// tokens of a row, with four loads of each on their way per thread.  Eight rows of up to 1,024 tokens, 32
+// heads of 128: 28.6 us with two tokens a CTA, 31.6 with one (bound by the chain length, page, codes, store).
+template <typename T, int TOK>
 __global__ void __launch_bounds__(APP_THREADS)
     q4_read_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor k, Q4Tensor v, int vec) {
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / rows.T, t = blockIdx.x - b * rows.T;
+  const int runs = (rows.T + TOK - 1) / TOK, b = blockIdx.x / runs, t0 = (blockIdx.x - b * runs) * TOK;
   int len, count;
   if (!q4_row(rows, b, &len, &count, cache.P)) {
     if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
     return;
   }
-  if (t >= count) return;
+  if (t0 >= count) return;
   const int D = cache.D, G = cache.G, log8 = D == 128 ? 4 : (D == 64 ? 3 : 2);
-  const int pos = len + t;
-  const int64_t page = q4_page(cache, rows, b, pos);
-  if (page < 0) {
-    if (threadIdx.x == 0) evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
-    return;
+  int64_t page[TOK];
+  int slot[TOK];
+#pragma unroll
+  for (int x = 0; x < TOK; ++x) {
+    const int pos = len + t0 + x;
+    page[x] = t0 + x < count ? q4_page(cache, rows, b, pos) : -1;
+    slot[x] = pos % cache.P;
+    if (page[x] < 0 && t0 + x < count && threadIdx.x == 0)
+      evs_record_error(cache.err, EVS_ERANGE, EVS_K_Q4_CACHE, b);
   }
-  const int slot = pos % cache.P, units = 2 * G << log8;
-  const uint8_t* first = cache.block(page, 0);
-  constexpr int BATCH = 4;  // loads of a thread in flight
+  const int units = 2 * G << log8;
+  constexpr int BATCH = 4;
   for (int i0 = blockIdx.y * APP_THREADS * BATCH + threadIdx.x; i0 < units; i0 += gridDim.y * APP_THREADS * BATCH) {
-    uint32_t codes[BATCH], sb[BATCH];
+    uint32_t codes[TOK][BATCH], sb[TOK][BATCH];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
-      if (i >= units) continue;
-      const bool is_v = row >= G;
-      const uint8_t* block = first + static_cast<size_t>(is_v ? row - G : row) * cache.block_bytes;
-      codes[u] = __ldg(reinterpret_cast<const uint32_t*>(block + (is_v ? cache.P * (D / 2) : 0) + slot * (D / 2) + 4 * w));
-      sb[u] = __ldg(reinterpret_cast<const uint16_t*>(block + cache.P * D) + (is_v ? cache.P * (D / 32) : 0) +
-                    (w >> 2) * cache.P + slot);
-    }
+    for (int x = 0; x < TOK; ++x)
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
-      if (i >= units) break;
-      const float s = __uint_as_float(sb[u] << 16);
-      float x[8];
+      for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
+        if (i >= units || page[x] < 0) continue;
+        const bool is_v = row >= G;
+        const uint8_t* block = cache.block(page[x], is_v ? row - G : row);
+        codes[x][u] = __ldg(
+            reinterpret_cast<const uint32_t*>(block + (is_v ? cache.P * (D / 2) : 0) + slot[x] * (D / 2) + 4 * w));
+        sb[x][u] = __ldg(reinterpret_cast<const uint16_t*>(block + cache.P * D) + (is_v ? cache.P * (D / 32) : 0) +
+                         (w >> 2) * cache.P + slot[x]);
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = (static_cast<int>((codes[u] >> (4 * j)) & 15u) - 8) * s;
-      const Q4Tensor& dst = row >= G ? v : k;
-      store8<T>(static_cast<T*>(dst.p) + b * dst.sb + t * dst.st + (row >= G ? row - G : row) * dst.sh + 8 * w, x,
-                vec != 0);
-    }
+    for (int x = 0; x < TOK; ++x)
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * APP_THREADS, row = i >> log8, w = i & ((1 << log8) - 1);
+        if (i >= units || page[x] < 0) continue;
+        const float s = __uint_as_float(sb[x][u] << 16);
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (static_cast<int>((codes[x][u] >> (4 * j)) & 15u) - 8) * s;
+        const Q4Tensor& dst = row >= G ? v : k;
+        store8<T>(static_cast<T*>(dst.p) + b * dst.sb + (t0 + x) * dst.st + (row >= G ? row - G : row) * dst.sh + 8 * w,
+                  y, vec != 0);
+      }
   }
 }
 
@@ -424,10 +432,12 @@ int launch_q4_read(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& k, c
                    cudaStream_t st) {
   const size_t el = dtype == EVS_DTYPE_BF16 ? 2 : 4;
   const int vec = q4_vec(k, el) && q4_vec(v, el);
-  const int tokens = r.B * r.T;
-  const dim3 grid(tokens, tokens >= FEW_TOKENS ? 1 : (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS));
+  const bool few = static_cast<int64_t>(r.B) * r.T < 4 * FEW_TOKENS;
+  const int runs = few ? r.T : (r.T + 1) / 2;
+  const dim3 grid(r.B * runs, few ? (2 * c.G * (c.D / 8) + 4 * APP_THREADS - 1) / (4 * APP_THREADS) : 1);
   EVS_CHECK_ARG(grid.y <= 65535, "q4 read: too many heads");
-  auto* kern = dtype == EVS_DTYPE_BF16 ? q4_read_kernel<__nv_bfloat16> : q4_read_kernel<float>;
+  auto* kern = dtype == EVS_DTYPE_BF16 ? (few ? q4_read_kernel<__nv_bfloat16, 1> : q4_read_kernel<__nv_bfloat16, 2>)
+                                       : (few ? q4_read_kernel<float, 1> : q4_read_kernel<float, 2>);
   EVS_CUDA_TRY(evs_launch(kern, grid, dim3(APP_THREADS), 0, st, false, c, r, k, v, vec));
   evs_count_launch(1);
   return EVS_OK;
