@@ -49,7 +49,7 @@ def _need_cuda(t: torch.Tensor, what: str) -> None:
 # (current_stream() builds a Stream object, 2 us a call), device indices instead of torch.device objects, and
 # the C structs packed as bytes.
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch.cuda.current_device
+_current_device = torch._C._cuda_getDevice
 _fns: dict = {}
 _pack_rows = struct.Struct("@PPPqiii4x").pack  # evs_q4_rows
 _pack_strides = struct.Struct("@3q").pack

@@ -471,6 +471,17 @@ def test_attention_long_unaligned_queries_and_growing_scores(q4):
     assert torch.equal(out, q4.q4_attention(q.contiguous(), cache, table, i32([start])))
 
 
+def test_attention_long_sharp_scores(q4):
+    """One key takes nearly all the weight, at every place of a step."""
+    D, G, H, T, start = 128, 1, 4, 20, 4700
+    cache, table = make_rows(q4, [start + T], 64, G, D)
+    k, v = fill_cache(q4, cache, table, [start], [start + T], G, D)
+    q = randn(1, T, H, D, seed=5, dtype=BF) * 20
+    out = q4.q4_attention(q, cache, table, i32([start]), scale=0.5)
+    want, av, mag = R.attend(q[0], k[0].double(), v[0].double(), start, 0.5)
+    assert bool(((out[0].double() - want).abs() <= R.attend_bound(want, av, mag, start + T, D, BF)).all())
+
+
 def test_attention_long_nan_groups_and_bad_pages(q4):
     D, G, H, T, start = 128, 2, 24, 7, 4400
     cache, table = make_rows(q4, [start + T, start + T], 16, G, D)
