@@ -256,8 +256,10 @@ int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, 
 
 // 4-bit weights and KV cache
 constexpr int Q4_STATE_PAGE = 64;
+// pdl: launched ahead of its predecessor's end; wait_first: the weight may be an earlier kernel's, too
 int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void* codes, const void* scales, int N, int K,
-                     int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl);
+                     int group, void* out, int out_dtype, int64_t ldo, cudaStream_t st, bool pdl,
+                     bool wait_first = false);
 int launch_q4_decode(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
                      int64_t ldo, cudaStream_t st, bool pdl);
 int q4_check_weight(const void* codes, const void* scales, int N, int K, int group);

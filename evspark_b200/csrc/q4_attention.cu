@@ -794,7 +794,7 @@ int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG(in_place || !q4_share(to, n_heads, tq, n_heads, B, T, D, dtype == EVS_DTYPE_BF16 ? 2 : 4),
                 "q4 attention: out overlaps q");
   return launch_q4_attention(q4_cache_dev(cache), q4_rows_dev(rows), tq, to, n_heads, scale,
-                             bound_of(cache, rows, max_length), workspace, workspace_bytes, dtype, st, false);
+                             bound_of(cache, rows, max_length), workspace, workspace_bytes, dtype, st, true);
 }
 
 }  // extern "C"

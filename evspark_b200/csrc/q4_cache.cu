@@ -438,7 +438,7 @@ int launch_q4_read(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& k, c
   EVS_CHECK_ARG(grid.y <= 65535, "q4 read: too many heads");
   auto* kern = dtype == EVS_DTYPE_BF16 ? (few ? q4_read_kernel<__nv_bfloat16, 1> : q4_read_kernel<__nv_bfloat16, 2>)
                                        : (few ? q4_read_kernel<float, 1> : q4_read_kernel<float, 2>);
-  EVS_CUDA_TRY(evs_launch(kern, grid, dim3(APP_THREADS), 0, st, false, c, r, k, v, vec));
+  EVS_CUDA_TRY(evs_launch(kern, grid, dim3(APP_THREADS), 0, st, true, c, r, k, v, vec));
   evs_count_launch(1);
   return EVS_OK;
 }
@@ -472,7 +472,7 @@ int evs_q4_kv_append(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
                   "q4 append: q_out overlaps another tensor of the call");
   }
   return launch_q4_append(q4_cache_dev(cache), q4_rows_dev(rows), tq, tk, tv, to, q != nullptr ? n_heads : 0, dtype,
-                          rope_base, st, false);
+                          rope_base, st, true);
 }
 
 int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, void* k, const int64_t* k_strides, void* v,

@@ -634,3 +634,60 @@ def test_attention_long_in_graphs_and_on_two_streams_at_once(q4):
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
     cache.check()
+
+
+def test_captured_behind_copies_memsets_and_another_stream(q4):
+    """Every call of the module in one graph, each behind another kind of work: its inputs come from a copy, a
+    memset, a kernel of another stream, a kernel of its own stream and a call of the module."""
+    n, k, D, G, H = 512, 256, 64, 2, 4
+    w = q4.quantize_weight(randn(n, k, seed=1), 64)
+    host = torch.zeros(3, k).pin_memory()
+    x, y = torch.empty(3, k, device=DEV), torch.empty(3, n, device=DEV)
+    cache, table = make_rows(q4, [60], 16, G, D)
+    lengths = i32([50])
+    qkv = torch.empty(1, 4, (H + 2 * G) * D, device=DEV)
+    qkv_in = randn(1, 4, (H + 2 * G) * D, seed=2)
+    fill_cache(q4, cache, table, [0], [50], G, D, dtype=F32)
+    outs = [torch.zeros_like(y) for _ in range(3)]
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def run():
+        x.copy_(host, non_blocking=True)  # a copy
+        q4.q4_linear(x, w, out=outs[0])
+        x.zero_()  # a memset or a kernel
+        q4.q4_linear(x, w, out=outs[1])
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            x.fill_(0.5)
+            qkv.copy_(qkv_in * 2)
+        main.wait_stream(side)  # a join of two streams
+        q4.q4_linear(x, w, out=outs[2])
+        q, kk, v = (qkv[..., a * D:b * D].unflatten(-1, (-1, D)) for a, b in ((0, H), (H, H + G), (H + G, H + 2 * G)))
+        rot = q4.q4_kv_append(cache, table, lengths, kk, v, q=q)
+        att = q4.q4_attention(rot, cache, table, lengths)
+        with torch.cuda.stream(side):
+            side.wait_stream(main)
+            back = q4.q4_kv_read(cache, table, lengths, 4)
+        main.wait_stream(side)
+        return rot, att, *back
+
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        host.copy_(torch.randn(3, k, generator=torch.Generator().manual_seed(0)))
+        run()
+        main.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=main):
+            captured = run()
+        for seed in (1, 2, 3):
+            host.copy_(torch.randn(3, k, generator=torch.Generator().manual_seed(seed)))
+            qkv_in.copy_(randn(1, 4, (H + 2 * G) * D, seed=40 + seed))
+            graph.replay()
+            main.synchronize()
+            got = [t.clone() for t in (*outs, *captured)]
+            main.synchronize()
+            want = [*outs, *run()]
+            main.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
+            assert torch.equal(got[0], q4.q4_linear(host.to(DEV), w)) and not bool(got[1].any())
+    cache.check()
