@@ -7,8 +7,9 @@
 // depends on the row's own position alone (32 keys below 1,024, 64 below 4,096, 256 below 131,072, else
 // 1,024), so a token's result does not depend on what else is in the call: verify blocks and single
 // steps agree bit for bit.  (Calls of more than 64 rows a kv head leave positions from 4,096 on to
-// q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give few keys to many CTAs; from 131,072 keys on there are
-// enough of them, and longer ones spare partial results (440 us instead of 479 at 262,144 keys).
+// q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give
+// few keys to many CTAs; from 131,072 keys on there are enough of them, and longer ones spare partial
+// results (440 us instead of 479 at 262,144 keys).
 //
 // Keys and values are decoded in the registers that the products read them from, with no rounding
 // between codes and product.  What bounds it: about 1,000 warp instructions per 32 keys and row tile
@@ -465,8 +466,8 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
 // whether row b's token t is a token, and its position; a row that cannot be read (bad lengths, or beyond
 // the launch's slots) is set to NaN
 template <typename T, int DH>
-__device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDev& rows, int b, int t, int nslots, bool tcore,
-                                         T* dst, int* n) {
+__device__ __forceinline__ bool fold_row(const Q4CacheDev& cache, const Q4RowsDev& rows, int b, int t, int nslots,
+                                         bool tcore, T* dst, int* n) {
   const int lane = threadIdx.x & 31;
   int len, count;
   const bool ok = q4_row(rows, b, &len, &count, cache.P);

@@ -304,9 +304,10 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
       auto chunk_of = [&](int i, int sub, int* sl) {
         const int at = (4 * i + sub) & 31, id = __shfl_sync(0xffffffffu, page, at);
         *sl = __shfl_sync(0xffffffffu, slot, at);
-        const bool in = kbeg + i * TC_KEYS + 16 * sub < kend, ok = in && static_cast<uint32_t>(id) < static_cast<uint32_t>(cache.pages);
-        bad |= in && !ok;
-        return ok ? id : -1;
+        const bool in = kbeg + i * TC_KEYS + 16 * sub < kend;
+        const bool known = static_cast<uint32_t>(id) < static_cast<uint32_t>(cache.pages);
+        bad |= in && !known;
+        return in && known ? id : -1;
       };
       // keys: a thread takes 32 features c of key 32 p + 8 dw + lane % 8 (p: two passes); values: eight
       // features f8 of the eight keys from k8 on

@@ -370,7 +370,8 @@ __global__ void q4_quantize_kernel(const TW* __restrict__ w, int64_t ldw, int N,
   const uint32_t s = __any_sync(0xffffffffu, bad) ? 0x7FC0u : q4_scale_bits(static_cast<double>(m));
   uint32_t c[4];
   for (int j = 0; j < per; ++j) c[j] = q4_code(static_cast<double>(v[j]), s);
-  uint8_t* dst = codes + static_cast<size_t>(n) * (groups * static_cast<size_t>(group) / 2) + static_cast<size_t>(gi) * (group / 2);
+  uint8_t* dst = codes + static_cast<size_t>(n) * (groups * static_cast<size_t>(group) / 2) +
+                 static_cast<size_t>(gi) * (group / 2);
   if (per == 1) {
     const uint32_t other = __shfl_down_sync(0xffffffffu, c[0], 1);
     if ((lane & 1) == 0) dst[lane / 2] = static_cast<uint8_t>(c[0] | other << 4);

@@ -78,8 +78,9 @@ def attend_bound(out, av, mag, keys: int, D: int, dtype: torch.dtype) -> torch.T
     """A score is off by at most (3 D / 16 + 2) 2^-22 of its sum of magnitudes (fp32 product steps, the scale)
     and one rounding of its base-2 exponent (2^-23 of it); a weight exp2(s - m) by that (times ln 2 < 1,
     both s and m), by 2^-22 of the exponential and by its rounding as a product operand (bf16 queries: one
-    bf16 part, half a step of at most 2^-8 of the weight; fp32: three parts, 2^-24).  Sums over n keys add (n / 16 + 40) 2^-22 (product steps, folds).  Numerator and denominator
-    each move by that relative error: twice it, times sum p |v| / sum p; then one rounding to the type.
+    bf16 part, half a step of at most 2^-8 of the weight; fp32: three parts, 2^-24).  Sums over n keys add
+    (n / 16 + 40) 2^-22 (product steps, folds).  Numerator and denominator each move by that relative
+    error: twice it, times sum p |v| / sum p; then one rounding to the type.
     fp32 and bf16 hold nothing below 2^-126 at full precision: the second part of a weight under 2^-110
     of the largest (2^-8 of it, so under 2^-118) may be lost, and with it 2^-118 |v| of each of the n
     keys, |v| being at most 2^6 in these tests: the sum of the weights is at least the largest."""
