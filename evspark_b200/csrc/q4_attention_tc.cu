@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
             *reinterpret_cast<uint4*>(vst + tile_at<DH>(8 * f8 + 4 * h + e, k8 >> 3)) =
                 make_uint4(o[e][0], o[e][1], o[e][2], o[e][3]);
         }
-        fence_async_smem();  // also waits for loads on their way: one a step
+        fence_async_smem();  // the stores before the products
         __syncwarp();
         if (lane == 0) mbar_arrive(kv_full + n % STAGES);
         load(x, i + 2);
