@@ -12,9 +12,9 @@
 // results (440 us instead of 479 at 262,144 keys).
 //
 // Keys and values are decoded in the registers that the products read them from, with no rounding
-// between codes and product.  What bounds it: about 1,000 warp instructions per 32 keys and row tile
-// (384 the decode), 0.54 issued a clock and scheduler at 12 warps an SM.  bf16, 32 heads of 128, 13
-// tokens: 128 us at 65,536 keys (2.4 TB/s of codes and scales; floor 46 us), 411 us at 262,144 (2.9 TB/s).
+// between codes and product.  What bounds it: about 1,070 warp instructions per 32 keys and row tile
+// (384 the decode, 96 products) at 12 warps an SM.  bf16, 32 heads of 128, 13 tokens: 145 us at 65,536 keys
+// (2.1 TB/s of codes and scales; floor 46 us), 477 us at 262,144 (2.5 TB/s).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -47,11 +47,11 @@ __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
 }
 
 constexpr int qa_parts_q(size_t elem) { return elem == 2 ? 1 : 3; }  // bf16 parts of a query value
-// ... and of a probability.  One for bf16 queries: the weight of a key is then off by at most 2^-8 of
-// itself, beside outputs that are rounded by as much once more (relative error against 64 bits 1.7e-3
-// to 1.75e-3 at 1,024 keys); a second part cost a third of the products, 170 us instead of 154 at 64k
-// keys and 540 instead of 479 at 262k.  The sums of the weights take them unrounded.
-constexpr int qa_parts_p(size_t elem) { return elem == 2 ? 1 : 3; }
+// ... and of a probability.  Two for bf16 queries: a key's weight is then off by at most 2^-18 of itself (two
+// roundings to the nearest bf16, 2^-9 of what each is given), as in the attention over the bf16 cache.  One part
+// would be off by 2^-9, beside outputs that are rounded by as much once more, and take 130 us instead of 145 at
+// 65,536 keys (13 tokens, 32 heads of 128) and 414 instead of 477 at 262,144.
+constexpr int qa_parts_p(size_t elem) { return elem == 2 ? 2 : 3; }
 
 // The K codes and scales of 32 keys, as one thread multiplies them: per 16-key chunk two 8-key tiles,
 // of which it holds key 4 (g / 2) + g % 2 + 2 u, features c DH / 4 .. + DH / 4 - 1.

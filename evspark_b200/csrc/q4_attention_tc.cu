@@ -5,7 +5,7 @@
 // One CTA takes up to 128 query rows (a row is one token of one query head of the kv head) over its slot of
 // keys, 64 keys a step: S = Q K^T (128 x 64 x 128) and O += P V (128 x 128 x 64).  Four warps decode keys and
 // values into shared memory once for all rows; one warp issues whatever product is ready first; four warps run
-// the online softmax, one row a thread, with S, then P in S's place, and O in tensor memory.  Two stages of
+// the online softmax, one row a thread, with S, then P (two bf16 parts) in S's place, and O in tensor memory.  Two stages of
 // everything, so that a step's scores are there while the one before is still worked on; two CTAs an SM.
 //
 // Measured beside the 16-row mma.sync kernel, which decodes the keys once per 16 rows: 16 rows of 13 tokens,
@@ -80,6 +80,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 16-byte unit u of row r of an operand of ROWS rows, 128-byte swizzle
@@ -89,7 +94,7 @@ __device__ __forceinline__ uint32_t tile_at(int r, int u) {
 }
 
 // One step of the online softmax of a row (its thread's lane): the scores at tm -> probabilities in their
-// place, the outputs so far (at to) moved to a new reference once complete() says that they are complete.  Keys
+// place (the upper parts, then the lower ones), the outputs so far (at to) moved to a new reference once complete() says that they are complete.  Keys
 // from seen on are masked.
 template <bool MASKED, typename F>
 __device__ __forceinline__ void softmax_step(uint32_t tm, uint32_t to, float scale_log2, int seen, float& m, float& l,
@@ -129,18 +134,21 @@ __device__ __forceinline__ void softmax_step(uint32_t tm, uint32_t to, float sca
   const float mu = m == -CUDART_INF_F ? 0.f : -m * scale_log2;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int c0 = 0; c0 < TC_KEYS; c0 += 32) {
-    uint32_t w[16];
+  for (int c0 = 0; c0 < TC_KEYS; c0 += 16) {
+    uint32_t w[8], low[8];  // a weight in two bf16 parts: off by at most 2^-18 of itself
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      const float p0 = qa_ex2(fmaf(s[(c0 + j) >> 4][j & 15], scale_log2, mu));
-      const float p1 = qa_ex2(fmaf(s[(c0 + j) >> 4][(j & 15) + 1], scale_log2, mu));
+    for (int j = 0; j < 16; j += 2) {
+      const float p0 = qa_ex2(fmaf(s[c0 >> 4][j], scale_log2, mu));
+      const float p1 = qa_ex2(fmaf(s[c0 >> 4][j + 1], scale_log2, mu));
       sum[j & 2] += p0;
       sum[(j & 2) + 1] += p1;
       const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
       w[j >> 1] = *reinterpret_cast<const uint32_t*>(&h);
+      const __nv_bfloat162 r = __floats2bfloat162_rn(p0 - __low2float(h), p1 - __high2float(h));
+      low[j >> 1] = *reinterpret_cast<const uint32_t*>(&r);
     }
-    tmem_st_32x32b_x16(tm + c0 / 2, w);
+    tmem_st_32x32b_x8(tm + c0 / 2, w);
+    tmem_st_32x32b_x8(tm + TC_KEYS / 2 + c0 / 2, low);
   }
   l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   tmem_st_wait();
@@ -448,7 +456,10 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
           tc_fence_after();
           const uint32_t st = (it + pv) % STAGES, p = tmem + st * TC_KEYS, v = v0 + st * (KV_BYTES >> 4);
 #pragma unroll
-          for (int j = 0; j < TC_KEYS / 16; ++j) mma_ts(on, tmem_o, p + 8 * j, v + 2 * j, high, O_DESC, pv != 0 || j != 0);
+          for (int j = 0; j < TC_KEYS / 16; ++j) {
+            mma_ts(on, tmem_o, p + TC_KEYS / 2 + 8 * j, v + 2 * j, high, O_DESC, pv != 0 || j != 0);
+            mma_ts(on, tmem_o, p + 8 * j, v + 2 * j, high, O_DESC, 1);
+          }
           mma_commit(on, smem_u32(pv_done) + 8 * st);
           ++pv, idle = 0;
         } else if ((++idle & 255) == 0) {
