@@ -906,13 +906,13 @@ int launch_attention_t(const evs_model* m, evs_state* s, int layer, int B, int T
 
 }  // namespace
 
-int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int kv_blocks,
+int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int kv_blocks, bool prefill,
                      cudaStream_t st) {
   // P.V gives each thread two head columns and at most PV_QMAX of the QT queries of a pass
   EVS_CHECK_ARG(m->cfg.head_dim >= 32 && m->cfg.head_dim <= 128 && 256 % m->cfg.head_dim == 0,
                 "head_dim must be 32, 64 or 128");
   EVS_CHECK_RANGE(kv_blocks >= 1 && kv_blocks <= s->attn_blocks, "KV length beyond max_seqlen");
-  if (s->kv_q4) return launch_attention_q4(m, s, layer, B, T, splits, kv_blocks * ATTN_BLOCK, st);
+  if (s->kv_q4) return launch_attention_q4(m, s, layer, B, T, splits, kv_blocks * ATTN_BLOCK, prefill, st);
   if (m->cfg.dtype == EVS_DTYPE_BF16) return launch_attention_t<__nv_bfloat16>(m, s, layer, B, T, splits, kv_blocks, st);
   return launch_attention_t<float>(m, s, layer, B, T, splits, kv_blocks, st);
 }

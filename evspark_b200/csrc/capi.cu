@@ -193,7 +193,9 @@ int run_forward(const evs_model* m, evs_state* s, const int64_t* ids, int B, int
       EVS_TRY(G(&L.tm_qkv, nullptr, L.w_qkv, nullptr, 3 * dl, d, 0, nullptr, 0, nullptr, q4_of(EVS_W_QKV)));
       const double kv_el = s->kv_q4 ? 0.5 + 2.0 / 32 : el;
       const double kv_bytes = 2.0 * B * (maxlen + T) * H * Dh * kv_el + 4.0 * sp * M * 3 * dl + 2.0 * M * dl * el;
-      EVS_TRY(timed(s, st, EVS_PROF_ATTN, kv_bytes, [&] { return launch_attention(m, s, i, B, T, sp, kv_blocks, st); }));
+      EVS_TRY(timed(s, st, EVS_PROF_ATTN, kv_bytes, [&] {
+        return launch_attention(m, s, i, B, T, sp, kv_blocks, prefill != 0, st);
+      }));
       EVS_TRY(RP(&L.tm_o, L.w_o, dl, nullptr, q4_of(EVS_W_O)));
     } else {
       EVS_TRY(G(&L.tm_in, nullptr, L.w_in, nullptr, 3 * dl, d, 0, nullptr, 0, nullptr, q4_of(EVS_W_IN)));

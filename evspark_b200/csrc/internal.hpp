@@ -251,7 +251,7 @@ int launch_rollback(evs_state* s, const int32_t* k, int B, cudaStream_t st);
 int launch_state_export(const evs_state* s, int layer, int which, int row, int width, void* dst, cudaStream_t st);
 
 // attention: rope + KV append + split-KV partials + ordered combine (output into s->act)
-int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int kv_blocks,
+int launch_attention(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int kv_blocks, bool prefill,
                      cudaStream_t st);
 
 // 4-bit weights and KV cache
@@ -263,8 +263,10 @@ int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void*
 int launch_q4_decode(const void* codes, const void* scales, int N, int K, int group, void* out, int out_dtype,
                      int64_t ldo, cudaStream_t st, bool pdl);
 int q4_check_weight(const void* codes, const void* scales, int N, int K, int group);
-// rope + append into the 4-bit pages + attention over them (output into s->act); bound >= lengths + T
-int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound,
+// rope + append into the 4-bit pages + attention over them (output into s->act); bound >= lengths + T.
+// Positions from 4,096 on: prompts on the tensor-core kernel, every other forward on that of few rows, whatever T, so
+// that a state depends neither on the chunks of its prompt nor on the blocks behind it.
+int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound, bool prefill,
                         cudaStream_t st);
 int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound);
 int launch_q4_state_read(const evs_state* s, int layer, int row, int width, void* dst, cudaStream_t st);

@@ -6,8 +6,8 @@
 // folded in order, and a second kernel folds the CTAs' partial results in order.  The unit's length
 // depends on the row's own position alone (32 keys below 1,024, 64 below 4,096, 256 below 131,072, else
 // 1,024), so a token's result does not depend on what else is in the call: verify blocks and single
-// steps agree bit for bit.  (Calls of more than 64 rows a kv head leave positions from 4,096 on to
-// q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give
+// steps agree bit for bit.  (Calls of more than 64 rows a kv head, and a model's prompts, leave positions from
+// 4,096 on to q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give
 // few keys to many CTAs; from 131,072 keys on there are enough of them, and longer ones spare partial
 // results (440 us instead of 479 at 262,144 keys).
 //
@@ -606,7 +606,7 @@ inline bool fused_fits(int nslots, int64_t T, int grp, int G) {
 
 template <typename T, int DH>
 int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& out, int H, float scale,
-                int64_t bound, float* ws, int64_t ws_floats, cudaStream_t st, bool pdl) {
+                int64_t bound, QaLong longs, float* ws, int64_t ws_floats, cudaStream_t st, bool pdl) {
   const int grp = H / c.G;
   const float scale_log2 = scale * 1.4426950408889634f;
   const int q_vec = q4_vec(q, sizeof(T));
@@ -641,9 +641,9 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
   // From 65 rows a kv head on the tensor-core kernel takes the long positions: it wins from 39 rows on (151 us
   // instead of 183 at 32,768 keys, 32 kv heads; 26 rows: 257 instead of 242), but blocks of up to 64 tokens
-  // keep the sums of single steps.
-  const bool tcore = sizeof(T) == 2 && DH == 128 && static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS &&
-                     bound > QA_TC_BEGIN;
+  // keep the sums of single steps.  A model says which kernel, as its rule must not depend on a call's tokens.
+  const bool many = longs == QaLong::BY_ROWS ? static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS : longs == QaLong::TENSOR_CORE;
+  const bool tcore = sizeof(T) == 2 && DH == 128 && many && bound > QA_TC_BEGIN;
   const int nslots = tcore ? qa_tc_slots(bound) : qa_slots(bound);
   // tokens per pass: as many as the workspace holds partial results for
   const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
@@ -681,9 +681,10 @@ int64_t bound_of(const evs_q4_cache* c, const evs_q4_rows* r, int max_length) {
 }  // namespace
 
 int launch_q4_attention(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, const Q4Tensor& out, int H,
-                        float scale, int64_t bound, void* ws, int64_t ws_bytes, int dtype, cudaStream_t st, bool pdl) {
+                        float scale, int64_t bound, QaLong longs, void* ws, int64_t ws_bytes, int dtype, cudaStream_t st,
+                        bool pdl) {
 #define QA_GO(T, DH) \
-  return launch_attn<T, DH>(c, r, q, out, H, scale, bound, static_cast<float*>(ws), ws_bytes / 4, st, pdl)
+  return launch_attn<T, DH>(c, r, q, out, H, scale, bound, longs, static_cast<float*>(ws), ws_bytes / 4, st, pdl)
   if (dtype == EVS_DTYPE_BF16) {
     if (c.D == 32) QA_GO(__nv_bfloat16, 32);
     if (c.D == 64) QA_GO(__nv_bfloat16, 64);
@@ -729,7 +730,7 @@ Q4CacheDev state_cache(const evs_state* s, int layer) {
 }
 }  // namespace
 
-int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound,
+int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int T, int splits, int bound, bool prefill,
                         cudaStream_t st) {
   const int d = m->dl, H = m->Hl, D = m->cfg.head_dim, dtype = m->cfg.dtype;
   const bool pdl = s->use_pdl();
@@ -750,7 +751,8 @@ int launch_attention_q4(const evs_model* m, evs_state* s, int layer, int B, int 
   const Q4Tensor qr{s->qrot, static_cast<int64_t>(T) * d, d, D};
   const Q4Tensor out{s->act, static_cast<int64_t>(T) * s->ld_act, s->ld_act, D};
   EVS_TRY(launch_q4_append(c, r, q, k, v, qr, H, dtype, m->cfg.rope_base, st, pdl));
-  return launch_q4_attention(c, r, qr, out, H, 1.f / std::sqrt(static_cast<float>(D)), bound, s->attn_part,
+  return launch_q4_attention(c, r, qr, out, H, 1.f / std::sqrt(static_cast<float>(D)), bound,
+                             prefill ? QaLong::TENSOR_CORE : QaLong::ROW_TILES, s->attn_part,
                              static_cast<int64_t>(s->attn_part_bytes), dtype, st, pdl);
 }
 
@@ -795,7 +797,8 @@ int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const v
   EVS_CHECK_ARG(in_place || !q4_share(to, n_heads, tq, n_heads, B, T, D, dtype == EVS_DTYPE_BF16 ? 2 : 4),
                 "q4 attention: out overlaps q");
   return launch_q4_attention(q4_cache_dev(cache), q4_rows_dev(rows), tq, to, n_heads, scale,
-                             bound_of(cache, rows, max_length), workspace, workspace_bytes, dtype, st, true);
+                             bound_of(cache, rows, max_length), QaLong::BY_ROWS, workspace, workspace_bytes, dtype, st,
+                             true);
 }
 
 }  // extern "C"

@@ -19,6 +19,8 @@ __host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (
 // keys (64 / 8 heads) 2,076 instead of 2,640.
 constexpr int QA_FEW_ROWS = 64;
 constexpr int QA_TC_BEGIN = 4096;
+// Which kernel takes them: as the call's rows say, or one of the two whatever the rows.
+enum class QaLong { BY_ROWS, ROW_TILES, TENSOR_CORE };
 constexpr int QA_TC_CLASSES = 3;
 __host__ __device__ constexpr int qa_tc_class(int64_t pos) { return pos < 16384 ? 0 : (pos < 65536 ? 1 : 2); }
 __host__ __device__ constexpr int qa_tc_class_begin(int cl) { return cl == 0 ? QA_TC_BEGIN : (cl == 1 ? 16384 : 65536); }

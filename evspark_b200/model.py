@@ -90,9 +90,10 @@ class TargetModel:
         ``kv_format="q4"`` makes states with the KV cache in 4 bits (``evspark_b200.q4``).  Both change the
         model's numbers; greedy speculative decoding still equals native decoding.  With 4-bit weights a
         prompt is prefilled on the weights decoded for it (the same held values, summed as the bf16
-        projections sum), and over a 4-bit cache forwards of more than 64 tokens attend with other sums from
-        position 4,096 on (bf16, head_dim 128), so a token's rounding differs between prefill and later
-        forwards of few tokens."""
+        projections sum), and over a 4-bit cache a prompt's positions from 4,096 on attend with other sums
+        than those of later forwards (bf16, head_dim 128).  So a token's rounding differs between prefill and
+        the forwards behind it; it depends neither on how the prompt is cut into chunks nor on how later
+        tokens are grouped into forwards."""
         check_formats(weight_format, weight_group, kv_format, tp)
         self.device = require_device(device)
         self.weight_format, self.kv_format = weight_format, kv_format

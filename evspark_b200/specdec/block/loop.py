@@ -490,7 +490,7 @@ def speculative_generate(model, draft, prompt_ids, n_tokens: int, gamma: int, gr
 
 def _native_prefill(model, prompt: torch.Tensor, ip) -> torch.Tensor:
     """Consume the prompt, return its last token's logits.  A model with 4-bit weights decodes them for the
-    prompt's projections, and attention over a 4-bit cache has another kernel for long chunks (other sums than a
+    prompt's projections, and attention over a 4-bit cache has another kernel for long prompts (other sums than a
     step's, so other roundings): the last prompt token goes through a step, as it goes through the first verify
     block of the speculative loop, and the two stay equal."""
     low_bit = getattr(model, "weight_format", None) is not None or getattr(model, "kv_format", None) is not None
