@@ -23,6 +23,14 @@ constexpr float Q4_HUGE = 1.329227995784916e36f;  // 2^120
 constexpr int Q4_KV_GROUP = 32;                   // values per scale of the KV cache (along head_dim)
 constexpr int Q4_KBLOCK = 128;                    // weights: input features are padded to a multiple of this
 
+// Weights, codes, scales, page ids and partial results may be written by a kernel that still runs when their reader
+// starts (programmatic launches): readers load them by ordinary loads behind pdl_wait(), never by the read-only path,
+// which asks for data that nothing writes while the kernel lives.  So no __ldg, and no restrict on such inputs.
+template <typename V>
+__device__ __forceinline__ V q4_ld(const void* p) {
+  return *reinterpret_cast<const V*>(p);
+}
+
 // fma of bf16 pairs
 __device__ __forceinline__ uint32_t q4_fma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;

@@ -36,13 +36,13 @@ constexpr int QA_STEP = 16 * NS;
 template <int NW>
 __device__ __forceinline__ void ld_words(uint32_t (&w)[NW], const uint8_t* p) {
   if constexpr (NW == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint4 v = q4_ld<uint4>(p);
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if constexpr (NW == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    const uint2 v = q4_ld<uint2>(p);
     w[0] = v.x, w[1] = v.y;
   } else {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    w[0] = q4_ld<uint32_t>(p);
   }
 }
 
@@ -166,7 +166,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
     int page_of = -1;
     auto load_pages = [&](int key) {
       const int kk = key + 16 * lane;
-      page_of = kk < kend ? __ldg(table + kk / P) : -1;
+      page_of = kk < kend ? table[kk / P] : -1;
     };
     auto page_at = [&](int key, int sub) { return __shfl_sync(0xffffffffu, page_of, (((key - kbeg) >> 4) + sub) & 31); };
     KTile<DH> kt;
@@ -185,7 +185,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             ld_words<KW>(kt.w[sub][u], blk + (k_off + (slot[sub] + 2 * u) * (DH / 2)));
-            kt.s[sub][u] = __ldg(reinterpret_cast<const uint16_t*>(blk + (ks_off + 2 * (slot[sub] + 2 * u))));
+            kt.s[sub][u] = q4_ld<uint16_t>(blk + (ks_off + 2 * (slot[sub] + 2 * u)));
           }
         } else {
           bad |= in;
@@ -208,11 +208,11 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
           for (int j = 0; j < 4; ++j) {
             const uint8_t* p = blk + (v_off + (slot[sub] + j) * (DH / 2));
             if constexpr (DH == 32)
-              vt.w[sub][j][0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+              vt.w[sub][j][0] = q4_ld<uint16_t>(p);
             else
               ld_words<VTile<DH>::NW>(vt.w[sub][j], p);
           }
-          const uint2 s = __ldg(reinterpret_cast<const uint2*>(blk + (vs_off + 2 * slot[sub])));
+          const uint2 s = q4_ld<uint2>(blk + (vs_off + 2 * slot[sub]));
           vt.s[sub][0] = s.x, vt.s[sub][1] = s.y;
         } else {
 #pragma unroll
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(QA_THREADS, sizeof(T) == 2 ? 3 : 2)
 template <typename T, int DH>
 __global__ void __launch_bounds__(QA_THREADS)
     q4_combine_kernel(Q4CacheDev cache, Q4RowsDev rows, Q4Tensor out, int grp, int t0, int prows, int nslots,
-                      int tcore, const float* __restrict__ part_o, const float2* __restrict__ part_s) {
+                      int tcore, const float* part_o, const float2* part_s) {
   __shared__ float fold[QA_WARPS][DH + 1];
   pdl_trigger();
   pdl_wait();
@@ -709,8 +709,7 @@ int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound) {
 namespace {
 // qkv projection: partial sums [splits][M][3d] -> data dtype [M][3d]
 template <typename TD>
-__global__ void __launch_bounds__(256) qkv_collect_kernel(const float* __restrict__ ws, int splits, size_t n,
-                                                          TD* __restrict__ out) {
+__global__ void __launch_bounds__(256) qkv_collect_kernel(const float* ws, int splits, size_t n, TD* out) {
   pdl_trigger();
   pdl_wait();
   const size_t i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4;

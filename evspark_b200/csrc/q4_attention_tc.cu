@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
         if (kk < kend) {
           const int n = kk / P;
           slot_next = kk - n * P;
-          page_next = __ldg(table + n);
+          page_next = table[n];
         }
       };
       // chunk sub of step i: whether its page is one of the pool, and its slot
@@ -340,8 +340,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
           x.ksc[p] = 0x7FC0u;  // keys without a page: a NaN score for whoever sees them
           if (id >= 0) {
             const uint8_t* blk = head_base + id * page_bytes;
-            x.kw[p] = __ldg(reinterpret_cast<const uint4*>(blk + sl * (DH / 2) + c * 16));
-            x.ksc[p] = __ldg(reinterpret_cast<const uint16_t*>(blk + P * DH) + c * P + sl);
+            x.kw[p] = q4_ld<uint4>(blk + sl * (DH / 2) + c * 16);
+            x.ksc[p] = q4_ld<uint16_t>(blk + P * DH + 2 * (c * P + sl));
           }
         }
         int sl;
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(TC_THREADS, 2)
           const uint8_t* blk = head_base + id * page_bytes;
           const uint8_t* at = blk + P * (DH / 2) + sl * (DH / 2) + f8 * 4;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x.vw[j] = __ldg(reinterpret_cast<const uint32_t*>(at + j * (DH / 2)));
-          x.vsc = __ldg(reinterpret_cast<const uint4*>(blk + P * DH + P * (DH / 16) + 2 * ((f8 >> 2) * P + sl)));
+          for (int j = 0; j < 8; ++j) x.vw[j] = q4_ld<uint32_t>(at + j * (DH / 2));
+          x.vsc = q4_ld<uint4>(blk + P * DH + P * (DH / 16) + 2 * ((f8 >> 2) * P + sl));
         }
       };
       auto decode = [&](Raw& x, int i) {

@@ -284,10 +284,9 @@ __global__ void __launch_bounds__(APP_THREADS)
         if (i >= units || page[x] < 0) continue;
         const bool is_v = row >= G;
         const uint8_t* block = cache.block(page[x], is_v ? row - G : row);
-        codes[x][u] = __ldg(
-            reinterpret_cast<const uint32_t*>(block + (is_v ? cache.P * (D / 2) : 0) + slot[x] * (D / 2) + 4 * w));
-        sb[x][u] = __ldg(reinterpret_cast<const uint16_t*>(block + cache.P * D) + (is_v ? cache.P * (D / 32) : 0) +
-                         (w >> 2) * cache.P + slot[x]);
+        codes[x][u] = q4_ld<uint32_t>(block + (is_v ? cache.P * (D / 2) : 0) + slot[x] * (D / 2) + 4 * w);
+        sb[x][u] = q4_ld<uint16_t>(block + cache.P * D +
+                                   2 * ((is_v ? cache.P * (D / 32) : 0) + (w >> 2) * cache.P + slot[x]));
       }
 #pragma unroll
     for (int x = 0; x < TOK; ++x)

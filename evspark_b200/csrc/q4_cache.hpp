@@ -81,7 +81,7 @@ __device__ __forceinline__ bool q4_row(const Q4RowsDev& r, int b, int* len, int*
 
 // page of position pos (inside the table), or -1 when the table's entry is no page of the pool
 __device__ __forceinline__ int64_t q4_page(const Q4CacheDev& c, const Q4RowsDev& r, int b, int64_t pos) {
-  const int32_t id = __ldg(r.table + b * r.table_stride + pos / c.P);
+  const int32_t id = r.table[b * r.table_stride + pos / c.P];
   return id >= 0 && id < c.pages ? id : -1;
 }
 

@@ -33,7 +33,7 @@ __device__ __forceinline__ uint4 pair_up(uint4 v) {
 }
 
 template <typename TX, int NT>
-__device__ __forceinline__ void stage_x(uint4* xs, const TX* __restrict__ x, int64_t ldx, int M, int K, int m0, int kb0,
+__device__ __forceinline__ void stage_x(uint4* xs, const TX* x, int64_t ldx, int M, int K, int m0, int kb0,
                                         int nkb, bool vec) {
   constexpr int NP = sizeof(TX) == 2 ? 1 : 3, NR = NP == 1 ? 1 : 2;
   constexpr int TPB = LIN_THREADS / 16;                   // tokens that the CTA loads at once
@@ -87,12 +87,13 @@ struct LinTile {  // one warp's share of a K block: 32 rows x 128 features
   uint32_t s[4];
 };
 
-// the weight streams through once: no space in L1
+// the weight streams through once: no space in L1 (volatile, so that it stays behind the wait)
 __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
+               : "l"(p)
+               : "memory");
   return v;
 }
 
@@ -106,9 +107,8 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
 // while one is multiplied; the first ones are on their way before x is staged.
 template <typename TX, typename TO, int NT, int KW>
 __global__ void __launch_bounds__(LIN_THREADS, lin_per_sm<TX, NT>())
-    q4_linear_kernel(const TX* __restrict__ x, int64_t ldx, int M, const uint8_t* __restrict__ codes,
-                     const uint16_t* __restrict__ scales, int N, int K, int group_shift, TO* __restrict__ out,
-                     int64_t ldo, int chunk_kb, int vec, int wait_first, uint32_t red_offset) {
+    q4_linear_kernel(const TX* x, int64_t ldx, int M, const uint8_t* codes, const uint16_t* scales, int N, int K,
+                     int group_shift, TO* out, int64_t ldo, int chunk_kb, int vec, int wait_first, uint32_t red_offset) {
   constexpr int NP = sizeof(TX) == 2 ? 1 : 3;
   constexpr int LIN_ROWS = 32 * LIN_WARPS / KW, LIN_KW = KW;
   extern __shared__ __align__(16) unsigned char lin_sm[];
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(LIN_THREADS, lin_per_sm<TX, NT>())
 #pragma unroll
     for (int i = 0; i < 4; ++i) t.w[i] = ld_stream(base + (off[i] + static_cast<uint32_t>(kb) * (Q4_KBLOCK / 2)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.s[i] = __ldg(reinterpret_cast<const uint16_t*>(sbase + (soff[i] + so)));
+    for (int i = 0; i < 4; ++i) t.s[i] = q4_ld<uint16_t>(sbase + (soff[i] + so));
   };
 
   float acc[2][NT][4];
@@ -384,8 +384,8 @@ __global__ void q4_quantize_kernel(const TW* __restrict__ w, int64_t ldw, int N,
 // one thread per 16 codes of a row: 16 values
 template <typename TO>
 __global__ void __launch_bounds__(256)
-    q4_decode_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict__ scales, int N, int K,
-                     int group_shift, TO* __restrict__ out, int64_t ldo, int vec) {
+    q4_decode_kernel(const uint8_t* codes, const uint16_t* scales, int N, int K, int group_shift, TO* out,
+                     int64_t ldo, int vec) {
   pdl_trigger();
   pdl_wait();
   const int units = (K + 15) / 16;
@@ -393,9 +393,8 @@ __global__ void __launch_bounds__(256)
   if (i >= static_cast<int64_t>(N) * units) return;
   const int n = static_cast<int>(i / units), k = static_cast<int>(i - static_cast<int64_t>(n) * units) * 16;
   const size_t row_bytes = static_cast<size_t>((K + Q4_KBLOCK - 1) / Q4_KBLOCK) * (Q4_KBLOCK / 2);
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(codes + n * row_bytes + k / 2));
-  const float s =
-      __uint_as_float(static_cast<uint32_t>(__ldg(scales + static_cast<size_t>(k >> group_shift) * N + n)) << 16);
+  const uint2 w = q4_ld<uint2>(codes + n * row_bytes + k / 2);
+  const float s = __uint_as_float(static_cast<uint32_t>(scales[static_cast<size_t>(k >> group_shift) * N + n]) << 16);
   float v[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) v[j] = (static_cast<int>(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u) - 8) * s;

@@ -1,0 +1,35 @@
+"""CPU: what the 4-bit kernels and calls promise and no device run can show."""
+
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+CSRC = Path(__file__).resolve().parents[1] / "evspark_b200" / "csrc"
+
+
+def kernels(source: str):
+    """(name, parameters, body) of the kernels of a source file."""
+    for m in re.finditer(r"__global__ void\s*(?:__launch_bounds__\([^{;]*?\)\s*)?(\w+)\(", source):
+        depth, at = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(source[at], 0)
+            at += 1
+        end = source.index("\n}\n", at)
+        yield m.group(1), source[m.end():at - 1], source[at:end]
+
+
+def test_kernels_that_start_early_read_by_ordinary_loads():
+    """A kernel that waits for its predecessor while it runs must not ask for data that stay unwritten for its whole
+    life: no read-only loads, no restrict on an input, and no load that the compiler may move above the wait."""
+    early = 0
+    for path in sorted(CSRC.glob("q4*")):
+        source = re.sub(r"//[^\n]*", "", path.read_text())
+        assert "__ldg" not in source and ".nc." not in source, path.name
+        for asm in re.findall(r"asm(?: volatile)?\(\s*\"ld\.global.*?\);", source, re.S):
+            assert asm.startswith("asm volatile") and '"memory"' in asm, (path.name, asm)
+        for name, params, body in kernels(source):
+            if "pdl_wait" in body:
+                early += 1
+                assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", params), (path.name, name)
+    assert early >= 8
