@@ -233,7 +233,9 @@ class Q4Cache:
         return self.pool.device
 
     def check(self) -> None:
-        """Raise if a call since the last ``check`` met a bad length or page id (waits for the device)."""
+        """Raise if a call since the last ``check`` met a bad length or page id, on whatever stream it ran (waits
+        for the device)."""
+        torch.cuda.synchronize(self._index)
         code, where, info = self._err.tolist()
         if code:
             self._err.zero_()

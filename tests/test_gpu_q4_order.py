@@ -57,3 +57,20 @@ def test_decode_steps_behind_each_other(q4, start, H, G, D, dtype):  # noqa: F81
     kk, vv = q4.q4_kv_read(cache, table, at[0], steps)
     assert torch.equal(torch.cat([r[0] for r in read], 1), kk) and torch.equal(torch.cat([r[1] for r in read], 1), vv)
     cache.check()
+
+
+def test_check_sees_calls_of_other_streams(q4):  # noqa: F811
+    """A bad page met on another stream, behind work that is still running when check is called."""
+    cache, table = make_rows(q4, [40], 16, 1, 64)
+    q, at = randn(1, 1, 1, 64, seed=1), i32([20])
+    bad = torch.full_like(table, cache.num_pages)
+    side = torch.cuda.Stream()
+    q4.q4_attention(q, cache, table, at)  # the kernel is loaded: its first call may wait for the device
+    torch.cuda._sleep(1000)
+    cache.check()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+        q4.q4_attention(q, cache, bad, at)
+    with pytest.raises(RuntimeError, match="page table|pool"):
+        cache.check()
+    cache.check()  # read once
