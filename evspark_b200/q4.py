@@ -69,6 +69,15 @@ def _call(index: int, name: str, *args) -> None:
         N.check(status, name)
 
 
+# Sizes that the library takes.  Checked here, as they go to it as 32-bit integers, which would wrap.
+_MOST = 2 ** 31 - 1
+
+
+def _check_weight_size(n: int, k: int, what: str) -> None:
+    if n > _MOST or k > 2 ** 24 or n * k > 2 ** 35:
+        raise ValueError(f"{what}: at most 2^31 - 1 rows, 2^24 features and 2^35 values, got [{n}, {k}]")
+
+
 def padded_features(k: int) -> int:
     return -(-k // KBLOCK) * KBLOCK
 
@@ -82,6 +91,7 @@ class Q4Weight:
         n, k = int(shape[0]), int(shape[1])
         if n < 1 or k < 1:
             raise ValueError(f"Q4Weight: shape must be at least [1, 1], got {tuple(shape)}")
+        _check_weight_size(n, k, "Q4Weight")
         if group not in (32, 64, 128):
             raise ValueError(f"Q4Weight: group must be 32, 64 or 128, got {group}")
         kp = padded_features(k)
@@ -122,6 +132,7 @@ def quantize_weight(w: torch.Tensor, group: int = 64) -> Q4Weight:
     """A weight [N, K] (bf16 or fp32; rows may be strided) -> ``Q4Weight``."""
     if w.dim() != 2 or w.numel() == 0:
         raise ValueError(f"quantize_weight: w must be a non-empty [N, K] matrix, got {tuple(w.shape)}")
+    _check_weight_size(*w.shape, "quantize_weight")
     if group not in (32, 64, 128):
         raise ValueError(f"quantize_weight: group must be 32, 64 or 128, got {group}")
     dt = _dtype(w, "quantize_weight: w")
@@ -153,6 +164,9 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
         raise ValueError(f"q4_linear: x must be [..., {k}], got {tuple(shape)}")
     if x.get_device() != w._index:
         raise ValueError(f"q4_linear: x on {x.device}, the weight on {w.codes.device}")
+    m = x.numel() // k
+    if m > _MOST:
+        raise ValueError(f"q4_linear: too many rows ({m})")
     if out is not None:
         if out.shape != shape[:-1] + (n,) or out.get_device() != w._index or not out.is_contiguous():
             raise ValueError(f"q4_linear: out must be a contiguous [..., {n}] tensor of x's batch shape and device")
@@ -162,7 +176,6 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
         if odt is None:
             raise ValueError(f"q4_linear: out_dtype must be bf16 or fp32, got {out_dtype}")
         out = x.new_empty(shape[:-1] + (n,), dtype=out_dtype)
-    m = x.numel() // k
     if m == 0:
         return out
     ldx = k
@@ -261,7 +274,7 @@ def _rows(cache: Q4Cache, page_table, lengths, counts, batch: int, tokens: int, 
             raise ValueError(f"{what}: counts must be a contiguous int32 [{batch}] tensor on {cache.pool.device}")
         cp = counts.data_ptr()
     mp = shape[1]
-    if batch > 2 ** 31 - 1 or tokens > 2 ** 31 - 1 or mp > 2 ** 31 - 1:
+    if batch > _MOST or tokens > _MOST or mp > _MOST:
         raise ValueError(f"{what}: too large a call")
     return _pack_rows(page_table.data_ptr(), lengths.data_ptr(), cp, max(strides[0], mp), mp, batch, tokens), \
         mp * cache.page_size
@@ -306,8 +319,8 @@ def q4_kv_append(cache: Q4Cache, page_table: torch.Tensor, lengths: torch.Tensor
             q_out = q.new_empty(shape)
         qos = _heads(q_out, shape, dtype, index, "q4_kv_append: q_out")
         qp, qop = q.data_ptr(), q_out.data_ptr()
-        if H < 1:
-            raise ValueError("q4_kv_append: q needs at least one head")
+        if not 1 <= H <= _MOST:
+            raise ValueError(f"q4_kv_append: q needs between one and 2^31 - 1 heads, got {H}")
     elif q_out is not None:
         raise ValueError("q4_kv_append: q_out without q")
     if B == 0 or T == 0:
@@ -362,7 +375,7 @@ def q4_attention(q: torch.Tensor, cache: Q4Cache, page_table: torch.Tensor, leng
         raise ValueError(f"q4_attention: q must be [B, T, heads, D], got {tuple(q.shape)}")
     B, T, H, _ = q.shape
     dt, index = _dtype(q, "q4_attention: q"), cache._index
-    if H < 1 or H % cache.kv_heads:
+    if not 1 <= H <= _MOST or H % cache.kv_heads:
         raise ValueError(f"q4_attention: heads ({H}) must be a multiple of kv_heads ({cache.kv_heads})")
     shape = (B, T, H, cache.head_dim)
     qs = _heads(q, shape, q.dtype, index, "q4_attention: q")

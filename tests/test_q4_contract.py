@@ -5,6 +5,12 @@ from __future__ import annotations
 import re
 from pathlib import Path
 
+import pytest
+import torch
+
+from evspark_b200 import q4
+from tests.test_q4 import cache, weight
+
 CSRC = Path(__file__).resolve().parents[1] / "evspark_b200" / "csrc"
 
 
@@ -33,3 +39,24 @@ def test_kernels_that_start_early_read_by_ordinary_loads():
                 early += 1
                 assert not re.search(r"const\s+\w+\s*\*\s*__restrict__", params), (path.name, name)
     assert early >= 8
+
+
+@pytest.mark.parametrize("n,k", [(2 ** 31, 1), (2 ** 32 + 5, 1), (1, 2 ** 24 + 1), (1, 2 ** 32 + 5), (2 ** 20, 2 ** 16)])
+def test_sizes_beyond_32_bits_are_refused(n, k):
+    """Sizes go to the library as 32-bit integers: 2^32 + 5 rows must not come out as five."""
+    with pytest.raises(ValueError, match="at most"):
+        q4.quantize_weight(torch.zeros(1, 1).expand(n, k), 32)
+    with pytest.raises(ValueError, match="at most"):
+        q4.Q4Weight(torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.bfloat16), (n, k), 32)
+
+
+def test_calls_beyond_32_bits_are_refused():
+    with pytest.raises(ValueError, match="rows"):
+        q4.q4_linear(torch.zeros(1, 100).expand(2 ** 32 + 5, 100), weight())
+    c, one = cache(), torch.zeros(1, dtype=torch.int32)
+    table, k = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, 1, 2, 64)
+    q = torch.zeros(1, 1, 1, 64).expand(1, 1, 2 ** 32 + 4, 64)
+    with pytest.raises(ValueError, match="heads"):
+        q4.q4_attention(q, c, table, one, out=q)
+    with pytest.raises(ValueError, match="heads"):
+        q4.q4_kv_append(c, table, one, k, k, q=q, q_out=q)
