@@ -252,6 +252,9 @@ class Q4Cache:
         code, where, info = self._err.tolist()
         if code:
             self._err.zero_()
+            if code == N.EVS_ETIMEOUT:
+                raise N.EvsError(f"Q4Cache: a wait inside a kernel ran out at row {info}; what that call returned is not "
+                                 f"valid [evs status {code}, kernel {where}]")
             raise N.EvsError(f"Q4Cache: row {info} has a length outside its page table (or above max_length), "
                              f"or a page id outside the pool [evs status {code}, kernel {where}]")
 

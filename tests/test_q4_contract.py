@@ -8,6 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
+from evspark_b200 import _native as N
 from evspark_b200 import q4
 from tests.test_q4 import cache, weight
 
@@ -60,3 +61,17 @@ def test_calls_beyond_32_bits_are_refused():
         q4.q4_attention(q, c, table, one, out=q)
     with pytest.raises(ValueError, match="heads"):
         q4.q4_kv_append(c, table, one, k, k, q=q, q_out=q)
+
+
+def test_check_says_what_was_met(monkeypatch):
+    waited = []
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: waited.append(device))
+    c = cache()
+    c._err = torch.tensor([N.EVS_ETIMEOUT, 9, 3], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="wait.*row 3"):
+        c.check()
+    c._err = torch.tensor([N.EVS_ERANGE, 9, 5], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="row 5 has a length"):
+        c.check()
+    c.check()  # read once
+    assert waited == [c._index] * 3
