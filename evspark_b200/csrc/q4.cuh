@@ -7,8 +7,9 @@
 //   a NaN, an infinity or absmax / 7 > 2^120 in the group: s = NaN (the group reads back as NaN).
 // Why five bits: |c - 8| has three significant bits, so (c - 8) s has at most eight, a bf16's. The
 // decoded bf16 operands of a tensor-core product are then the held values themselves, with no
-// rounding between the codes and the product. A scale off by at most 1/64 costs less than the
-// codes' own rounding (absmax / s <= 7.11, and the clamp to 7 moves a value by at most 0.11 s).
+// rounding between the codes and the product. A scale off by at most 1/32 costs less than the
+// codes' own rounding (absmax / s <= 7 (1 + 1/32) < 7.22, reached just below and at the tie 1 + 1/32, and holding
+// such a value at 7 moves it by at most 0.22 s).
 //
 // Decoding two codes costs three instructions: a shift and a bitwise (w & mask) | 1.0 put the code
 // into the top mantissa bits of 1.0 (1 + c / 16), and one bf16x2 fma gives

@@ -50,9 +50,10 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], bool vec) {
 // Scale and codes of a group are decided in fp32 wherever that cannot differ from 64 bits, else in 64
 // bits.  Scale: t = absmax / 7 in fp32 is within 2^-22 of the exact quotient, so its five-bit rounding
 // is the exact one unless the dropped 19 bits lie within 4 units of a half (one group in 2^15).
-// Codes: the quotient x / s, corrected once by its exact remainder, is within 2^-23 of the exact one
-// (|x / s| < 7.12, so its rounding needs no clamp), and is a half exactly where x is; its rounding is
-// the exact one unless it lies within 2^-15 of a half.  Keys, rotated in 64 bits, are looked at again
+// Codes: the quotient x / s, corrected once by its remainder, is within 2^-21 of the exact one (half an
+// ulp at 4 .. 8 is 2^-22, and the correction is off by less than that); |x / s| <= 7 (1 + 1/32) < 7.5, so
+// its rounding needs no clamp.  It is a half exactly where x is, and its rounding is the exact one unless
+// it lies within 2^-15 of a half.  Keys, rotated in 64 bits, are looked at again
 // there.  Values are x themselves and may sit on a half.  Those of bf16 need no look at all: x = a 2^e
 // and s = b 2^f with a < 2^8 and b < 2^5, so a quotient above 0.49 that is not a half is at least
 // 1 / (2 max(b, a / 0.49)) > 2^-11 away from one.
