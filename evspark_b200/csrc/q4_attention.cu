@@ -448,7 +448,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
         }
       } else {
         const size_t prow =
-            ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tiles) * QA_ROWS) + R) * nslots + blockIdx.x;
+            ((static_cast<size_t>(b) * cache.G + kvh) * (static_cast<size_t>(tc) * grp) + R) * nslots + blockIdx.x;
         if (lane == 0) part_s[prow] = make_float2(big, sum);
 #pragma unroll
         for (int d = 0; d < DH; d += 32) {
@@ -646,9 +646,9 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   const bool tcore = sizeof(T) == 2 && DH == 128 && many && bound > QA_TC_BEGIN;
   const int nslots = tcore ? qa_tc_slots(bound) : qa_slots(bound);
   // tokens per pass: as many as the workspace holds partial results for
-  const int64_t per_tile = static_cast<int64_t>(r.B) * c.G * QA_ROWS * nslots * (DH + 2);
-  const int64_t fit = std::min<int64_t>(ws_floats / per_tile, 65535 / c.G);  // row tiles
-  int tokens = static_cast<int>(std::min<int64_t>(r.T, fit * QA_ROWS / grp));
+  const int64_t per_row = static_cast<int64_t>(r.B) * c.G * nslots * (DH + 2);
+  const int64_t fit = std::min<int64_t>(ws_floats / per_row, 65535 / c.G * QA_ROWS);  // rows a kv head
+  int tokens = static_cast<int>(std::min<int64_t>(r.T, fit / grp));
   EVS_CHECK_RANGE(tokens >= 1, "q4 attention: the workspace is too small");
   if (tokens < r.T && grp <= 128) {  // passes of the same length, in whole tiles of the tensor-core kernel
     const int passes = (r.T + tokens - 1) / tokens, tile = 128 / grp, even = (r.T + passes - 1) / passes;
@@ -656,7 +656,7 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   }
   for (int t0 = 0; t0 < r.T; t0 += tokens) {
     const int tc = std::min(tokens, r.T - t0);
-    const int prows = static_cast<int>(padded_rows(static_cast<int64_t>(tc) * grp)), tiles = prows / QA_ROWS;
+    const int prows = tc * grp, tiles = (prows + QA_ROWS - 1) / QA_ROWS;
     float* po = ws;
     float2* ps = reinterpret_cast<float2*>(ws + static_cast<int64_t>(r.B) * c.G * prows * nslots * DH);
     EVS_CUDA_TRY(evs_launch(kern, dim3(tcore ? qa_slots(QA_TC_BEGIN) : nslots, c.G * tiles, r.B),
@@ -697,13 +697,13 @@ int launch_q4_attention(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor&
 }
 
 int64_t q4_attention_ws(int B, int T, int G, int D, int H, int64_t bound) {
-  // every row in one pass where that takes at most 256 MiB, else as many as fit (a token at least)
+  // every row in one pass where that takes at most 256 MiB, else as many as fit (a token at least); tiles are
+  // whole, their partial results are those of the rows alone
   const int grp = H / G;
   if (fused_fits(qa_slots(bound), T, grp, G)) return 0;
   const int64_t per_row = static_cast<int64_t>(B) * G * qa_slots(bound) * (D + 2) * 4;
-  const int64_t all = padded_rows(static_cast<int64_t>(T) * grp), least = padded_rows(grp);
-  const int64_t fit = (256ll << 20) / per_row / QA_ROWS * QA_ROWS;
-  return std::min(all, std::max(least, fit)) * per_row;
+  const int64_t fit = (256ll << 20) / per_row;
+  return std::min(static_cast<int64_t>(T) * grp, std::max<int64_t>(grp, fit)) * per_row;
 }
 
 namespace {

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes as C
 import re
 from pathlib import Path
 
@@ -75,3 +76,13 @@ def test_check_says_what_was_met(monkeypatch):
         c.check()
     c.check()  # read once
     assert waited == [c._index] * 3
+
+
+def test_workspace_holds_the_rows_of_the_call_alone():
+    """One token of one query head a kv head: a row a head, not a tile of 16."""
+    d = N.Q4CacheDesc(256, None, 1 << 20, 64, 32, 128)
+    for batch, tokens, heads in ((64, 1, 32), (1, 13, 32), (3, 5, 96)):
+        r = N.Q4RowsDesc(256, 256, None, 2048, 2048, batch, tokens)
+        rows, slots = tokens * heads // 32, 2048 * 64 // 1024
+        need = N.lib().evs_q4_attention_workspace(C.byref(d), C.byref(r), heads, 0)
+        assert need == batch * 32 * rows * slots * (128 + 2) * 4
