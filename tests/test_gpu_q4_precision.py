@@ -76,3 +76,36 @@ def test_one_key_carries_the_weight_at_every_border(q4, start, rows):  # noqa: F
         out = check(q4, cache, table, q, kk, vv, start, D)
         # the other keys' weights are below e^-10 in sum
         assert float((out[0, :, 0].float() - vv[0, some, 0].float()).abs().max()) < 0.05
+
+
+@pytest.mark.parametrize("start,T,H,G,D,dtype", [(40, 5, 4, 2, 64, BF), (2500, 5, 4, 2, 64, F32), (5000, 40, 4, 2, 128, BF)])
+def test_output_inside_a_larger_tensor(q4, start, T, H, G, D, dtype):  # noqa: F811
+    """Rows at odd offsets, heads before tokens: the same bits, and nothing around them is written."""
+    cache, table = make_rows(q4, [start + T], 32, G, D)
+    fill_cache(q4, cache, table, [start], [start + T], G, D, dtype=dtype)
+    q = randn(1, T, H, D, seed=4, dtype=dtype)
+    want = q4.q4_attention(q, cache, table, i32([start]))
+    wide = torch.full((1, H + 2, T + 1, D + 5), 7.0, dtype=dtype, device=DEV)
+    out = wide[:, 1:H + 1, :T, 3:D + 3].transpose(1, 2)
+    assert q4.q4_attention(q, cache, table, i32([start]), out=out).data_ptr() == out.data_ptr()
+    assert torch.equal(out, want)
+    out.fill_(7.0)
+    assert bool((wide == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rotated_queries_and_read_back_inside_larger_tensors(q4, dtype):  # noqa: F811
+    D, G, H, T, start = 64, 2, 4, 9, 30
+    cache, table = make_rows(q4, [start + T], 16, G, D)
+    k, v, q = (randn(1, T, n, D, seed=s, dtype=dtype) for n, s in ((G, 1), (G, 2), (H, 3)))
+    want = q4.q4_kv_append(cache, table, i32([start]), k, v, q=q)
+    kk, vv = q4.q4_kv_read(cache, table, i32([start]), T, dtype=dtype)
+    wide = torch.full((3, 1, H + 1, T + 2, D + 3), 7.0, dtype=dtype, device=DEV)
+    q_out, k_out, v_out = (wide[i, :, 1:1 + n, 1:T + 1, 1:D + 1].transpose(1, 2) for i, n in enumerate((H, G, G)))
+    q4.q4_kv_append(cache, table, i32([start]), k, v, q=q, q_out=q_out)
+    q4.q4_kv_read(cache, table, i32([start]), T, out=(k_out, v_out))
+    assert torch.equal(q_out, want) and torch.equal(k_out, kk) and torch.equal(v_out, vv)
+    for t in (q_out, k_out, v_out):
+        t.fill_(7.0)
+    assert bool((wide == 7).all())
+    cache.check()
