@@ -9,12 +9,13 @@
 // steps agree bit for bit.  (Calls of more than 64 rows a kv head, and a model's prompts, leave positions from
 // 4,096 on to q4_attention_tc.cu, where a token's result does not depend on the others either.)  Short units give
 // few keys to many CTAs; from 131,072 keys on there are enough of them, and longer ones spare partial
-// results (440 us instead of 479 at 262,144 keys).
+// results (440 us instead of 479 at 262,144 keys, then).
 //
 // Keys and values are decoded in the registers that the products read them from, with no rounding
-// between codes and product.  What bounds it: about 1,070 warp instructions per 32 keys and row tile
-// (384 the decode, 96 products) at 12 warps an SM.  bf16, 32 heads of 128, 13 tokens: 145 us at 65,536 keys
-// (2.1 TB/s of codes and scales; floor 46 us), 477 us at 262,144 (2.5 TB/s).
+// between codes and product.  What it takes: 1,116 warp instructions per 32 keys and row tile (384 the
+// decode, 96 products), 0.52 issued a clock and scheduler: three warps a scheduler (168 registers) wait for their own
+// products, exponentials and loads.  bf16, 32 heads of 128, 13 tokens: 144 us at 65,536 keys (2.1 TB/s of codes and
+// scales; floor 46 us), 477 us at 262,144 (2.5 TB/s).
 #include <math_constants.h>
 
 #include <algorithm>
@@ -239,9 +240,9 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
       load_v(key);
       float s[NS][2][4];
 #pragma unroll
-        for (int sub = 0; sub < NS; ++sub)
+      for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) s[sub][u][0] = s[sub][u][1] = s[sub][u][2] = s[sub][u][3] = 0.f;
+        for (int u = 0; u < 2; ++u) s[sub][u][0] = s[sub][u][1] = s[sub][u][2] = s[sub][u][3] = 0.f;
       Q4Scale ks[NS][2];
 #pragma unroll
       for (int sub = 0; sub < NS; ++sub)
@@ -255,16 +256,16 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
 #pragma unroll
           for (int u = 0; u < 2; ++u) q4_word(kt.w[sub][u][w], ks[sub][u], kv[sub][u]);
 #pragma unroll
-          for (int p = NQ - 1; p >= 0; --p)
+        for (int p = NQ - 1; p >= 0; --p)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 a = qs[(p * 2 * KW + 2 * w + h) * 32 + lane];
+          for (int h = 0; h < 2; ++h) {
+            const uint4 a = qs[(p * 2 * KW + 2 * w + h) * 32 + lane];
 #pragma unroll
-              for (int sub = 0; sub < NS; ++sub)
+            for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                  q4_mma(s[sub][u], a.x, a.y, a.z, a.w, kv[sub][u][2 * h], kv[sub][u][2 * h + 1]);
-            }
+              for (int u = 0; u < 2; ++u)
+                q4_mma(s[sub][u], a.x, a.y, a.z, a.w, kv[sub][u][2 * h], kv[sub][u][2 * h + 1]);
+          }
       }
       const int next = key + QA_STEP;
       if (next < kend) {
@@ -279,12 +280,12 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
       const bool masked = key + QA_STEP > clear;
       if (masked) {  // thread's keys of a chunk are 4 c + 2 u + (0, 1)
 #pragma unroll
-          for (int sub = 0; sub < NS; ++sub)
+        for (int sub = 0; sub < NS; ++sub)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (key + 16 * sub + 4 * c + 2 * u + (e & 1) > lim[e >> 1]) s[sub][u][e] = -CUDART_INF_F;
+            for (int e = 0; e < 4; ++e)
+              if (key + 16 * sub + 4 * c + 2 * u + (e & 1) > lim[e >> 1]) s[sub][u][e] = -CUDART_INF_F;
       }
       float mx[2], a[2] = {1.f, 1.f};
 #pragma unroll
@@ -391,7 +392,7 @@ __device__ __forceinline__ void attn_tile(float* qa_sm, const Q4CacheDev& cache,
           for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                q4_mma(o[4 * n4 + j], pa[p][0], pa[p][1], pa[p][2], pa[p][3], b01[j], b23[j]);
+              q4_mma(o[4 * n4 + j], pa[p][0], pa[p][1], pa[p][2], pa[p][3], b01[j], b23[j]);
         }
       }
     }
@@ -639,10 +640,12 @@ int launch_attn(const Q4CacheDev& c, const Q4RowsDev& r, const Q4Tensor& q, cons
   const int smem = (qa_q_floats<T, DH>() + QA_WARPS * QA_ROWS * (DH + 2)) * 4;
   static std::atomic<unsigned long long> done{0};
   EVS_TRY(smem_attr_once(done, reinterpret_cast<const void*>(kern), smem));
-  // From 65 rows a kv head on the tensor-core kernel takes the long positions: it wins from 39 rows on (151 us
-  // instead of 183 at 32,768 keys, 32 kv heads; 26 rows: 257 instead of 242), but blocks of up to 64 tokens
-  // keep the sums of single steps.  A model says which kernel, as its rule must not depend on a call's tokens.
-  const bool many = longs == QaLong::BY_ROWS ? static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS : longs == QaLong::TENSOR_CORE;
+  // From 65 rows a kv head on the tensor-core kernel takes the long positions.  It wins from 17 rows, two of the
+  // other's tiles, on (65,536 keys, 32 kv heads: 245 us instead of 259 at 20 rows, 246 instead of 264 at 32, 266
+  // instead of 505 at 64, but 244 instead of 145 at 13), but blocks of up to 64 tokens keep the sums of single
+  // steps.  A model says which kernel, as its rule must not depend on a call's tokens.
+  const bool many =
+      longs == QaLong::BY_ROWS ? static_cast<int64_t>(r.T) * grp > QA_FEW_ROWS : longs == QaLong::TENSOR_CORE;
   const bool tcore = sizeof(T) == 2 && DH == 128 && many && bound > QA_TC_BEGIN;
   const int nslots = tcore ? qa_tc_slots(bound) : qa_slots(bound);
   // tokens per pass: as many as the workspace holds partial results for

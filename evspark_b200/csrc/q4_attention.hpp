@@ -15,8 +15,8 @@ __host__ __device__ constexpr int64_t qa_class_end(int cl) {
 __host__ __device__ constexpr int qa_cta_keys(int cl) { return cl == 0 ? 128 : (cl == 1 ? 256 : (cl == 2 ? 1024 : 4096)); }
 // Positions from QA_TC_BEGIN on are the tensor-core kernel's where the call has more than QA_FEW_ROWS rows (tokens
 // times query heads) a kv head.  It has classes of its own, with a slot of keys per CTA: with 2,048 keys instead
-// of 1,024, 16 rows of 13 tokens at up to 16,384 keys take 220 us instead of 196, but 1,024 tokens behind 32,768
-// keys (64 / 8 heads) 2,076 instead of 2,640.
+// of 1,024, 16 rows of 13 tokens at up to 16,384 keys took 220 us instead of 196, but 1,024 tokens behind 32,768
+// keys (64 / 8 heads) 2,076 instead of 2,640 (with probabilities in one bf16 part).
 constexpr int QA_FEW_ROWS = 64;
 constexpr int QA_TC_BEGIN = 4096;
 // Which kernel takes them: as the call's rows say, or one of the two whatever the rows.
@@ -46,9 +46,9 @@ inline int qa_tc_slots(int64_t bound) {
   return n;
 }
 
-// A row's sums are taken relative to 2^m; m moves up only when a score passes it by more than this (in
-// powers of two), as moving it costs a product per output. Sums in fp32 and probabilities in bf16 keep
-// their relative accuracy below 2^8.
+// Online softmax (Milakov and Gimelshein, 2018): a row's sums are taken relative to 2^m; m moves up only when a
+// score passes it by more than this (in powers of two), as moving it costs a product per output.  Sums in fp32 and
+// probabilities in two bf16 parts keep their relative accuracy below 2^8.
 constexpr float QA_SLACK = 8.f;
 
 // 2^x to two units in the last place, 0 below 2^-126

@@ -5,17 +5,19 @@
 // One CTA takes up to 128 query rows (a row is one token of one query head of the kv head) over its slot of
 // keys, 64 keys a step: S = Q K^T (128 x 64 x 128) and O += P V (128 x 128 x 64).  Four warps decode keys and
 // values into shared memory once for all rows; one warp issues whatever product is ready first; four warps run
-// the online softmax, one row a thread, with S, then P (two bf16 parts) in S's place, and O in tensor memory.  Two stages of
-// everything, so that a step's scores are there while the one before is still worked on; two CTAs an SM.
+// the online softmax, one row a thread, with S, then P (two bf16 parts) in S's place, and O in tensor memory.
+// Two stages of everything, so that a step's scores are there while the one before is still worked on; two CTAs
+// an SM.
 //
 // Measured beside the 16-row mma.sync kernel, which decodes the keys once per 16 rows: 16 rows of 13 tokens,
-// 64 / 8 heads, up to 16,384 keys 191 us instead of 304; 1,024 tokens, 32 heads, behind 16,384 keys 616
-// instead of 1,886; but 13 tokens of 32 heads at 65,536 keys 242 instead of 131: a step takes nearly the same
-// time for 1 row as for 128.  What bounds it: a step's 64 keys take about 1,700 clocks an SM, of which shared
-// memory (decoded operands stored once and read twice, the queries once a step) is busy for 770; a CTA's
-// decoding warps work 2,200 clocks on a step, its softmax warps 1,400, both at a third of the issue slots.
-// Tried and no faster: one CTA an SM with four stages and 8 or 16 decoding warps; the queries in tensor memory
-// with one stage of scores; a barrier each for decoded keys and values.
+// 64 / 8 heads, up to 16,384 keys 209 us instead of 332; 1,024 tokens, 32 heads, behind 16,384 keys 703
+// instead of 2,072; but 13 tokens of 32 heads at 65,536 keys 244 instead of 145: a step takes nearly the same
+// time for 1 row as for 128.  What it takes: a step's 64 keys about 1,900 clocks an SM, of which shared memory
+// (keys stored and read once, values stored once and read for both parts of the probabilities, the queries read
+// once a step) is busy for 900 and the tensor pipe for a third; 0.45 instructions issued a clock and scheduler, the
+// decoding warps (2,200 clocks a step) and the softmax warps waiting for barriers and tensor memory.
+// Tried and no faster (with one part): one CTA an SM with four stages and 8 or 16 decoding warps; the queries in
+// tensor memory with one stage of scores; a barrier each for decoded keys and values.
 #include <math_constants.h>
 
 #include <algorithm>

@@ -99,10 +99,13 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
 
 // Weight rows are the product's 16-row operand and tokens its 8-column one: a warp takes 32 rows x 128
 // features a step against every token of the tile, so the codes are decoded once, in the registers that
-// the product reads.  What bounds it is the decode's instructions and their latency: 420 warp
-// instructions per 4,096 codes (192 of them shifts, masks and fma of the decode), 0.44 issued a clock and
-// scheduler.  13 x 22016 x 4096, group 64: 20.0 us, 2.4 TB/s of codes and scales (floor 7.5 us at 6.5 TB/s);
-// 13 x 8192 x 22528: 34.1 us; 1 x 4096 x 4096: 6.4 us; 32 x 4096 x 4096: 12.4 us.
+// the product reads.  What it takes: 420 warp instructions per 4,096 codes (192 of them shifts,
+// masks and fma of the decode), 0.44 issued a clock and scheduler: 16 warps an SM wait for their codes, products and
+// decode.  13 x 22016 x 4096, group 64: 19.8 us, 2.4 TB/s of codes and scales (floor 7.5 us at 6.5 TB/s);
+// 13 x 8192 x 22528: 34.3 us; 1 x 4096 x 4096: 6.3 us (5.6 with the weight in L2); 32 x 4096 x 4096: 12.3 us.
+// bf16 rows add all product steps of a warp's K blocks to one fp32 accumulator, which the product cuts instead of
+// rounding: 6.7e-7 of the result at 13 x 8192 x 22528.  A sum of its own for each block, as fp32 rows have, brings
+// 1.0e-7 but costs 2 to 7 % at up to 16 tokens and 11 to 22 % beyond (its registers spill), so it is left out.
 // grid (K splits = cluster, row tiles, token tiles).  Registers hold the next two K blocks' codes
 // while one is multiplied; the first ones are on their way before x is staged.
 template <typename TX, typename TO, int NT, int KW>
@@ -318,7 +321,7 @@ int launch_linear_kw(const void* x, int64_t ldx, int M, const void* codes, const
   EVS_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<const TX*>(x), ldx, M, static_cast<const uint8_t*>(codes),
                                   static_cast<const uint16_t*>(scales), N, K, group == 32 ? 5 : (group == 64 ? 6 : 7),
                                   static_cast<TO*>(out), ldo, chunk, vec, wait_first ? 1 : 0,
-                                      static_cast<uint32_t>(red_offset)));
+                                  static_cast<uint32_t>(red_offset)));
   evs_count_launch(1);
   return EVS_OK;
 }
@@ -328,13 +331,15 @@ int launch_linear_nt(const void* x, int64_t ldx, int M, const void* codes, const
                      void* out, int64_t ldo, cudaStream_t st, bool pdl, bool wait_first) {
   const int KB = (K + Q4_KBLOCK - 1) / Q4_KBLOCK;
   // From N and K alone, so that a token's sums do not depend on the other tokens: 256 rows per CTA
-  // where that leaves enough CTAs, and as many splits of K as keep every cluster resident at once
-  // (two CTAs an SM; clusters of up to eight pack into about 264 of the 296 places).
+  // where that leaves enough CTAs (13 x N x 4096: 9.4 us instead of 10.1 with 128 at N = 7,168, 13.7 instead of
+  // 16.3 at 12,288, 19.8 instead of 29.9 at 22,016; but 9.5 instead of 9.3 at 6,144, 9.1 instead of 7.6 at 4,096 and
+  // 18.7 instead of 13.0 at 13 x 4096 x 11008), and as many splits of K as keep every cluster resident at once: two
+  // CTAs an SM, of whose 296 places clusters of up to eight fill 256 to 258 at the sizes above.
   const int KW = N >= 6400 ? 1 : 2;
   const int tiles = (N + 256 / KW - 1) / (256 / KW);
   const int S = std::max(1, std::min({LIN_CLUSTER, 264 / tiles, KB / KW}));
-  if (KW == 1) return launch_linear_kw<TX, TO, NT, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, S, st, pdl,
-      wait_first);
+  if (KW == 1)
+    return launch_linear_kw<TX, TO, NT, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, S, st, pdl, wait_first);
   return launch_linear_kw<TX, TO, NT, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, S, st, pdl, wait_first);
 }
 
@@ -344,7 +349,7 @@ int launch_linear_t(const void* x, int64_t ldx, int M, const void* codes, const 
   if (M <= 8) return launch_linear_nt<TX, TO, 1>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl, wait_first);
   if (M <= 16) return launch_linear_nt<TX, TO, 2>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl, wait_first);
   // tokens beyond one tile's read the weight again: tiles of 64 would leave one CTA an SM (64 tokens x 4096 x
-  // 4096 then take 35 us, and 64 x 8192 x 22528 145)
+  // 4096 then take 35 us, and 64 x 8192 x 22528 145, instead of 22 and 109)
   return launch_linear_nt<TX, TO, 4>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl, wait_first);
 }
 
@@ -430,7 +435,7 @@ int launch_q4_linear(const void* x, int x_dtype, int64_t ldx, int M, const void*
   if (x_dtype == EVS_DTYPE_BF16) {
     if (out_dtype == EVS_DTYPE_BF16)
       return launch_linear_t<__nv_bfloat16, __nv_bfloat16>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl,
-          wait_first);
+                                                           wait_first);
     return launch_linear_t<__nv_bfloat16, float>(x, ldx, M, codes, scales, N, K, group, out, ldo, st, pdl, wait_first);
   }
   if (out_dtype == EVS_DTYPE_BF16)

@@ -281,10 +281,11 @@ EVS_API int evs_q4_kv_read(const evs_q4_cache* cache, const evs_q4_rows* rows, v
  * q's dtype), already rotated; n_heads a multiple of kv_heads (query head h reads kv head
  * h / (n_heads / kv_heads)); out may be q itself but must not overlap it otherwise.  max_length >=
  * max(lengths + counts) bounds the launch (0: the whole table).  scale must be positive, at most 1e38.
- * workspace: device scratch of at least evs_q4_attention_workspace bytes (0 for short contexts, -1 for arguments that are refused), one per call in flight.  A token's
- * result depends on its position, its q and the keys it sees alone: not on the batch, the other tokens,
- * max_length, the page size or the workspace. One size matters: from position 4,096 on, calls of more
- * than 64 rows (tokens * n_heads / kv_heads; bf16, D = 128) sum in another order than smaller ones. */
+ * workspace: device scratch of at least evs_q4_attention_workspace bytes (0 for short contexts, -1 for
+ * arguments that are refused), one per call in flight.  A token's result depends on its position, its q
+ * and the keys it sees alone: not on the batch, the other tokens, max_length, the page size or the
+ * workspace.  One size matters: from position 4,096 on, calls of more than 64 rows (tokens * n_heads /
+ * kv_heads; bf16, D = 128) sum in another order than smaller ones. */
 EVS_API int64_t evs_q4_attention_workspace(const evs_q4_cache* cache, const evs_q4_rows* rows, int n_heads,
                                            int max_length);
 EVS_API int evs_q4_attention(const evs_q4_cache* cache, const evs_q4_rows* rows, const void* q, const int64_t* q_strides,
