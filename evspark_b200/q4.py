@@ -82,10 +82,24 @@ def padded_features(k: int) -> int:
     return -(-k // KBLOCK) * KBLOCK
 
 
-class Q4Weight:
+class _Fixed:
+    """Objects whose calls keep the addresses of their tensors: what those belong to cannot be replaced."""
+
+    _FIXED = frozenset()
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and "_index" in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}: {name} cannot be replaced, its address is kept; "
+                                 f"write into it or make a new {type(self).__name__}")
+        super().__setattr__(name, value)
+
+
+class Q4Weight(_Fixed):
     """A weight [N, K] held in 4 bits: ``codes`` uint8 [N, Kp / 2] (two input features per byte, the even
     one in the low half, Kp = K rounded up to 128 with codes of 8 behind K), ``scales`` bf16
     [Kp / group, N]."""
+
+    _FIXED = frozenset(("codes", "scales", "shape", "group"))
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int], group: int):
         n, k = int(shape[0]), int(shape[1])
@@ -188,7 +202,7 @@ def q4_linear(x: torch.Tensor, w: Q4Weight, *, out_dtype: torch.dtype = torch.fl
     return out
 
 
-class Q4Cache:
+class Q4Cache(_Fixed):
     """A pool of KV pages in 4 bits, shared by any number of rows and layers' worth of page tables.
 
     ``pool`` uint8 [num_pages, kv_heads, block]: per page and head K codes [P, D / 2], V codes [P, D / 2],
@@ -197,6 +211,8 @@ class Q4Cache:
 
     Calls that meet a length outside the page table or a page id outside the pool skip that row (its
     attention result is NaN) and note it on the device; ``check`` reads the note and raises."""
+
+    _FIXED = frozenset(("pool", "num_pages", "kv_heads", "head_dim", "page_size"))
 
     def __init__(self, num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64, device="cuda:0"):
         self._init(None, num_pages, kv_heads, head_dim, page_size, torch.device(device))

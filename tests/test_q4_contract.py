@@ -86,3 +86,17 @@ def test_workspace_holds_the_rows_of_the_call_alone():
         rows, slots = tokens * heads // 32, 2048 * 64 // 1024
         need = N.lib().evs_q4_attention_workspace(C.byref(d), C.byref(r), heads, 0)
         assert need == batch * 32 * rows * slots * (128 + 2) * 4
+
+
+def test_tensors_whose_addresses_are_kept_cannot_be_replaced():
+    """A replaced tensor would be freed while calls go on reading its memory."""
+    w, c = weight(), cache()
+    for obj, names in ((w, ("codes", "scales")), (c, ("pool",))):
+        for name in names:
+            before = getattr(obj, name)
+            with pytest.raises(AttributeError, match="replaced"):
+                setattr(obj, name, before.clone())
+            assert getattr(obj, name) is before
+    for obj, name in ((w, "shape"), (w, "group"), (c, "page_size"), (c, "head_dim"), (c, "num_pages"), (c, "kv_heads")):
+        with pytest.raises(AttributeError, match="replaced"):
+            setattr(obj, name, 32)
